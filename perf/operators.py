@@ -445,7 +445,9 @@ def _plain_sample(s):
     k = torch.where(greedy, 1.0, k)
     cum = w.cumsum(1)
     mass = cum.gather(1, k.clamp(max=n).long()[:, None] - 1)
-    keep = (j < k[:, None]) & ((cum - w < full(s["top_p"], 1.0)[:, None] * mass) | (j == 0))
+    p = full(s["top_p"], 1.0)
+    p = torch.where(p < 1, p, math.inf)  # from 1 on: no such filter
+    keep = (j < k[:, None]) & ((cum - w < p[:, None] * mass) | (j == 0))
     keep &= (w >= full(s["min_p"], 0.0)[:, None]) & (w > 0) | (j == 0)
     kept = keep.long().cumprod(1).sum(1)
     mass = cum.gather(1, kept[:, None] - 1)
@@ -535,7 +537,8 @@ def _exact_sample(s):
         p = torch.softmax(x / t, 0)[ids][:k if k > 0 else None]
         p = p / p.sum()
         before = torch.cat([p.new_zeros(1), p.cumsum(0)[:-1]])
-        keep = (before < value(host["top_p"], r, 1.0)) & (p >= value(host["min_p"], r, 0.0) * p[0]) & (p > 0)
+        most = value(host["top_p"], r, 1.0)
+        keep = (before < (most if most < 1 else math.inf)) & (p >= value(host["min_p"], r, 0.0) * p[0]) & (p > 0)
         keep[0] = True
         p = p[keep] / p[keep].sum()
         got.append(float(p[min(int((p.cumsum(0) <= float(host["uniform"][r])).sum()), len(p) - 1)].log()))
