@@ -387,6 +387,32 @@ mx_status mx_head_argmax_mfma(const mx_qweight* w, const uint16_t* x, int32_t m,
 mx_status mx_argmax_bf16(const uint16_t* logits, int32_t rows, int32_t n, uint32_t* tokens,
                          void* stream);
 
+/* mx_sample_bf16: tokens[r] drawn from bf16 logits [rows, n] (rows `stride`
+ * elements apart, any alignment) with a given uniform number, beside
+ * mx_argmax_bf16's greedy choice.  Tokens are ordered by logit (largest first,
+ * lowest id on ties), w_j = exp((l_j - l_0) / temperature[r]); of the first
+ * top_k[r] tokens the shortest prefix with at least top_p[r] of their mass is
+ * kept, of that the tokens with w_j >= min_p[r]; token 0 of the order always
+ * is.  The token is the first whose prefix mass exceeds uniform[r] times the
+ * kept mass.  Counts are exact and masses 64-bit sums, so a row's token
+ * depends on its own inputs only, bit for bit.
+ * All per-row arrays are on the device.  NULL, or: temperature NULL = 1, <= 0
+ * or NaN = greedy; top_k NULL or <= 0 = off; top_p NULL, >= 1 or NaN = off, <= 0
+ * keeps one token; min_p NULL, <= 0 or NaN = off.  uniform is cut to [0, 1],
+ * NaN counts as 0.  Logits of -inf (and NaN) and weights below the smallest
+ * double are never kept; +inf logits share the whole mass; a row in which
+ * nothing exceeds -inf gives token 0, kept 0 and logprob -inf.  logprob
+ * (optional): log of the token's share of the kept mass, fp32; kept
+ * (optional): the number of tokens kept.  n <= 1048576.  workspace:
+ * mx_sample_workspace_bytes(rows, n) bytes (0 bytes: NULL will do), 16-byte
+ * aligned, one call at a time.  No reference counterpart (its server decodes
+ * greedily). */
+size_t mx_sample_workspace_bytes(int32_t rows, int32_t n);
+mx_status mx_sample_bf16(const uint16_t* logits, int64_t stride, int32_t rows, int32_t n,
+                         const float* temperature, const int32_t* top_k, const float* top_p,
+                         const float* min_p, const float* uniform, uint32_t* tokens,
+                         float* logprob, int32_t* kept, void* workspace, void* stream);
+
 /* ---- A10/A11/A12: GatedDeltaNet -------------------------------------------
  * Rows are `groups` sequences of `t` consecutive tokens (row = g*t + i);
  * slots[g] (device int32) selects the group's cached conv window and state.
@@ -459,6 +485,108 @@ mx_status mx_attn_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_str
                          const int32_t* slots, const int32_t* pos, const uint16_t* k_cache,
                          const uint16_t* v_cache, const mx_attn_dims* dims, int32_t flags,
                          void* workspace, uint16_t* out, void* stream);
+
+/* ---- the paged cache ----------------------------------------------------------
+ * A KV cache in pages of page_size positions that sequences share by need, in
+ * place of one range of max_ctx positions per slot: what writes it, and
+ * attention of single tokens and of prompts over it.  No reference counterpart
+ * (its KvCache is one growing array per request, src/dense.rs:46-110).
+ *
+ * Layout, elements of dtype (MX_DT_BF16, or MX_DT_F8E4M3: one byte, the value
+ * is the stored number times its kv head's scale), page_stride elements from
+ * page to page:
+ *   k_cache  [pages][kv_heads][page_size][head_dim]
+ *   v_cache  [pages][kv_heads][head_dim][page_size]   (transposed)
+ * table: int32 [sequences][table_width], the pages of each sequence in order:
+ * position p of sequence s lies at p % page_size of page
+ * table[s][p / page_size].  An entry outside [0, pages) holds no positions:
+ * appends to it write nothing, attention leaves its positions out.  Sequences
+ * may share pages (a common prefix); what no sequence's length covers may hold
+ * anything, NaN too.  The values of positions that a length covers must be
+ * finite.
+ *
+ * head_dim 64, 128 or 256; 1..16 q heads per kv head; page_size 16, 32, 64, 128
+ * or 256 (MX_EUNSUPPORTED otherwise).  q, qkv rows (qkv_stride % 8 == 0), out,
+ * workspaces and both caches are 16-byte aligned.  The pointers and the stream belong
+ * to the current device.  A workspace serves one call at a time: calls that
+ * may overlap (two streams, two captured graphs) need one each. */
+typedef struct mx_page_dims {
+  int32_t heads;        /* q heads */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t pages;
+  int32_t sequences;    /* rows of the page table */
+  int32_t table_width;  /* entries of a row of the page table */
+  int32_t dtype;        /* MX_DT_BF16 or MX_DT_F8E4M3 */
+  int32_t gated;        /* 1: qkv rows hold [heads][q | gate], outputs are gated; 0: [heads][q] */
+  int64_t page_stride;  /* >= kv_heads * page_size * head_dim, a multiple of 16 */
+} mx_page_dims;
+/* Rotary positions: pair i of the first rotary_dim values is (i, i +
+ * rotary_dim / 2) and turns by rope_pos[pair_axis[i]][row] * inv_freq[i], so
+ * text uses one axis and pictures or video several (time, height, width) in
+ * any order of pairs.  inv_freq: device fp64 [rotary_dim / 2]. */
+typedef struct mx_rope_axes {
+  int32_t rotary_dim;  /* even, 0 (no rotation) .. head_dim */
+  int32_t axes;        /* 1..4 */
+  const double* inv_freq;
+  uint8_t pair_axis[128];
+} mx_rope_axes;
+/* mx_attn_paged_append: takes projected rows qkv [rows][heads (q, or q | gate)
+ * | kv_heads k | kv_heads v][head_dim] to q_out bf16 [rows, heads, head_dim] and
+ * into the cache: q and k heads RMS-normalised (x rsqrt(mean x^2 + eps)
+ * (norm + 1); a NULL norm leaves them as they are) and rotated, in fp32 with
+ * one rounding; v as it is.  Row r is position pos[r] of sequence seqs[r]
+ * (seqs NULL: sequence r).  An e4m3 cache takes round(clamp(value / scale,
+ * +-448)); k_scale / v_scale: device fp32 [kv_heads], NULL for 1 (and ignored
+ * for bf16).  rope_pos: int32 [axes][rows].  A row whose sequence is not in
+ * [0, sequences) is padding: nothing of it is written; a position outside the
+ * table writes q_out only.  Rows must not name the same position twice.
+ * Replaces, for paged caches, the norms, RoPE and KvCache::update of
+ * Attention::forward_selection (src/dense.rs:139-270, 46-110). */
+mx_status mx_attn_paged_append(const uint16_t* qkv, int64_t qkv_stride, int32_t rows,
+                               const int32_t* seqs, const int32_t* pos, const int32_t* rope_pos,
+                               const mx_rope_axes* rope, const uint16_t* q_norm,
+                               const uint16_t* k_norm, float eps, const int32_t* table,
+                               const mx_page_dims* dims, const float* k_scale,
+                               const float* v_scale, uint16_t* q_out, void* k_cache, void* v_cache,
+                               void* stream);
+/* mx_attn_paged_decode: attention of one token a row, q bf16 [rows, heads,
+ * head_dim], over positions 0 .. lens[r] - 1 of its sequence (seqs[r], or r):
+ *   out[r, h] = bf16(softmax(q k^T scale) v [* sigmoid(gate[r, h])])
+ * with scale 0 meaning 1 / sqrt(head_dim), and for gated caches gate[r, h] =
+ * qkv[r * qkv_stride + h * 2 * head_dim + head_dim ..] (qkv NULL otherwise).  A
+ * row without positions (lens[r] <= 0, or none in a page) gives zeros; a row
+ * whose sequence is not in [0, sequences) is padding and keeps its out.
+ * Lengths past the table are cut to it.  Matrix-core sums in fp32; the result
+ * depends on the lengths of all rows (the keys' split follows them) to within
+ * those sums' rounding, and is the same for the same inputs.  workspace:
+ * mx_attn_paged_decode_workspace_bytes(rows, dims) bytes.  The paged form of
+ * mx_attn_decode. */
+size_t mx_attn_paged_decode_workspace_bytes(int32_t rows, const mx_page_dims* dims);
+mx_status mx_attn_paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride,
+                               int32_t rows, const int32_t* seqs, const int32_t* lens,
+                               const int32_t* table, const void* k_cache, const void* v_cache,
+                               const float* k_scale, const float* v_scale,
+                               const mx_page_dims* dims, float scale, void* workspace,
+                               uint16_t* out, void* stream);
+/* mx_attn_paged_prefill: causal attention of packed sequences.  Rows starts[s]
+ * .. starts[s + 1] - 1 of q (starts: int32 [sequences + 1], not decreasing, up
+ * to `rows`) are the last positions of sequence s, whose lens[s] positions are
+ * in the cache already (this call's and any cached prefix): row starts[s] + i
+ * sits at position lens[s] - (starts[s + 1] - starts[s]) + i and sees the
+ * positions up to its own.  Rows before position 0 see none and give zeros;
+ * rows outside every sequence keep their out.  P is rounded to bf16 for the
+ * second product.  Otherwise as mx_attn_paged_decode; workspace:
+ * mx_attn_paged_prefill_workspace_bytes(rows, dims) bytes (0 bytes: NULL will
+ * do).  The packed and paged form of mx_attn_decode's prefill form. */
+size_t mx_attn_paged_prefill_workspace_bytes(int32_t rows, const mx_page_dims* dims);
+mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride,
+                                int32_t rows, const int32_t* starts, const int32_t* lens,
+                                const int32_t* table, const void* k_cache, const void* v_cache,
+                                const float* k_scale, const float* v_scale,
+                                const mx_page_dims* dims, float scale, void* workspace,
+                                uint16_t* out, void* stream);
 
 /* mx_gdn_recurrence_fast: mx_gdn_recurrence's contract (groups of t tokens,
  * optional per-token history) with the matrix-core engine's fast-mode
@@ -629,6 +757,7 @@ mx_status mx_engine_tensor(mx_engine* e, const char* name, void** device_ptr, si
 #define MX_DT_BF16 1
 #define MX_DT_F16 2
 #define MX_DT_F32 3
+#define MX_DT_F8E4M3 4 /* paged caches only */
 /* Writes one checkpoint tensor, named as in an MLX checkpoint of the hybrid
  * model (the names Weights / HybridModel::load / Mtp::load read:
  * src/weights.rs:22-99, src/hybrid.rs:56-66, 130-142, 335-352, 529-567,

@@ -68,6 +68,17 @@ class AttnDimsC(C.Structure):
                 ("max_ctx", C.c_int32), ("slot_stride", C.c_int64)]
 
 
+class PageDimsC(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("heads", "kv_heads", "head_dim", "page_size", "pages",
+                                         "sequences", "table_width", "dtype", "gated")] + [
+        ("page_stride", C.c_int64)]
+
+
+class RopeAxesC(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("axes", C.c_int32), ("inv_freq", C.c_void_p),
+                ("pair_axis", C.c_uint8 * 128)]
+
+
 MAX_LAYERS = 128  # MX_MAX_LAYERS
 
 
@@ -190,6 +201,16 @@ def _load() -> C.CDLL:
         "mx_attn_workspace_bytes": ([i32, i32, i32, i32], sz),
         "mx_attn_decode": ([vp, vp, i64, i32, vp, vp, vp, vp, C.POINTER(AttnDimsC), i32, vp, vp,
                             vp], i32),
+        "mx_attn_paged_append": ([vp, i64, i32, vp, vp, vp, C.POINTER(RopeAxesC), vp, vp, f32, vp,
+                                  C.POINTER(PageDimsC), vp, vp, vp, vp, vp, vp], i32),
+        "mx_attn_paged_decode_workspace_bytes": ([i32, C.POINTER(PageDimsC)], sz),
+        "mx_attn_paged_decode": ([vp, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp,
+                                  C.POINTER(PageDimsC), f32, vp, vp, vp], i32),
+        "mx_attn_paged_prefill_workspace_bytes": ([i32, C.POINTER(PageDimsC)], sz),
+        "mx_attn_paged_prefill": ([vp, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp,
+                                   C.POINTER(PageDimsC), f32, vp, vp, vp], i32),
+        "mx_sample_workspace_bytes": ([i32, i32], sz),
+        "mx_sample_bf16": ([vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp], i32),
         "mx_engine_create": ([C.POINTER(ModelConfigC), C.POINTER(vp)], i32),
         "mx_engine_destroy": ([vp], i32),
         "mx_engine_reset_slot": ([vp, i32], i32),
@@ -399,7 +420,7 @@ def sync() -> None:
 
 
 # ---- model configurations (benchmark configs 3 and 4, and a tiny test model) ----
-MX_DT_U32, MX_DT_BF16, MX_DT_F16, MX_DT_F32 = 0, 1, 2, 3
+MX_DT_U32, MX_DT_BF16, MX_DT_F16, MX_DT_F32, MX_DT_F8E4M3 = 0, 1, 2, 3, 4
 
 CONFIG3 = dict(hidden=2048, layers=48, attn_every=4, vocab=151936, hc=4, hc_rank=256, gdn_hk=16,
                gdn_hv=32, gdn_dk=128, gdn_dv=128, conv_k=4, heads=16, kv_heads=2, head_dim=256,

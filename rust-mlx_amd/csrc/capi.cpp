@@ -349,6 +349,27 @@ MX_ABI mx_status mx_argmax_bf16(const uint16_t* logits, int32_t rows, int32_t n,
   return finish(argmax_bf16(logits, rows, n, tokens, hipStream_t(stream)), "mx_argmax_bf16");
 }
 
+MX_ABI size_t mx_sample_workspace_bytes(int32_t rows, int32_t n) {
+  return rows > 0 && n > 0 && n <= kSampleMaxVocab ? sample_workspace(rows, n) : 0;
+}
+
+MX_ABI mx_status mx_sample_bf16(const uint16_t* logits, int64_t stride, int32_t rows, int32_t n,
+                                const float* temperature, const int32_t* top_k,
+                                const float* top_p, const float* min_p, const float* uniform,
+                                uint32_t* tokens, float* logprob, int32_t* kept, void* workspace,
+                                void* stream) {
+  MX_CHECK(rows >= 0 && n > 0 && stride >= n, MX_EINVAL, "mx_sample_bf16: bad shape");
+  MX_CHECK(n <= kSampleMaxVocab, MX_EUNSUPPORTED, "mx_sample_bf16: at most 1048576 logits a row");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(logits && uniform && tokens && (workspace || sample_workspace(rows, n) == 0), MX_EINVAL,
+           "mx_sample_bf16: null pointer");
+  MX_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, MX_EUNSUPPORTED,
+           "mx_sample_bf16: the workspace must be 16-byte aligned");
+  return finish(sample_bf16(logits, stride, rows, n, temperature, top_k, top_p, min_p, uniform,
+                            tokens, logprob, kept, workspace, hipStream_t(stream)),
+                "mx_sample_bf16");
+}
+
 // ---- GatedDeltaNet --------------------------------------------------------
 MX_ABI mx_status mx_gdn_conv(const uint16_t* qkv, int64_t row_stride, int32_t groups, int32_t t,
                              const int32_t* slots, uint16_t* conv_state, const float* conv_w,
@@ -514,6 +535,170 @@ MX_ABI mx_status mx_attn_decode(const uint16_t* q, const uint16_t* qkv, int64_t 
   if (rc == MX_OK)
     rc = attn_combine(o_part, ml_part, qkv, qkv_stride, rows, pos, d, chunks, fast, out, s);
   return finish(rc, "mx_attn_decode");
+}
+
+// ---- the paged cache ----------------------------------------------------------
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Checks a cache's description and takes it over; nullptr when it is good, else
+// what is wrong with it (*code: the status).
+const char* check_pages(const mx_page_dims* dims, PageDims* d, int* code) {
+  *code = MX_EINVAL;
+  if (!dims) return "null dims";
+  if (dims->heads <= 0 || dims->kv_heads <= 0 || dims->heads % dims->kv_heads != 0)
+    return "heads must be a positive multiple of kv_heads";
+  if (dims->pages <= 0 || dims->sequences <= 0 || dims->table_width <= 0)
+    return "pages, sequences and table_width must be positive";
+  if (dims->gated != 0 && dims->gated != 1) return "gated must be 0 or 1";
+  *code = MX_EUNSUPPORTED;
+  if (dims->head_dim != 64 && dims->head_dim != 128 && dims->head_dim != 256)
+    return "head_dim must be 64, 128 or 256";
+  if (dims->heads / dims->kv_heads > 16) return "at most 16 q heads per kv head";
+  if (dims->heads > 65536) return "at most 65536 heads";
+  int log2 = 4;
+  while (log2 < 8 && (1 << log2) != dims->page_size) ++log2;
+  if ((1 << log2) != dims->page_size) return "page_size must be 16, 32, 64, 128 or 256";
+  if (dims->dtype != MX_DT_BF16 && dims->dtype != MX_DT_F8E4M3)
+    return "dtype must be MX_DT_BF16 or MX_DT_F8E4M3";
+  if ((int64_t(dims->table_width) << log2) > 0x7fffffff)
+    return "table_width * page_size must stay below 2^31";
+  *code = MX_EINVAL;
+  if (dims->page_stride < int64_t(dims->kv_heads) * dims->page_size * dims->head_dim ||
+      dims->page_stride % 16 != 0)
+    return "page_stride must cover a page and be a multiple of 16";
+  if (dims->page_stride > (int64_t(1) << 60) / dims->pages) return "cache too large";
+  *d = PageDims{dims->heads,     dims->kv_heads,    dims->head_dim,
+                log2,            dims->pages,       dims->sequences,
+                dims->table_width, dims->dtype == MX_DT_F8E4M3, dims->gated != 0,
+                dims->page_stride};
+  return nullptr;
+}
+
+// What the two attentions over pages check alike.
+mx_status check_paged_attention(const char* what, const mx_page_dims* dims, PageDims* d,
+                                const void* q, const uint16_t* qkv, int64_t qkv_stride,
+                                const void* k, const void* v, float scale, float* used_scale) {
+  int code = 0;
+  if (const char* err = check_pages(dims, d, &code))
+    return mx_status(set_error(code, std::string(what) + ": " + err));
+  if (d->gated && (!qkv || qkv_stride < int64_t(2) * d->heads * d->head_dim))
+    return mx_status(set_error(MX_EINVAL, std::string(what) + ": a gated cache needs qkv rows"));
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) ||
+      (d->gated && (!aligned16(qkv) || qkv_stride % 8 != 0)))
+    return mx_status(set_error(MX_EUNSUPPORTED,
+                               std::string(what) + ": q, qkv rows and the cache must be 16-byte aligned"));
+  if (!(scale >= 0.0f && scale < 1e30f))
+    return mx_status(set_error(MX_EINVAL, std::string(what) + ": scale must be finite and not negative"));
+  *used_scale = scale > 0.0f ? scale : 1.0f / __builtin_sqrtf(float(d->head_dim));
+  return MX_OK;
+}
+
+}  // namespace
+
+MX_ABI mx_status mx_attn_paged_append(const uint16_t* qkv, int64_t qkv_stride, int32_t rows,
+                                      const int32_t* seqs, const int32_t* pos,
+                                      const int32_t* rope_pos, const mx_rope_axes* rope,
+                                      const uint16_t* q_norm, const uint16_t* k_norm, float eps,
+                                      const int32_t* table, const mx_page_dims* dims,
+                                      const float* k_scale, const float* v_scale, uint16_t* q_out,
+                                      void* k_cache, void* v_cache, void* stream) {
+  const char* what = "mx_attn_paged_append";
+  PageDims d;
+  int code = 0;
+  if (const char* err = check_pages(dims, &d, &code))
+    return mx_status(set_error(code, std::string(what) + ": " + err));
+  MX_CHECK(rows >= 0, MX_EINVAL, "mx_attn_paged_append: negative rows");
+  MX_CHECK(rope != nullptr, MX_EINVAL, "mx_attn_paged_append: null rope");
+  MX_CHECK(rope->rotary_dim >= 0 && rope->rotary_dim % 2 == 0 && rope->rotary_dim <= d.head_dim &&
+               rope->axes >= 1 && rope->axes <= 4,
+           MX_EINVAL, "mx_attn_paged_append: rotary_dim must be even and within head_dim, axes 1..4");
+  RopeAxes r{rope->rotary_dim, rope->axes, rope->inv_freq, {}};
+  for (int i = 0; i < rope->rotary_dim / 2; ++i) {
+    MX_CHECK(rope->pair_axis[i] < rope->axes, MX_EINVAL,
+             "mx_attn_paged_append: pair_axis names an axis that is not there");
+    r.pair_axis[i] = rope->pair_axis[i];
+  }
+  MX_CHECK(eps >= 0.0f, MX_EINVAL, "mx_attn_paged_append: eps must not be negative");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(qkv && pos && table && q_out && k_cache && v_cache &&
+               (rope->rotary_dim == 0 || (rope_pos && rope->inv_freq)),
+           MX_EINVAL, "mx_attn_paged_append: null pointer");
+  const int64_t width =
+      (int64_t(d.heads) * (d.gated ? 2 : 1) + 2 * int64_t(d.kv_heads)) * d.head_dim;
+  MX_CHECK(qkv_stride >= width, MX_EINVAL, "mx_attn_paged_append: qkv_stride shorter than a row");
+  MX_CHECK(aligned16(qkv) && qkv_stride % 8 == 0 && aligned16(q_out) && aligned16(k_cache) &&
+               aligned16(v_cache),
+           MX_EUNSUPPORTED,
+           "mx_attn_paged_append: qkv rows, q_out and the cache must be 16-byte aligned");
+  return finish(paged_append(qkv, qkv_stride, rows, seqs, pos, rope_pos, r, q_norm, k_norm, eps,
+                             table, d, k_scale, v_scale, q_out, k_cache, v_cache,
+                             hipStream_t(stream)),
+                what);
+}
+
+MX_ABI size_t mx_attn_paged_decode_workspace_bytes(int32_t rows, const mx_page_dims* dims) {
+  PageDims d;
+  int code = 0;
+  if (rows <= 0 || check_pages(dims, &d, &code)) return 0;
+  return paged_decode_workspace(rows, d);
+}
+
+MX_ABI mx_status mx_attn_paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride,
+                                      int32_t rows, const int32_t* seqs, const int32_t* lens,
+                                      const int32_t* table, const void* k_cache,
+                                      const void* v_cache, const float* k_scale,
+                                      const float* v_scale, const mx_page_dims* dims, float scale,
+                                      void* workspace, uint16_t* out, void* stream) {
+  const char* what = "mx_attn_paged_decode";
+  PageDims d;
+  float sc = 0.0f;
+  if (const mx_status rc = check_paged_attention(what, dims, &d, q, qkv, qkv_stride, k_cache,
+                                                 v_cache, scale, &sc);
+      rc != MX_OK)
+    return rc;
+  MX_CHECK(rows >= 0, MX_EINVAL, "mx_attn_paged_decode: negative rows");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(q && lens && table && k_cache && v_cache && workspace && out, MX_EINVAL,
+           "mx_attn_paged_decode: null pointer");
+  MX_CHECK(aligned16(workspace), MX_EUNSUPPORTED,
+           "mx_attn_paged_decode: the workspace must be 16-byte aligned");
+  return finish(paged_decode(q, qkv, qkv_stride, rows, seqs, lens, table, k_cache, v_cache,
+                             k_scale, v_scale, d, sc, workspace, out, hipStream_t(stream)),
+                what);
+}
+
+MX_ABI size_t mx_attn_paged_prefill_workspace_bytes(int32_t rows, const mx_page_dims* dims) {
+  PageDims d;
+  int code = 0;
+  if (rows <= 0 || check_pages(dims, &d, &code)) return 0;
+  return paged_prefill_workspace(rows, d);
+}
+
+MX_ABI mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride,
+                                       int32_t rows, const int32_t* starts, const int32_t* lens,
+                                       const int32_t* table, const void* k_cache,
+                                       const void* v_cache, const float* k_scale,
+                                       const float* v_scale, const mx_page_dims* dims, float scale,
+                                       void* workspace, uint16_t* out, void* stream) {
+  const char* what = "mx_attn_paged_prefill";
+  PageDims d;
+  float sc = 0.0f;
+  if (const mx_status rc = check_paged_attention(what, dims, &d, q, qkv, qkv_stride, k_cache,
+                                                 v_cache, scale, &sc);
+      rc != MX_OK)
+    return rc;
+  MX_CHECK(rows >= 0, MX_EINVAL, "mx_attn_paged_prefill: negative rows");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(q && starts && lens && table && k_cache && v_cache && out &&
+               (workspace || paged_prefill_workspace(rows, d) == 0),
+           MX_EINVAL, "mx_attn_paged_prefill: null pointer");
+  MX_CHECK(aligned16(workspace) && aligned16(out), MX_EUNSUPPORTED,
+           "mx_attn_paged_prefill: the workspace and out must be 16-byte aligned");
+  return finish(paged_prefill(q, qkv, qkv_stride, rows, starts, lens, table, k_cache, v_cache,
+                              k_scale, v_scale, d, sc, workspace, out, hipStream_t(stream)),
+                what);
 }
 
 // ---- engine ---------------------------------------------------------------

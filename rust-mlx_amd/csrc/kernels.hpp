@@ -208,6 +208,39 @@ int attn_combine_splits(const float* o_part, const float* ml_part, const uint16_
                         int max_chunks, uint16_t* out, hipStream_t s);
 constexpr int kAttnRows = 128;  // query rows per attention launch of a prefill chunk
 
+// ---- the paged cache (paged.hip, paged_prefill.hip) ----
+struct PageDims {
+  int heads, kv_heads, head_dim;
+  int page_log2;      // positions per page: 16 .. 256
+  int pages;          // pages of the cache
+  int sequences;      // rows of the page table
+  int table_width;    // entries of a row of the page table
+  bool f8, gated;     // e4m3 cache; qkv rows hold [q | gate] per head
+  int64_t page_stride;  // elements between pages
+};
+struct RopeAxes {
+  int rotary_dim, axes;
+  const double* inv_freq;
+  uint8_t pair_axis[128];
+};
+int paged_append(const uint16_t* qkv, int64_t qkv_stride, int rows, const int32_t* seqs,
+                 const int32_t* pos, const int32_t* rope_pos, const RopeAxes& rope,
+                 const uint16_t* q_norm, const uint16_t* k_norm, float eps, const int32_t* table,
+                 const PageDims& d, const float* k_scale, const float* v_scale, uint16_t* q_out,
+                 void* k_cache, void* v_cache, hipStream_t s);
+size_t paged_decode_workspace(int rows, const PageDims& d);
+int paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int rows,
+                 const int32_t* seqs, const int32_t* lens, const int32_t* table,
+                 const void* k_cache, const void* v_cache, const float* k_scale,
+                 const float* v_scale, const PageDims& d, float scale, void* workspace,
+                 uint16_t* out, hipStream_t s);
+size_t paged_prefill_workspace(int rows, const PageDims& d);
+int paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int rows,
+                  const int32_t* starts, const int32_t* lens, const int32_t* table,
+                  const void* k_cache, const void* v_cache, const float* k_scale,
+                  const float* v_scale, const PageDims& d, float scale, void* workspace,
+                  uint16_t* out, hipStream_t s);
+
 // ---- MoE ----
 constexpr int kMaxRoutes = 8 * 16 + 1;
 // Work list of one MoE step: distinct routed experts (first appearance order)
@@ -303,6 +336,13 @@ int moe_reduce_norm(const uint16_t* p, const uint16_t* factor, uint16_t* h, cons
 int head_parts(int n, int k);
 int head_partials(const QWeight& w, const uint16_t* x, int m, float* maxima, uint32_t* indices,
                   int* parts, hipStream_t s);
+// ---- sampling (sample.hip) ----
+constexpr int kSampleMaxVocab = 1 << 20;
+size_t sample_workspace(int rows, int n);
+int sample_bf16(const uint16_t* logits, int64_t stride, int rows, int n, const float* temperature,
+                const int32_t* top_k, const float* top_p, const float* min_p,
+                const float* uniform, uint32_t* tokens, float* logprob, int32_t* kept,
+                void* workspace, hipStream_t s);
 // Greedy head without a workspace: the partials live in a static device
 // array of kHeadNoAllocScratchBytes per GPU (head.hip); MX_EUNSUPPORTED when
 // head_noalloc_bytes(n, k, m) exceeds it.

@@ -1,0 +1,644 @@
+// The paged cache: rows appended to it, and attention of one new token a row over it.
+#include "paged_core.hpp"
+
+namespace mx {
+
+namespace {
+
+using namespace pg;
+
+// ---------------------------------------------------------------------------
+// Append: RMS norm, rotary positions and the cache's writes, in one launch.
+//
+//   y = x rsqrt(mean x^2 + eps) (w + 1)       (q and k heads; w absent: y = x)
+//   pair (i, i + rot/2), a = position[axis(i)] inv_freq[i]:
+//     (y1 cos a - y2 sin a, y2 cos a + y1 sin a)
+//
+// all in fp32 with one rounding, to bf16 or, divided by the kv head's scale, to
+// e4m3.  The angle is formed in 64 bits as a fraction of a turn, so positions
+// of millions keep their low bits; its sine and cosine are then fp32 series
+// around the nearest quarter turn, once per row and workgroup.
+//
+// Bytes bound it.  The first workgroups of the grid take the q and k heads of
+// one row each, eight values a lane; the others take one kv head's V of 32 rows
+// each: they pass through LDS so that neighbouring lanes store neighbouring
+// positions of a page, where V lies transposed.
+constexpr int kQkThreads = 256;
+constexpr int kVRows = 32;
+
+// sin and cos of 2 pi t
+__device__ __forceinline__ void sincos_turn(double t, float* sn, float* cs) {
+  const double f = __builtin_amdgcn_fract(t);           // [0, 1)
+  const double quarter = __builtin_rint(f * 4.0);       // 0 .. 4
+  const float r = float((f - quarter * 0.25) * 6.283185307179586477);  // |r| <= pi / 4
+  const float z = r * r;
+  float s = fmaf_(z, 2.7557319e-6f, -1.9841270e-4f);    // 1/9!, 1/7!
+  s = fmaf_(z, s, 8.3333333e-3f);                       // 1/5!
+  s = fmaf_(z, s, -1.6666667e-1f);                      // 1/3!
+  s = fmaf_(r * z, s, r);
+  float c = fmaf_(z, -2.7557319e-7f, 2.4801587e-5f);    // 1/10!, 1/8!
+  c = fmaf_(z, c, -1.3888889e-3f);                      // 1/6!
+  c = fmaf_(z, c, 4.1666667e-2f);                       // 1/4!
+  c = fmaf_(z, c, -0.5f);
+  c = fmaf_(z, c, 1.0f);
+  const int n = int(quarter) & 3;
+  const float a = n & 1 ? c : s, b = n & 1 ? s : c;
+  *sn = n & 2 ? -a : a;
+  *cs = (n == 1 || n == 2) ? -b : b;
+}
+
+template <int HD, bool F8>
+__global__ __launch_bounds__(kQkThreads) void append_kernel(
+    const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
+    const int32_t* __restrict__ seqs, const int32_t* __restrict__ pos,
+    const int32_t* __restrict__ rope_pos, RopeAxes rope, const uint16_t* __restrict__ q_norm,
+    const uint16_t* __restrict__ k_norm, float eps, const int32_t* __restrict__ table, PageDims d,
+    const float* __restrict__ k_scale, const float* __restrict__ v_scale,
+    uint16_t* __restrict__ q_out, void* __restrict__ k_cache, void* __restrict__ v_cache,
+    int groups, int64_t qk_blocks) {
+  constexpr int LPH = HD / 8;           // lanes per head
+  constexpr int HPB = kQkThreads / LPH; // heads per workgroup
+  __shared__ float trig[2][128];
+  __shared__ float pairs[kQkThreads][9];  // nine: lanes of a wave start in different banks
+  __shared__ uint16_t vbuf[kVRows][HD + 2];
+  const int t = threadIdx.x;
+  const int page = 1 << d.page_log2;
+  const int q_width = d.gated ? 2 * HD : HD;
+  const int64_t b = blockIdx.x;
+  if (b < qk_blocks) {
+    const int row = int(b / groups), group = int(b % groups);
+    const int seq = seqs ? seqs[row] : row;
+    if (unsigned(seq) >= unsigned(d.sequences)) return;  // a padding row (uniform)
+    const int head = group * HPB + t / LPH, piece = t % LPH;
+    const bool alive = head < d.heads + d.kv_heads, is_q = head < d.heads;
+    const int kvh = head - d.heads;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (alive) {
+      const uint16_t* src = qkv + int64_t(row) * qkv_stride +
+                            (is_q ? int64_t(head) * q_width
+                                  : int64_t(d.heads) * q_width + int64_t(kvh) * HD) + 8 * piece;
+      raw = *reinterpret_cast<const uint4*>(src);
+    }
+    const int half = rope.rotary_dim / 2;
+    if (t < half) {
+      const double p = double(rope_pos[int64_t(rope.pair_axis[t]) * rows + row]);
+      sincos_turn(p * rope.inv_freq[t] * 0.15915494309189533577, &trig[1][t], &trig[0][t]);
+    }
+    float y[8];
+    const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[2 * i] = u2f(w4[i] << 16);
+      y[2 * i + 1] = u2f(w4[i] & 0xffff0000u);
+    }
+    const uint16_t* norm = is_q ? q_norm : k_norm;
+    if (norm && alive) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf_(y[i], y[i], ss);
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+      const float inv = 1.0f / __builtin_sqrtf(ss * (1.0f / HD) + eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * (bf16_to_f32(norm[8 * piece + i]) + 1.0f);
+    }
+    // every value's partner of the rotation, half a rotary width away
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pairs[t][i] = y[i];
+    __syncthreads();
+    if (!alive) return;
+    const int head0 = t - piece;  // the head's first lane
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = 8 * piece + i;
+      if (c < 2 * half) {
+        const int pi = c < half ? c : c - half;
+        const int other = c < half ? c + half : c - half;
+        const float x = pairs[head0 + (other >> 3)][other & 7];
+        y[i] = c < half ? y[i] * trig[0][pi] - x * trig[1][pi]
+                        : y[i] * trig[0][pi] + x * trig[1][pi];
+      }
+    }
+    if (is_q) {
+      *reinterpret_cast<uint4*>(q_out + (int64_t(row) * d.heads + head) * HD + 8 * piece) =
+          make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
+      return;
+    }
+    const int p = pos[row];
+    if (p < 0 || (p >> d.page_log2) >= d.table_width) return;
+    const int pid = page_at(table, d, seq, p >> d.page_log2);
+    if (pid < 0) return;
+    const int64_t at =
+        pid * d.page_stride + (int64_t(kvh) * page + (p & (page - 1))) * HD + 8 * piece;
+    if constexpr (F8) {
+      const float s = k_scale ? k_scale[kvh] : 1.0f;
+      uint32_t o[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i >> 2] |= uint32_t(narrow(y[i] / s)) << (8 * (i & 3));
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(k_cache) + at) = make_uint2(o[0], o[1]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(k_cache) + at) =
+          make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
+    }
+    return;
+  }
+  // V of kVRows rows and one kv head
+  const int64_t vb = b - qk_blocks;
+  const int kvh = int(vb % d.kv_heads);
+  const int row0 = int(vb / d.kv_heads) * kVRows;
+  const int64_t col = int64_t(d.heads) * q_width + int64_t(d.kv_heads + kvh) * HD;
+  for (int i = t; i < kVRows * LPH; i += kQkThreads) {
+    const int r = i / LPH, piece = i % LPH;
+    if (row0 + r < rows) {
+      const uint4 v =
+          *reinterpret_cast<const uint4*>(qkv + int64_t(row0 + r) * qkv_stride + col + 8 * piece);
+      uint32_t* dst = reinterpret_cast<uint32_t*>(&vbuf[r][8 * piece]);  // rows are 4-byte aligned
+      dst[0] = v.x;
+      dst[1] = v.y;
+      dst[2] = v.z;
+      dst[3] = v.w;
+    }
+  }
+  __syncthreads();
+  const int r = t % kVRows, row = row0 + r;
+  if (row >= rows) return;
+  const int seq = seqs ? seqs[row] : row, p = pos[row];
+  if (unsigned(seq) >= unsigned(d.sequences) || p < 0 || (p >> d.page_log2) >= d.table_width) return;
+  const int pid = page_at(table, d, seq, p >> d.page_log2);
+  if (pid < 0) return;
+  const int64_t at = pid * d.page_stride + (int64_t(kvh) * HD << d.page_log2) + (p & (page - 1));
+  float s = 1.0f;
+  if constexpr (F8) s = v_scale ? v_scale[kvh] : 1.0f;
+  for (int c = t / kVRows; c < HD / 2; c += kQkThreads / kVRows) {
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(&vbuf[r][2 * c]);
+    const int64_t o = at + (int64_t(2 * c) << d.page_log2);
+    if constexpr (F8) {
+      uint8_t* dst = static_cast<uint8_t*>(v_cache);
+      dst[o] = narrow(u2f(v << 16) / s);
+      dst[o + page] = narrow(u2f(v & 0xffff0000u) / s);
+    } else {
+      uint16_t* dst = static_cast<uint16_t*>(v_cache);
+      dst[o] = uint16_t(v);
+      dst[o + page] = uint16_t(v >> 16);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Decode: softmax(q k^T scale) v of one row over its sequence's positions.
+//
+// The keys of all rows are cut into chunks of whole units (four waves' tiles)
+// whose length follows from all rows' lengths, so that a few chunks a compute
+// unit cover any mix of short and long contexts; every wave forms that plan
+// from the lengths itself.  A workgroup takes one (row, chunk, kv head) for the
+// group's q heads, so each K and V value is read once; its four waves take
+// tiles of KT keys in turn with a running maximum, sum and output each, and
+// join through LDS.  Rows of one chunk are finished there, the others leave
+// partials that the second launch joins in order.
+//
+// Matrix cores do both products with the q heads as columns (columns past the
+// group are zero): S^T = K Q^T gives lane (head, quarter g) the scores of keys
+// KT/4 g .. of the tile, because K's rows enter in that order, and these are the
+// k-slots that the same lane supplies as P^T for O^T = V^T P^T.  So scores never
+// leave their lane, and K and V come from memory straight into operands.  P is
+// split in two bf16 parts: the matrix cores have time, and P keeps 16 bits.
+constexpr int kDecodeTarget = 512;  // chunks wanted: two workgroups a compute unit
+
+template <bool F8>
+struct DecodeTile {
+  static constexpr int kKeys = F8 ? 64 : 32;  // a lane's 16 bytes of V: 16 or 8 keys
+  static constexpr int kUnit = 4 * kKeys;
+};
+
+// The length of a row's context, or -1 for a padding row.
+__device__ __forceinline__ int row_len(const int32_t* __restrict__ seqs,
+                                       const int32_t* __restrict__ lens, const PageDims& d, int r,
+                                       int rows) {
+  if (r >= rows) return -1;
+  const int seq = seqs ? seqs[r] : r;
+  if (unsigned(seq) >= unsigned(d.sequences)) return -1;
+  const int64_t most = int64_t(d.table_width) << d.page_log2;
+  const int len = lens[r];
+  return len < 0 ? 0 : (len > most ? int(most) : len);
+}
+
+__device__ __forceinline__ int wave_sum(int v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Units of a chunk: the smallest with at most kDecodeTarget chunks beside the rounding of each row.
+__device__ __forceinline__ int plan_chunk(const int32_t* seqs, const int32_t* lens,
+                                          const PageDims& d, int rows, int unit) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;
+  for (int r = 0; r < rows; r += 64) {
+    const int len = row_len(seqs, lens, d, r + lane, rows);
+    total += wave_sum(len > 0 ? (len + unit - 1) / unit : 0);
+  }
+  const int64_t c = (total * d.kv_heads + kDecodeTarget - 1) / kDecodeTarget;
+  return c < 1 ? 1 : int(c);
+}
+
+template <int HD, bool F8>
+__global__ __launch_bounds__(256, 2) void decode_kernel(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
+    const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
+    const int32_t* __restrict__ table, const void* __restrict__ k_cache,
+    const void* __restrict__ v_cache, const float* __restrict__ k_scale,
+    const float* __restrict__ v_scale, PageDims d, float scale, float* __restrict__ o_part,
+    float* __restrict__ ml_part, uint16_t* __restrict__ out) {
+  constexpr int KT = DecodeTile<F8>::kKeys, kUnit = DecodeTile<F8>::kUnit;
+  constexpr int T = KT / 16;        // score tiles
+  constexpr int KG = KT / 4;        // keys of a lane quarter
+  constexpr int NV = HD / 16;       // dim tiles of the output
+  constexpr int KL = HD / (F8 ? 64 : 32);  // 16-byte pieces of a K row a lane
+  constexpr int QLD = HD + 8;       // padded q row in LDS
+  constexpr int OLD = HD + 4;       // padded output row in LDS
+  // the next tile's K is requested once this one's scores are done; at 256 dims the
+  // registers hold one tile of each, and the other waves cover its latency
+  constexpr bool kAhead = HD < 256;
+  __shared__ __align__(16) uint16_t qs[16 * QLD];
+  __shared__ float mls[2][4][16];
+  extern __shared__ __align__(16) float os[];  // [4 waves][group][OLD]
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const int col = lane & 15, g = lane >> 4;
+  const int group = d.heads / d.kv_heads;
+  // this workgroup's (row, chunk, kv head)
+  const int item = blockIdx.x, kvh = item % d.kv_heads;
+  const int want = item / d.kv_heads;
+  const int cu = plan_chunk(seqs, lens, d, rows, kUnit);
+  int row = -1, chunk = 0, before = 0, len = 0;
+  for (int r = 0; r < rows; r += 64) {
+    const int l = row_len(seqs, lens, d, r + lane, rows);
+    const int units = l > 0 ? (l + kUnit - 1) / kUnit : 0;
+    const int n = (units + cu - 1) / cu;
+    int sum = n;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(sum, o, 64);
+      sum += lane >= o ? v : 0;
+    }
+    const uint64_t past = __ballot(before + sum > want);
+    if (past) {
+      const int f = __builtin_ctzll(past);
+      row = r + f;
+      len = __shfl(l, f, 64);
+      chunk = want - (before + __shfl(sum, f, 64) - __shfl(n, f, 64));
+      break;
+    }
+    before += __shfl(sum, 63, 64);
+  }
+  if (row < 0) return;  // uniform: past the last chunk
+  const int seq = seqs ? seqs[row] : row;
+  const int k0 = chunk * cu * kUnit;
+  const int k1 = min(len, k0 + cu * kUnit);  // k0 < len
+  const bool whole = k0 == 0 && k1 == len;
+  const int last_page = (len - 1) >> d.page_log2;
+
+  // q heads into LDS (rows past the group zero)
+  for (int i = t; i < 16 * HD / 8; i += 256) {
+    const int h = i / (HD / 8), piece = i % (HD / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (h < group)
+      v = *reinterpret_cast<const uint4*>(
+          q + (int64_t(row) * d.heads + kvh * group + h) * HD + 8 * piece);
+    *reinterpret_cast<uint4*>(qs + h * QLD + 8 * piece) = v;
+  }
+  __syncthreads();
+
+  const char* kc = static_cast<const char*>(k_cache);
+  const char* vc = static_cast<const char*>(v_cache);
+  constexpr int E = F8 ? 1 : 2;
+  const int page = 1 << d.page_log2;
+  const float sl2 =
+      scale * kLog2e * (F8 && k_scale ? k_scale[kvh] : 1.0f);  // scores in log2 units
+  // K row of score tile s for this lane's operand row: key KG (col / 4) + 4 s + col % 4
+  const int krow = KG * (col >> 2) + (col & 3);
+  const int vrow = KG * g;  // first key of this lane's V operands and scores
+  float m_run = neg_inf(), l_run = 0.0f;
+  floatx4_t o[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) o[n] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  uint4 kb[T][KL], vb[NV];
+  int pk = 0, pv = 0;
+  auto pages_of = [&](int tile) {
+    pk = page_at(table, d, seq, min((tile + krow) >> d.page_log2, last_page));
+    pv = page_at(table, d, seq, min((tile + vrow) >> d.page_log2, last_page));
+  };
+  auto load_k = [&](int tile) {
+    const int64_t base = (pk < 0 ? 0 : pk) * d.page_stride + (int64_t(kvh) << d.page_log2) * HD;
+    const int off = (tile + krow) & (page - 1);
+#pragma unroll
+    for (int s = 0; s < T; ++s)
+#pragma unroll
+      for (int i = 0; i < KL; ++i)
+        kb[s][i] = *reinterpret_cast<const uint4*>(
+            kc + (base + int64_t(off + 4 * s) * HD) * E + 64 * i + 16 * g);
+  };
+  auto load_v = [&](int tile) {
+    const int64_t base = (pv < 0 ? 0 : pv) * d.page_stride + (int64_t(kvh) << d.page_log2) * HD +
+                         ((tile + vrow) & (page - 1));
+    const char* p = vc + (base + (int64_t(col) << d.page_log2)) * E;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      vb[n] = *reinterpret_cast<const uint4*>(p);
+      p += (16 * E) << d.page_log2;
+      asm("" : "+v"(p));  // one address that walks: sixteen at once would spill
+    }
+  };
+  int tile = k0 + wave * KT;
+  if (tile < k1) {
+    pages_of(tile);
+    load_k(tile);
+    load_v(tile);
+  }
+  for (; tile < k1; tile += kUnit) {
+    // q is read again for every tile: held, its 32 registers would spill at 256 dims
+    if constexpr (HD == 256) asm volatile("" ::: "memory");
+    // valid keys of this lane quarter
+    const int nk = pv < 0 ? 0 : min(max(k1 - (tile + vrow), 0), KG);
+    floatx4_t sc[T];
+#pragma unroll
+    for (int s = 0; s < T; ++s) sc[s] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      if constexpr (F8) {
+        const uint4 qa = *reinterpret_cast<const uint4*>(qs + col * QLD + 64 * i + 16 * g);
+        const uint4 qb = *reinterpret_cast<const uint4*>(qs + col * QLD + 64 * i + 16 * g + 8);
+#pragma unroll
+        for (int s = 0; s < T; ++s) {
+          sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8_t, widen8(kb[s][i].x, kb[s][i].y)),
+              __builtin_bit_cast(bf16x8_t, qa), sc[s], 0, 0, 0);
+          sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8_t, widen8(kb[s][i].z, kb[s][i].w)),
+              __builtin_bit_cast(bf16x8_t, qb), sc[s], 0, 0, 0);
+        }
+      } else {
+        const uint4 qa = *reinterpret_cast<const uint4*>(qs + col * QLD + 32 * i + 8 * g);
+#pragma unroll
+        for (int s = 0; s < T; ++s)
+          sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8_t, kb[s][i]), __builtin_bit_cast(bf16x8_t, qa), sc[s], 0,
+              0, 0);
+      }
+    }
+    const int next = tile + kUnit;
+    const bool more = next < k1;
+    const int nv = nk;
+    if (kAhead && more) {
+      pages_of(next);
+      load_k(next);
+    }
+    float mt = neg_inf();
+#pragma unroll
+    for (int s = 0; s < T; ++s)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[s][r] = 4 * s + r < nk ? sc[s][r] * sl2 : neg_inf();
+        mt = fmaxf(mt, sc[s][r]);
+      }
+    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    const float mn = fmaxf(m_run, mt);
+    const float ref = mn == neg_inf() ? 0.0f : mn;  // no key yet: every weight is 0
+    if (__any(mn != m_run)) {
+      const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
+      l_run *= alpha;
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[n][r] *= alpha;
+      m_run = mn;
+    }
+    uint32_t ph[2 * T], pl[2 * T];
+#pragma unroll
+    for (int s = 0; s < T; ++s)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float a = __builtin_amdgcn_exp2f(sc[s][r] - ref);
+        const float b = __builtin_amdgcn_exp2f(sc[s][r + 1] - ref);
+        l_run += a + b;
+        const uint32_t h = pack2(a, b);
+        ph[2 * s + r / 2] = h;
+        pl[2 * s + r / 2] = pack2(a - u2f(h << 16), b - u2f(h & 0xffff0000u));
+      }
+    // keys past the end may hold anything: their values become 0 (the last tile only)
+    if (!__all(nv == KG)) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        uint32_t w[4] = {vb[n].x, vb[n].y, vb[n].z, vb[n].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          constexpr int P = 4 / E;  // keys a word
+          const int left = nv - P * i;
+          const int bits = left <= 0 ? 0 : (left >= P ? 32 : left * 8 * E);
+          w[i] = bits == 32 ? w[i] : (w[i] & ((1u << bits) - 1u));
+        }
+        vb[n] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      if constexpr (F8) {
+        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, widen8(vb[n].x, vb[n].y));
+        const bf16x8_t vd = __builtin_bit_cast(bf16x8_t, widen8(vb[n].z, vb[n].w));
+        const uint4 h0 = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+        const uint4 h1 = make_uint4(ph[4], ph[5], ph[6], ph[7]);
+        const uint4 l0 = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+        const uint4 l1 = make_uint4(pl[4], pl[5], pl[6], pl[7]);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8_t, h0), o[n], 0, 0, 0);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8_t, l0), o[n], 0, 0, 0);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vd, __builtin_bit_cast(bf16x8_t, h1), o[n], 0, 0, 0);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vd, __builtin_bit_cast(bf16x8_t, l1), o[n], 0, 0, 0);
+      } else {
+        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, vb[n]);
+        const uint4 h0 = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+        const uint4 l0 = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8_t, h0), o[n], 0, 0, 0);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8_t, l0), o[n], 0, 0, 0);
+      }
+    }
+    if (!kAhead && more) {
+      pages_of(next);
+      load_k(next);
+    }
+    if (more) load_v(next);
+  }
+  // the four waves' parts
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  if (g == 0) {
+    mls[0][wave][col] = m_run;
+    mls[1][wave][col] = l_run;
+  }
+  if (col < group) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+      *reinterpret_cast<floatx4_t*>(os + (wave * group + col) * OLD + 16 * n + 4 * g) = o[n];
+  }
+  __syncthreads();
+  const float vs = F8 && v_scale ? v_scale[kvh] : 1.0f;
+  const int64_t part0 = (int64_t(item / d.kv_heads) * d.kv_heads + kvh) * group;
+  for (int i = t; i < group * HD; i += 256) {
+    const int h = i / HD, c = i % HD;
+    float M = mls[0][0][h];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) M = fmaxf(M, mls[0][w][h]);
+    const float ref = M == neg_inf() ? 0.0f : M;
+    float L = 0.0f, O = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float e = __builtin_amdgcn_exp2f(mls[0][w][h] - ref);
+      L = fmaf_(mls[1][w][h], e, L);
+      O = fmaf_(os[(w * group + h) * OLD + c], e, O);
+    }
+    if (whole) {
+      float y = L == 0.0f ? 0.0f : O / L * vs;
+      const int head = kvh * group + h;
+      if (d.gated)
+        y *= gate_of(bf16_to_f32(qkv[int64_t(row) * qkv_stride + int64_t(head) * 2 * HD + HD + c]));
+      out[(int64_t(row) * d.heads + head) * HD + c] = f32_to_bf16(y);
+    } else {
+      o_part[(part0 + h) * HD + c] = O;
+      if (c == 0) {
+        ml_part[(part0 + h) * 2] = M;
+        ml_part[(part0 + h) * 2 + 1] = L;
+      }
+    }
+  }
+}
+
+// Joins the chunks of one (row, head), four waves taking every fourth one, in a
+// fixed order; rows without keys become 0, rows of one chunk are done already.
+template <int HD>
+__global__ __launch_bounds__(256) void decode_join_kernel(
+    const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
+    const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
+    const float* __restrict__ v_scale, PageDims d, int unit, const float* __restrict__ o_part,
+    const float* __restrict__ ml_part, uint16_t* __restrict__ out) {
+  constexpr int DPL = HD / 64;
+  __shared__ float ls[4];
+  __shared__ float os[4][HD];
+  const int head = blockIdx.x % d.heads, row = blockIdx.x / d.heads;
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const int group = d.heads / d.kv_heads, kvh = head / group;
+  const int len = row_len(seqs, lens, d, row, rows);
+  if (len < 0) return;
+  uint16_t* dst = out + (int64_t(row) * d.heads + head) * HD;
+  if (len == 0) {
+    if (t < HD) dst[t] = 0;
+    return;
+  }
+  const int cu = plan_chunk(seqs, lens, d, rows, unit);
+  const int units = (len + unit - 1) / unit, n = (units + cu - 1) / cu;
+  if (n == 1) return;
+  int64_t before = 0;
+  for (int r = 0; r < row; r += 64) {
+    const int l = r + lane < row ? row_len(seqs, lens, d, r + lane, rows) : 0;
+    before += wave_sum(l > 0 ? ((l + unit - 1) / unit + cu - 1) / cu : 0);
+  }
+  const int64_t step = int64_t(d.kv_heads) * group;
+  const int64_t part0 = before * step + head;
+  float M = neg_inf();
+  for (int c = lane; c < n; c += 64) M = fmaxf(M, ml_part[(part0 + c * step) * 2]);
+  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  const float ref = M == neg_inf() ? 0.0f : M;
+  float L = 0.0f, O[DPL];
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) O[i] = 0.0f;
+#pragma unroll 4
+  for (int c = wave; c < n; c += 4) {
+    const int64_t p = part0 + c * step;
+    const float e = __builtin_amdgcn_exp2f(ml_part[p * 2] - ref);
+    L = fmaf_(ml_part[p * 2 + 1], e, L);
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) O[i] = fmaf_(o_part[p * HD + 64 * i + lane], e, O[i]);
+  }
+  if (lane == 0) ls[wave] = L;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) os[wave][64 * i + lane] = O[i];
+  __syncthreads();
+  if (t >= HD) return;
+  const float l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+  float y = (os[0][t] + os[1][t]) + (os[2][t] + os[3][t]);
+  y = l == 0.0f ? 0.0f : y / l * (v_scale ? v_scale[kvh] : 1.0f);
+  if (d.gated) y *= gate_of(bf16_to_f32(qkv[int64_t(row) * qkv_stride + int64_t(head) * 2 * HD + HD + t]));
+  dst[t] = f32_to_bf16(y);
+}
+
+int decode_unit(const PageDims& d) {
+  return d.f8 ? DecodeTile<true>::kUnit : DecodeTile<false>::kUnit;
+}
+
+// The most chunks (times kv heads) that any lengths give.
+int64_t decode_items(int rows, const PageDims& d) {
+  const int64_t unit = decode_unit(d);
+  const int64_t most = ((int64_t(d.table_width) << d.page_log2) + unit - 1) / unit;
+  const int64_t all = int64_t(rows) * d.kv_heads;
+  return all * most < kDecodeTarget + all ? all * most : kDecodeTarget + all;
+}
+
+}  // namespace
+
+int paged_append(const uint16_t* qkv, int64_t qkv_stride, int rows, const int32_t* seqs,
+                 const int32_t* pos, const int32_t* rope_pos, const RopeAxes& rope,
+                 const uint16_t* q_norm, const uint16_t* k_norm, float eps, const int32_t* table,
+                 const PageDims& d, const float* k_scale, const float* v_scale, uint16_t* q_out,
+                 void* k_cache, void* v_cache, hipStream_t s) {
+  const int per = kQkThreads / (d.head_dim / 8);
+  const int groups = (d.heads + d.kv_heads + per - 1) / per;
+  const int64_t qk = int64_t(rows) * groups;
+  const int64_t blocks = qk + int64_t((rows + kVRows - 1) / kVRows) * d.kv_heads;
+  if (blocks > 0x7fffffff) return MX_EUNSUPPORTED;
+#define MX_APPEND(HH, FF)                                                                       \
+  if (d.head_dim == HH && d.f8 == FF) {                                                         \
+    hipLaunchKernelGGL((append_kernel<HH, FF>), dim3(unsigned(blocks)), dim3(kQkThreads), 0, s, \
+                       qkv, qkv_stride, rows, seqs, pos, rope_pos, rope, q_norm, k_norm, eps,   \
+                       table, d, k_scale, v_scale, q_out, k_cache, v_cache, groups, qk);        \
+    return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;                                   \
+  }
+  MX_APPEND(64, false) MX_APPEND(128, false) MX_APPEND(256, false)
+  MX_APPEND(64, true) MX_APPEND(128, true) MX_APPEND(256, true)
+#undef MX_APPEND
+  return MX_EUNSUPPORTED;
+}
+
+size_t paged_decode_workspace(int rows, const PageDims& d) {
+  return size_t(decode_items(rows, d)) * (d.heads / d.kv_heads) * (d.head_dim + 2) * 4;
+}
+
+int paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int rows,
+                 const int32_t* seqs, const int32_t* lens, const int32_t* table,
+                 const void* k_cache, const void* v_cache, const float* k_scale,
+                 const float* v_scale, const PageDims& d, float scale, void* workspace,
+                 uint16_t* out, hipStream_t s) {
+  const int64_t items = decode_items(rows, d), joins = int64_t(rows) * d.heads;
+  if (items > 0x7fffffff || joins > 0x7fffffff) return MX_EUNSUPPORTED;
+  const int group = d.heads / d.kv_heads;
+  float* o_part = static_cast<float*>(workspace);
+  float* ml_part = o_part + items * group * d.head_dim;
+  const int lds = 4 * group * (d.head_dim + 4) * 4;
+#define MX_DECODE(HH, FF)                                                                        \
+  if (d.head_dim == HH && d.f8 == FF) {                                                          \
+    const auto fn = decode_kernel<HH, FF>;                                                       \
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn),                                   \
+                            hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)      \
+      return MX_EHIP;                                                                            \
+    hipLaunchKernelGGL(fn, dim3(unsigned(items)), dim3(256), lds, s, q, qkv, qkv_stride, rows,   \
+                       seqs, lens, table, k_cache, v_cache, k_scale, v_scale, d, scale, o_part,  \
+                       ml_part, out);                                                            \
+    if (hipGetLastError() != hipSuccess) return MX_EHIP;                                         \
+    hipLaunchKernelGGL((decode_join_kernel<HH>), dim3(unsigned(joins)), dim3(256), 0, s, qkv,    \
+                       qkv_stride, rows, seqs, lens, FF ? v_scale : nullptr, d, decode_unit(d),  \
+                       o_part, ml_part, out);                                                    \
+    return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;                                    \
+  }
+  MX_DECODE(64, false) MX_DECODE(128, false) MX_DECODE(256, false)
+  MX_DECODE(64, true) MX_DECODE(128, true) MX_DECODE(256, true)
+#undef MX_DECODE
+  return MX_EUNSUPPORTED;
+}
+
+}  // namespace mx
