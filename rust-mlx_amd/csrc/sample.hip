@@ -8,22 +8,25 @@
 // n is the shortest of them (at least one token), and the sampled token is the
 // first whose prefix mass exceeds u times the mass of n.
 //
-// bf16 has 65536 values, so a row is known by how often each occurs: one
-// workgroup counts them in LDS (16-bit counters, 128 KB) and needs an
-// exponential per occurring value instead of one per token.  Counts are exact
-// and masses are sums of few products in 64 bits, so neither the order of the
-// atomics nor the launch shape can change a token, and a u next to a border
-// falls on the side that the definition says.
+// bf16 has 65536 values, so a row is known by how often each occurs, and needs an
+// exponential per occurring value instead of one per token, without any sort.
+// Counts are exact and masses are sums of few products in 64 bits, so neither the
+// order of the atomics nor the launch shape can change a token, and a u next to a
+// border falls on the side that the definition says.
 //
-// Counters are cut into 1024 segments of 64 neighbouring values.  Each gets its
-// count and mass, one scan over the workgroup's threads gives the prefixes, and
-// every question (which value holds rank k, which holds mass x) is a search over
-// segments and then over one segment's 64 values by a wave.  The rank within the
-// value's tokens then picks the id, by counts of matches per 512 tokens.
+// Launch 1 counts: a workgroup takes a part of a row (at most 65024 tokens, so
+// 16-bit counters suffice: 128 KB of LDS for all values) and writes the segments
+// of 64 neighbouring values that occur, with a bit each.
+// Launch 2 chooses, a workgroup a row: it adds the parts' segments, weighs them,
+// forms prefixes over the 1024 segments, and one wave answers each question
+// (which value holds rank k, which holds mass x) by a search over the prefixes
+// and then over one segment's 64 values, a lane each.  The rank within the
+// value's tokens picks the part by the parts' own counts, and only that part is
+// read again for the id.
 //
-// A row of one value that occurs over 65535 times does not fit 16-bit counters;
-// the sum of all counters shows it (a carry or a wrap only ever loses), and such a
-// row is counted again with 32-bit counters, half the values at a time.
+// The latency of few dependent steps bounds it.  One workgroup a row that counts,
+// chooses and reads the row three times takes 76 us for 1 to 256 rows of 151936:
+// each read is 19 dependent trips of one compute unit.
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -34,19 +37,21 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kSegments = 1024;
-constexpr int kPiece = 512;  // tokens of one wave's step: eight a lane
+constexpr int kPiece = 512;        // tokens of one wave's step: eight a lane
+constexpr int kPartPieces = 127;   // pieces of a part at most: 65024 tokens
+constexpr int kWavePieces = 8;     // of them a wave's, held in registers
+constexpr int kBatchParts = 512;   // parts in flight: two rounds of the device
+constexpr int kMaxParts = 32;
+constexpr int kSlots = 480;        // segments whose sums launch 2 keeps in LDS
 constexpr int kHistBytes = 65536 * 2;
+static_assert(kWavePieces * kWaves >= kPartPieces, "a part fits its waves");
+static_assert((kSampleMaxVocab / kPiece + 2) / kPartPieces + 1 <= kMaxParts, "parts of the longest row");
 
-struct Shared {
-  double mass[kSegments];     // of the segment, then of all before it
-  uint32_t count[kSegments];
-  double wmass[kWaves];
-  uint32_t wcount[kWaves];
-  uint32_t seg32[64];         // one segment's counters (32-bit rows)
-  uint32_t pieces[kSampleMaxVocab / kPiece];
-  int red[kWaves];
-  int answer;
-  uint32_t total, counted, above;
+// The workspace: counters of every part, then their segment bits, then their largest keys.
+struct Parts {
+  uint16_t* counts;  // [part][65536], segments without a bit are not written
+  uint32_t* bits;    // [part][32]
+  uint32_t* top;     // [part]
 };
 
 // bf16 bits as a 16-bit key that orders like the values; NaN counts as -inf, -0 as 0.
@@ -60,43 +65,128 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 constexpr uint32_t kNegInfKey = 0x007fu;
 
-// One row; a workgroup.
-__global__ __launch_bounds__(kThreads) void sample_kernel(
-    const uint16_t* __restrict__ logits, int64_t stride, int n,
+// A row in blocks of eight at 16-byte borders: block b holds tokens 8 b - lead .. + 7.
+struct Row {
+  const uint16_t* x;
+  int n, lead;
+  __device__ Row(const uint16_t* p, int n_)
+      : x(p), n(n_), lead(int((reinterpret_cast<uintptr_t>(p) & 15) >> 1)) {}
+  __device__ __forceinline__ int pieces() const { return (n + lead + kPiece - 1) / kPiece; }
+  __device__ __forceinline__ int first(int piece, int lane) const {
+    return piece * kPiece + 8 * lane - lead;
+  }
+  // the lane's eight tokens of a piece; those outside the row are -inf
+  __device__ __forceinline__ uint4 load(int piece, int lane) const {
+    const int at = first(piece, lane);
+    if (at >= 0 && at + 8 <= n) return *reinterpret_cast<const uint4*>(x + at);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = at + 2 * j;
+      const uint32_t lo = i >= 0 && i < n ? x[i] : 0xff80u;
+      const uint32_t hi = i + 1 >= 0 && i + 1 < n ? x[i + 1] : 0xff80u;
+      w[j] = lo | hi << 16;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+__device__ __forceinline__ uint32_t token_of(const uint4& v, int j) {
+  const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+  return j & 1 ? w >> 16 : w & 0xffffu;
+}
+
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(kThreads) void count_kernel(const uint16_t* __restrict__ logits,
+                                                         int64_t stride, int n, int parts,
+                                                         Parts ws) {
+  extern __shared__ __align__(16) uint32_t hist[];  // 32768 words, two counters each
+  __shared__ uint32_t bits[32], best_of;
+  const int row = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const Row r(logits + int64_t(row) * stride, n);
+  const int each = (r.pieces() + parts - 1) / parts;
+  const int p0 = part * each, p1 = min(r.pieces(), p0 + each);
+  uint4 v[kWavePieces];
+#pragma unroll
+  for (int i = 0; i < kWavePieces; ++i)
+    if (p0 + wave + kWaves * i < p1) v[i] = r.load(p0 + wave + kWaves * i, lane);
+  for (int i = t; i < 32768 / 4; i += kThreads)
+    reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+  if (t < 32) bits[t] = 0;
+  if (t == 32) best_of = 0;
+  __syncthreads();
+  uint32_t best = 0;
+#pragma unroll
+  for (int i = 0; i < kWavePieces; ++i)
+    if (p0 + wave + kWaves * i < p1) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t k = key_of(token_of(v[i], j)), d = 0xffffu - k;
+        best = max(best, k);
+        if (k > kNegInfKey) atomicAdd(&hist[d >> 1], d & 1 ? 0x10000u : 1u);
+      }
+    }
+  for (int o = 32; o > 0; o >>= 1) best = max(best, uint32_t(__shfl_xor(int(best), o, 64)));
+  if (lane == 0) atomicMax(&best_of, best);
+  __syncthreads();
+  // eight counters a lane, eight lanes a segment
+  uint16_t* counts = ws.counts + int64_t(blockIdx.x) * 65536;
+#pragma unroll
+  for (int i = 0; i < kSegments / 8 / kWaves; ++i) {
+    const int at = (kWaves * i + wave) * 64 + lane;  // in sixteen bytes
+    const uint4 c = reinterpret_cast<const uint4*>(hist)[at];
+    const uint64_t some = __ballot((c.x | c.y | c.z | c.w) != 0);
+    if (some >> (lane & 56) & 255) {
+      reinterpret_cast<uint4*>(counts)[at] = c;
+      if ((lane & 7) == 0) atomicOr(&bits[at >> 8], 1u << (at >> 3 & 31));
+    }
+  }
+  __syncthreads();
+  if (t < 32) ws.bits[int64_t(blockIdx.x) * 32 + t] = bits[t];
+  if (t == 32) ws.top[blockIdx.x] = best_of;
+}
+
+// ---------------------------------------------------------------------------
+constexpr int kNone = 0xffff;
+struct Shared {
+  double mass[kSegments];  // of the segment, then of all up to and with it
+  uint32_t count[kSegments];
+  uint16_t slot[kSegments];  // its place among the occurring segments, kNone where it does not occur
+  uint16_t list[kSegments];  // the occurring segments
+  uint32_t bits[kMaxParts * 32];
+  double wmass[kWaves];
+  uint32_t wcount[kWaves];
+  uint32_t pieces[kPartPieces + 1];
+  uint32_t top, above;
+  uint32_t chosen, rank, part;
+};
+
+__global__ __launch_bounds__(kThreads) void choose_kernel(
+    const uint16_t* __restrict__ logits, int64_t stride, int n, int parts, Parts ws,
     const float* __restrict__ temperature, const int32_t* __restrict__ top_k,
     const float* __restrict__ top_p, const float* __restrict__ min_p,
     const float* __restrict__ uniform, uint32_t* __restrict__ tokens, float* __restrict__ logprob,
     int32_t* __restrict__ kept) {
-  extern __shared__ __align__(16) uint32_t hist[];  // 32768 words
+  extern __shared__ __align__(16) uint32_t sums[];  // [kSlots][64]
   __shared__ Shared sh;
   const int row = blockIdx.x, t = threadIdx.x, wave = t >> 6, lane = t & 63;
-  const uint16_t* x = logits + int64_t(row) * stride;
-  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  const int pieces = (n + kPiece - 1) / kPiece;
-
-  // calls f(key, id) for every token of piece i, eight neighbouring ones a lane
-  auto each_of = [&](int i, auto&& f) {
-    const int at = i * kPiece + 8 * lane;
-    if (aligned && at + 8 <= n) {
-      const uint4 v = *reinterpret_cast<const uint4*>(x + at);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f(key_of(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu), at + j);
-    } else {
-      for (int j = 0; j < 8 && at + j < n; ++j) f(key_of(x[at + j]), at + j);
+  const uint16_t* counts = ws.counts + int64_t(row) * parts * 65536;
+  for (int i = t; i < parts * 32; i += kThreads) sh.bits[i] = ws.bits[int64_t(row) * parts * 32 + i];
+  if (wave == kWaves - 1) {
+    uint32_t best = lane < parts ? ws.top[int64_t(row) * parts + lane] : 0;
+    for (int o = 32; o > 0; o >>= 1) best = max(best, uint32_t(__shfl_xor(int(best), o, 64)));
+    if (lane == 0) {
+      sh.top = best;
+      sh.above = 0;
     }
-  };
-
-  // the largest key
-  int best = 0;
-  for (int i = wave; i < pieces; i += kWaves)
-    each_of(i, [&](uint32_t k, int) { best = max(best, int(k)); });
-  for (int o = 32; o > 0; o >>= 1) best = max(best, __shfl_xor(best, o, 64));
-  if (lane == 0) sh.red[wave] = best;
+  }
+  // the row's settings, on their way during the first steps
+  const float temp = temperature ? temperature[row] : 1.0f;
+  const int32_t k = top_k ? top_k[row] : 0;
+  const float p = top_p ? top_p[row] : 1.0f, mp = min_p ? min_p[row] : 0.0f;
+  const float u = uniform[row];
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) best = max(best, sh.red[w]);
-  const uint32_t top = uint32_t(best);
+  const uint32_t top = sh.top;
   if (top <= kNegInfKey) {  // uniform: nothing exceeds -inf
     if (t == 0) {
       tokens[row] = 0;
@@ -105,113 +195,107 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(
     }
     return;
   }
-  const float temp = temperature ? temperature[row] : 1.0f;
   const bool greedy = !(temp > 0.0f);
   const double lmax = double(value_of(top)), td = greedy ? 1.0 : double(temp);
-  // the weight of a key; keys without weight are no tokens
-  auto weight = [&](uint32_t key) {
+  // the weight of a value by its place below 0xffff
+  auto weight = [&](uint32_t d) {
+    const uint32_t key = 0xffffu - d;
     if (key == top) return 1.0;
-    if (key <= kNegInfKey) return 0.0;
     const double w = exp((double(value_of(key)) - lmax) / td);
     return w > 0.0 ? w : 0.0;  // also where both are infinite
   };
+  // lane's counter of a segment over all parts (of one that found no room in LDS)
+  auto gather = [&](int seg) {
+    uint32_t c = 0;
+    for (int i = 0; i < parts; ++i)
+      if (sh.bits[i * 32 + (seg >> 5)] >> (seg & 31) & 1)
+        c += counts[int64_t(i) * 65536 + seg * 64 + lane];
+    return c;
+  };
 
-  uint32_t chosen = top, rank = 0;  // the value and the rank among its tokens
   if (!greedy) {
-    // values that far below the largest weigh 0 even in 64 bits: not counted
-    const double cut = lmax - 750.0 * td;
-    uint32_t floor_key = kNegInfKey + 1;
-    {
-      float c = float(cut);
-      c = c < -3.3e38f ? -3.4e38f : c;
-      const uint32_t b = f2u(c) >> 16;  // towards 0 for negative c: above the cut or equal
-      const uint32_t k = key_of(b & 0xffffu);
-      if (c > -3.3e38f && k > kNegInfKey + 2) floor_key = k - 1;
+    {  // the list of occurring segments, in order
+      uint32_t a = 0;
+      for (int i = 0; i < parts; ++i) a |= sh.bits[i * 32 + (t >> 5)];
+      const bool here = a >> (t & 31) & 1;
+      const uint64_t m = __ballot(here);
+      if (lane == 0) sh.wcount[wave] = uint32_t(__builtin_popcountll(m));
+      sh.mass[t] = 0.0;
+      sh.count[t] = 0;
+      __syncthreads();
+      uint32_t at = uint32_t(__builtin_popcountll(m & ((1ull << lane) - 1)));
+      for (int w = 0; w < wave; ++w) at += sh.wcount[w];
+      sh.slot[t] = here ? uint16_t(at) : uint16_t(kNone);
+      if (here) sh.list[at] = uint16_t(t);
+      if (t == kThreads - 1) sh.pieces[0] = at + here;
+      __syncthreads();
     }
-    const uint32_t span = min(top - floor_key + 1, 65536u);  // values counted
-
-    auto clear = [&](int words) {
-      for (int i = t; i < words / 4; i += kThreads)
-        reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
-    };
-    // a segment's count and mass, from its counters by one wave
-    auto reduce = [&](int seg, uint32_t c, double floor_w, uint32_t* above) {
-      double m = 0.0;
-      if (__ballot(c != 0)) {
-        const uint32_t d = uint32_t(seg) * 64 + lane;
-        const double w = c ? weight(top - d) : 0.0;
-        c = w > 0.0 ? c : 0;
-        m = double(c) * w;
-        uint32_t a = w >= floor_w ? c : 0;
-        for (int o = 32; o > 0; o >>= 1) {
-          m += __shfl_xor(m, o, 64);
-          c += __shfl_xor(c, o, 64);
-          a += __shfl_xor(a, o, 64);
-        }
-        *above += a;
-      }
-      if (lane == 0) {
-        sh.mass[seg] = m;
-        sh.count[seg] = c;
-      }
-    };
-    const float mp = min_p ? min_p[row] : 0.0f;
+    const int occurring = int(sh.pieces[0]);
     const double floor_w = mp > 0.0f ? double(mp) : 0.0;
-
-    // all values in 16-bit counters
-    clear(32768);
-    if (t == 0) sh.counted = sh.total = sh.above = 0;
-    __syncthreads();
-    uint32_t mine = 0;
-    for (int i = wave; i < pieces; i += kWaves)
-      each_of(i, [&](uint32_t k, int) {
-        if (k >= floor_key) {
-          const uint32_t d = top - k;
-          atomicAdd(&hist[d >> 1], d & 1 ? 0x10000u : 1u);
-          ++mine;
-        }
-      });
-    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
-    if (lane == 0) atomicAdd(&sh.counted, mine);
-    __syncthreads();
-    uint32_t above = 0, sum = 0;
-    for (int seg = wave; seg < kSegments; seg += kWaves) {
-      const uint32_t c =
-          seg * 64 < int(span) ? reinterpret_cast<const uint16_t*>(hist)[seg * 64 + lane] : 0;
-      sum += c;
-      reduce(seg, c, floor_w, &above);
-    }
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) {
-      atomicAdd(&sh.total, sum);
-      atomicAdd(&sh.above, above);
-    }
-    __syncthreads();
-    const bool wide = sh.total != sh.counted;  // uniform
-    if (wide) {
-      __syncthreads();
-      if (t == 0) sh.above = 0;
-      above = 0;
-      for (int half = 0; half < 2; ++half) {
-        __syncthreads();
-        clear(32768);
-        __syncthreads();
-        for (int i = wave; i < pieces; i += kWaves)
-          each_of(i, [&](uint32_t k, int) {
-            const uint32_t d = top - k;
-            if (k >= floor_key && int(d >> 15) == half) atomicAdd(&hist[d & 32767], 1u);
-          });
-        __syncthreads();
-        for (int seg = wave; seg < kSegments / 2; seg += kWaves)
-          reduce(512 * half + seg, hist[seg * 64 + lane], floor_w, &above);
+    uint32_t above = 0;
+    // four segments a wave, a row of 16 lanes each, four counters a lane; the next four's
+    // counters of the first eight parts are requested before this four's are weighed
+    const int four = 4 * (lane & 15);
+    auto request = [&](int at, int first, uint2* v) {
+      const int seg = at < occurring ? sh.list[at] : -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = make_uint2(0, 0);
+        if (seg >= 0 && first + i < parts &&
+            (sh.bits[(first + i) * 32 + (seg >> 5)] >> (seg & 31) & 1))
+          v[i] = *reinterpret_cast<const uint2*>(counts + int64_t(first + i) * 65536 + seg * 64 + four);
       }
-      if (lane == 0) atomicAdd(&sh.above, above);
-      __syncthreads();
+    };
+    uint2 v[8];
+    request(4 * wave + (lane >> 4), 0, v);
+    for (int s0 = 4 * wave; s0 < occurring; s0 += 4 * kWaves) {
+      const int at = s0 + (lane >> 4);
+      uint32_t c[4] = {0, 0, 0, 0};
+      auto add = [&]() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          c[0] += v[i].x & 0xffffu;
+          c[1] += v[i].x >> 16;
+          c[2] += v[i].y & 0xffffu;
+          c[3] += v[i].y >> 16;
+        }
+      };
+      add();
+      for (int first = 8; first < parts; first += 8) {
+        request(at, first, v);
+        add();
+      }
+      request(at + 4 * kWaves, 0, v);
+      const bool here = at < occurring;
+      const int seg = here ? sh.list[at] : 0;
+      if (here && at < kSlots)
+        *reinterpret_cast<uint4*>(sums + at * 64 + four) = make_uint4(c[0], c[1], c[2], c[3]);
+      double m = 0.0;
+      uint32_t n_in = 0, a = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c[i]) {
+          const double w = weight(uint32_t(seg) * 64 + four + i);
+          m += double(c[i]) * w;
+          n_in += w > 0.0 ? c[i] : 0;
+          a += w > 0.0 && w >= floor_w ? c[i] : 0;
+        }
+      for (int o = 8; o > 0; o >>= 1) {
+        m += __shfl_xor(m, o, 64);
+        n_in += __shfl_xor(n_in, o, 64);
+        a += __shfl_xor(a, o, 64);
+      }
+      if (here && (lane & 15) == 0) {
+        sh.mass[seg] = m;
+        sh.count[seg] = n_in;
+        above += a;
+      }
     }
+    if ((lane & 15) == 0 && above) atomicAdd(&sh.above, above);
+    __syncthreads();
     // prefixes over the segments
     double m_in = sh.mass[t];
     uint32_t c_in = sh.count[t];
-    const uint32_t c_own = c_in;
     for (int o = 1; o < 64; o <<= 1) {
       const double m = __shfl_up(m_in, o, 64);
       const uint32_t c = __shfl_up(c_in, o, 64);
@@ -225,220 +309,238 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(
       sh.wcount[wave] = c_in;
     }
     __syncthreads();
-    double m_all = 0.0;
-    uint32_t c_all = 0;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w == wave) {
-        m_in += m_all;
-        c_in += c_all;
-      }
-      m_all += sh.wmass[w];
-      c_all += sh.wcount[w];
+    for (int w = 0; w < wave; ++w) {
+      m_in += sh.wmass[w];
+      c_in += sh.wcount[w];
     }
-    // A segment starts where the one before it ends, in the same bits.
     sh.mass[t] = m_in;
     sh.count[t] = c_in;
     __syncthreads();
-    const double m_before = t ? sh.mass[t - 1] : 0.0;
-    const uint32_t c_before = t ? sh.count[t - 1] : 0;
-
-    // the segment whose thread says so (the last with tokens, where none does)
-    auto find = [&](bool here) {
-      __syncthreads();
-      if (t == 0) sh.answer = -1;
-      __syncthreads();
-      if (here) atomicMax(&sh.answer, t);
-      __syncthreads();
-      int a = sh.answer;
-      if (a < 0) {
-        __syncthreads();
-        if (c_own) atomicMax(&sh.answer, t);
-        __syncthreads();
-        a = sh.answer;
-      }
-      return a;
-    };
-    // lane's counter and weight of segment seg
-    auto open = [&](int seg, uint32_t* c, double* w) {
-      if (!wide) {
-        *c = seg * 64 < int(span) ? reinterpret_cast<const uint16_t*>(hist)[seg * 64 + lane] : 0;
-      } else {
-        __syncthreads();
-        if (t < 64) sh.seg32[t] = 0;
-        __syncthreads();
-        for (int i = wave; i < pieces; i += kWaves)
-          each_of(i, [&](uint32_t k, int) {
-            const uint32_t d = top - k;
-            if (k >= floor_key && int(d >> 6) == seg) atomicAdd(&sh.seg32[d & 63], 1u);
-          });
-        __syncthreads();
-        *c = sh.seg32[lane];
-      }
-      *w = *c ? weight(top - (uint32_t(seg) * 64 + lane)) : 0.0;
-      *c = *w > 0.0 ? *c : 0;
-    };
-    // counts and masses of the segment's values up to and with the lane's own
-    auto prefix = [&](int seg, uint32_t c, double w, uint32_t* ci, double* mi) {
-      *ci = c;
-      *mi = double(c) * w;
-      for (int o = 1; o < 64; o <<= 1) {
-        const double m = __shfl_up(*mi, o, 64);
-        const uint32_t k = __shfl_up(*ci, o, 64);
-        if (lane >= o) {
-          *mi += m;
-          *ci += k;
+    if (wave == 0) {
+      const double m_all = sh.mass[kSegments - 1];
+      const uint32_t c_all = sh.count[kSegments - 1];
+      // the first segment whose prefix passes (the last with tokens where none does): over the
+      // waves' last segments, then within one wave's
+      auto find = [&](auto&& passes) {
+        uint64_t b = __ballot(passes(16 * lane + 15));
+        if (!b) b = __ballot(sh.count[16 * lane + 15] >= c_all);
+        const int base = 16 * __builtin_ctzll(b);
+        b = __ballot(lane < 16 && passes(base + (lane & 15)));
+        if (!b) b = __ballot(lane < 16 && sh.count[base + (lane & 15)] >= c_all);
+        return base + (b ? __builtin_ctzll(b) : 15);
+      };
+      uint32_t c = 0, ci = 0;  // of the open segment: the lane's counter, and up to it
+      double w = 0.0, mi = 0.0;
+      auto open = [&](int seg) {
+        const int s = sh.slot[seg];
+        c = s == kNone ? 0 : s < kSlots ? sums[s * 64 + lane] : gather(seg);
+        w = c ? weight(uint32_t(seg) * 64 + lane) : 0.0;
+        c = w > 0.0 ? c : 0;
+        ci = c;
+        mi = double(c) * w;
+        for (int o = 1; o < 64; o <<= 1) {
+          const double m = __shfl_up(mi, o, 64);
+          const uint32_t k = __shfl_up(ci, o, 64);
+          if (lane >= o) {
+            mi += m;
+            ci += k;
+          }
         }
+        mi += seg ? sh.mass[seg - 1] : 0.0;
+        ci += seg ? sh.count[seg - 1] : 0;
+      };
+      // the lane of the open segment that holds rank `want` (from 1), or the last with tokens
+      auto lane_of = [&](uint64_t past) {
+        if (!past) past = 1ull << (63 - __builtin_clzll(__ballot(c != 0) | 1ull));
+        return __builtin_ctzll(past);
+      };
+      // the mass of the first `want` tokens (1 <= want <= c_all)
+      auto mass_of = [&](uint32_t want) {
+        if (want >= c_all) return m_all;
+        open(find([&](int s) { return sh.count[s] >= want; }));
+        const int f = lane_of(__ballot(ci >= want));
+        const uint32_t over = __shfl(ci, f, 64) - want;  // tokens of the value past the rank
+        return __shfl(mi, f, 64) - double(over) * __shfl(w, f, 64);
+      };
+      uint32_t keep = c_all;
+      if (k > 0 && uint32_t(k) < keep) keep = uint32_t(k);
+      double mass = mass_of(keep);
+      const uint32_t first = keep;
+      if (p <= 0.0f) {
+        keep = 1;
+      } else if (p < 1.0f) {
+        const double target = double(p) * mass;
+        open(find([&](int s) { return sh.mass[s] >= target; }));
+        const int f = lane_of(__ballot(mi >= target && c != 0));
+        const uint32_t cf = __shfl(c, f, 64);
+        const double wf = __shfl(w, f, 64);
+        const double before = __shfl(mi, f, 64) - double(cf) * wf;
+        double q = __builtin_ceil((target - before) / wf);
+        q = q < 1.0 ? 1.0 : (q > double(cf) ? double(cf) : q);
+        keep = min(keep, uint32_t(__shfl(ci, f, 64)) - cf + uint32_t(q));
       }
-      *mi += seg ? sh.mass[seg - 1] : 0.0;
-      *ci += seg ? sh.count[seg - 1] : 0;
-    };
-    // the mass of the first `want` tokens (1 <= want <= c_all)
-    auto mass_of = [&](uint32_t want) {
-      if (want >= c_all) return m_all;
-      const int seg = find(c_before < want && want <= c_in);
-      uint32_t c, ci;
-      double w, mi;
-      open(seg, &c, &w);
-      prefix(seg, c, w, &ci, &mi);
-      const int f = __builtin_ctzll(__ballot(ci >= want) | (1ull << 63));
-      const uint32_t left = want - (__shfl(ci, f, 64) - __shfl(c, f, 64));
-      return __shfl(mi, f, 64) - double(__shfl(c, f, 64) - left) * __shfl(w, f, 64);
-    };
-    uint32_t keep = c_all;
-    const int32_t k = top_k ? top_k[row] : 0;
-    if (k > 0 && uint32_t(k) < keep) keep = uint32_t(k);
-    double mass = mass_of(keep);
-    const float p = top_p ? top_p[row] : 1.0f;
-    bool changed = false;
-    if (p <= 0.0f) {
-      keep = 1;
-      changed = true;
-    } else if (p < 1.0f) {
-      const double target = double(p) * mass;
-      const int seg = find(m_before < target && target <= m_in);
-      uint32_t c, ci;
-      double w, mi;
-      open(seg, &c, &w);
-      prefix(seg, c, w, &ci, &mi);
-      uint64_t past = __ballot(mi >= target && c != 0);
-      if (!past) past = 1ull << (63 - __builtin_clzll(__ballot(c != 0) | 1ull));
-      const int f = __builtin_ctzll(past);
-      const uint32_t cf = __shfl(c, f, 64);
-      const double wf = __shfl(w, f, 64);
+      if (floor_w > 0.0) keep = min(keep, sh.above);
+      keep = max(keep, 1u);
+      if (keep != first) mass = mass_of(keep);
+      const double at = (u > 0.0f ? (u < 1.0f ? double(u) : 1.0) : 0.0) * mass;
+      int seg = find([&](int s) { return sh.mass[s] > at; });
+      open(seg);
+      int f = lane_of(__ballot(mi > at && c != 0));
+      uint32_t cf = __shfl(c, f, 64);
+      double wf = __shfl(w, f, 64);
       const double before = __shfl(mi, f, 64) - double(cf) * wf;
-      double q = __builtin_ceil((target - before) / wf);
-      q = q < 1.0 ? 1.0 : (q > double(cf) ? double(cf) : q);
-      const uint32_t np = __shfl(ci, f, 64) - cf + uint32_t(q);
-      if (np < keep) {
-        keep = np;
-        changed = true;
+      double q = __builtin_floor((at - before) / wf);
+      q = q < 0.0 ? 0.0 : (q > double(cf - 1) ? double(cf - 1) : q);
+      uint32_t rank = uint32_t(q);  // among the value's tokens
+      if (uint32_t(__shfl(ci, f, 64)) - cf + rank >= keep) {  // a rounding past the last kept token
+        seg = find([&](int s) { return sh.count[s] >= keep; });
+        open(seg);
+        f = lane_of(__ballot(ci >= keep));
+        cf = __shfl(c, f, 64);
+        wf = __shfl(w, f, 64);
+        rank = keep - 1 - (uint32_t(__shfl(ci, f, 64)) - cf);
       }
-    }
-    const uint32_t least = sh.above;
-    if (floor_w > 0.0 && least < keep) {
-      keep = least;
-      changed = true;
-    }
-    if (keep < 1) {
-      keep = 1;
-      changed = true;
-    }
-    if (changed) mass = mass_of(keep);
-    const float u = uniform[row];
-    const double at = (u > 0.0f ? (u < 1.0f ? double(u) : 1.0) : 0.0) * mass;
-    const int seg = find(m_before <= at && at < m_in);
-    uint32_t c, ci;
-    double w, mi;
-    open(seg, &c, &w);
-    prefix(seg, c, w, &ci, &mi);
-    uint64_t past = __ballot(mi > at && c != 0);
-    if (!past) past = 1ull << (63 - __builtin_clzll(__ballot(c != 0) | 1ull));
-    int f = __builtin_ctzll(past);
-    const uint32_t cf = __shfl(c, f, 64);
-    const double wf = __shfl(w, f, 64);
-    const double before = __shfl(mi, f, 64) - double(cf) * wf;
-    double q = __builtin_floor((at - before) / wf);
-    q = q < 0.0 ? 0.0 : (q > double(cf - 1) ? double(cf - 1) : q);
-    uint32_t place = __shfl(ci, f, 64) - cf + uint32_t(q);  // among all tokens
-    double wt = wf;
-    uint32_t value = top - (uint32_t(seg) * 64 + f);
-    rank = uint32_t(q);
-    if (place >= keep) {  // a rounding past the last kept token
-      const int s2 = find(c_before < keep && keep <= c_in);
-      open(s2, &c, &w);
-      prefix(s2, c, w, &ci, &mi);
-      f = __builtin_ctzll(__ballot(ci >= keep) | (1ull << 63));
-      rank = keep - 1 - (__shfl(ci, f, 64) - __shfl(c, f, 64));
-      wt = __shfl(w, f, 64);
-      value = top - (uint32_t(s2) * 64 + f);
-    }
-    chosen = value;
-    if (t == 0) {
-      if (kept) kept[row] = int32_t(keep);
-      if (logprob) logprob[row] = float(log(wt / mass));
+      if (lane == 0) {
+        sh.chosen = 0xffffu - (uint32_t(seg) * 64 + f);
+        sh.rank = rank;
+        if (kept) kept[row] = int32_t(keep);
+        if (logprob) logprob[row] = float(log(wf / mass));
+      }
     }
   } else if (t == 0) {
+    sh.chosen = top;
+    sh.rank = 0;
     if (kept) kept[row] = 1;
     if (logprob) logprob[row] = 0.0f;
   }
-
-  // the id of the chosen value's rank-th token: matches per piece, then within one
-  __syncthreads();
-  for (int i = wave; i < pieces; i += kWaves) {
-    int c = 0;
-    each_of(i, [&](uint32_t k, int) { c += k == chosen; });
-    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
-    if (lane == 0) sh.pieces[i] = uint32_t(c);
-  }
-  __syncthreads();
-  if (wave != 0) return;
-  uint32_t before = 0;
-  for (int i0 = 0; i0 < pieces; i0 += 64) {
-    const uint32_t c = i0 + lane < pieces ? sh.pieces[i0 + lane] : 0;
+  // the part that holds the rank-th of the value's tokens (ids in order)
+  if (wave == 0) {
+    wave_sync();
+    const uint32_t d = 0xffffu - sh.chosen, seg = d >> 6, rank = sh.rank;
+    uint32_t c = 0;
+    if (lane < parts && (sh.bits[lane * 32 + (seg >> 5)] >> (seg & 31) & 1))
+      c = counts[int64_t(lane) * 65536 + d];
     uint32_t sum = c;
     for (int o = 1; o < 64; o <<= 1) {
       const uint32_t v = __shfl_up(sum, o, 64);
       sum += lane >= o ? v : 0;
     }
-    const uint64_t past = __ballot(before + sum > rank);
-    if (!past) {
-      before += __shfl(sum, 63, 64);
-      continue;
+    const int f = __builtin_ctzll(__ballot(sum > rank) | (1ull << 63));
+    const uint32_t before = uint32_t(__shfl(sum, f, 64)) - uint32_t(__shfl(c, f, 64));
+    if (lane == 0) {
+      sh.part = min(uint32_t(f), uint32_t(parts - 1));
+      sh.rank = rank - before;
     }
-    const int f = __builtin_ctzll(past);
-    before += __shfl(sum, f, 64) - __shfl(c, f, 64);
+  }
+  __syncthreads();
+  const uint32_t chosen = sh.chosen, rank = sh.rank;
+  const Row r(logits + int64_t(row) * stride, n);
+  const int each = (r.pieces() + parts - 1) / parts;
+  const int p0 = int(sh.part) * each, np = min(r.pieces(), p0 + each) - p0;
+  // matches of every piece, which its wave keeps
+  uint4 v[kWavePieces];
+#pragma unroll
+  for (int i = 0; i < kWavePieces; ++i)
+    if (wave + kWaves * i < np) v[i] = r.load(p0 + wave + kWaves * i, lane);
+#pragma unroll
+  for (int i = 0; i < kWavePieces; ++i) {
+    if (wave + kWaves * i >= np) continue;
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c += key_of(token_of(v[i], j)) == chosen;
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+    if (lane == 0) sh.pieces[wave + kWaves * i] = c;
+  }
+  __syncthreads();
+  // the piece that holds it: two a lane
+  const uint32_t a = 2 * lane < np ? sh.pieces[2 * lane] : 0;
+  const uint32_t b = 2 * lane + 1 < np ? sh.pieces[2 * lane + 1] : 0;
+  uint32_t sum = a + b;
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t x = __shfl_up(sum, o, 64);
+    sum += lane >= o ? x : 0;
+  }
+  const uint64_t past = __ballot(sum > rank);
+  if (!past) return;  // unreachable: the part's counters say that it is there
+  const int f = __builtin_ctzll(past);
+  uint32_t before = uint32_t(__shfl(sum, f, 64)) - uint32_t(__shfl(a + b, f, 64));
+  const uint32_t af = __shfl(a, f, 64);
+  const int piece = before + af > rank ? 2 * f : 2 * f + 1;
+  if (piece & 1) before += af;
+#pragma unroll
+  for (int i = 0; i < kWavePieces; ++i) {
+    if (piece != wave + kWaves * i) continue;  // uniform: one wave's one piece
     uint32_t own = 0;
-    each_of(i0 + f, [&](uint32_t k, int) { own += k == chosen; });
-    uint32_t mine = own;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) own += key_of(token_of(v[i], j)) == chosen;
+    uint32_t upto = own;
     for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t v = __shfl_up(mine, o, 64);
-      mine += lane >= o ? v : 0;
+      const uint32_t x = __shfl_up(upto, o, 64);
+      upto += lane >= o ? x : 0;
     }
-    uint32_t at = before + mine - own;
-    each_of(i0 + f, [&](uint32_t k, int id) {
-      if (k == chosen) {
-        if (at == rank) tokens[row] = uint32_t(id);
+    uint32_t at = before + upto - own;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (key_of(token_of(v[i], j)) == chosen) {
+        if (at == rank) tokens[row] = uint32_t(r.first(p0 + piece, lane) + j);
         ++at;
       }
-    });
-    return;
   }
+}
+
+// Parts of a row: enough workgroups for few rows, but no more than eight (launch 2
+// adds them up: at 151936 tokens it would then take as long as launch 1 saves), and
+// few enough tokens for 16-bit counters.
+int sample_parts(int rows, int n) {
+  const int pieces = (n + 7 + kPiece - 1) / kPiece;
+  const int least = (pieces + kPartPieces - 1) / kPartPieces;
+  int p = rows < 32 ? 8 : 256 / rows;
+  p = p < pieces / 4 ? p : pieces / 4;
+  p = p < 1 ? 1 : p;
+  return p > least ? p : least;
+}
+int sample_batch(int rows, int parts) {
+  const int b = kBatchParts / parts;
+  return rows < b ? rows : b;
 }
 
 }  // namespace
 
-size_t sample_workspace(int, int) { return 0; }
+size_t sample_workspace(int rows, int n) {
+  const int parts = sample_parts(rows, n);
+  return size_t(sample_batch(rows, parts)) * parts * (kHistBytes + 32 * 4 + 4);
+}
 
 int sample_bf16(const uint16_t* logits, int64_t stride, int rows, int n, const float* temperature,
                 const int32_t* top_k, const float* top_p, const float* min_p,
-                const float* uniform, uint32_t* tokens, float* logprob, int32_t* kept, void*,
-                hipStream_t s) {
-  if (hipFuncSetAttribute(reinterpret_cast<const void*>(sample_kernel),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, kHistBytes) != hipSuccess)
+                const float* uniform, uint32_t* tokens, float* logprob, int32_t* kept,
+                void* workspace, hipStream_t s) {
+  const int parts = sample_parts(rows, n), batch = sample_batch(rows, parts);
+  Parts ws;
+  ws.counts = static_cast<uint16_t*>(workspace);
+  ws.bits = reinterpret_cast<uint32_t*>(ws.counts + size_t(batch) * parts * 65536);
+  ws.top = ws.bits + size_t(batch) * parts * 32;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(count_kernel),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, kHistBytes) != hipSuccess ||
+      hipFuncSetAttribute(reinterpret_cast<const void*>(choose_kernel),
+                          hipFuncAttributeMaxDynamicSharedMemorySize,
+                          kSlots * 256) != hipSuccess)
     return MX_EHIP;
-  hipLaunchKernelGGL(sample_kernel, dim3(rows), dim3(kThreads), kHistBytes, s, logits, stride, n,
-                     temperature, top_k, top_p, min_p, uniform, tokens, logprob, kept);
-  return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;
+  // batches one after another on the stream share the workspace
+  for (int r = 0; r < rows; r += batch) {
+    const int m = rows - r < batch ? rows - r : batch;
+    const uint16_t* x = logits + int64_t(r) * stride;
+    hipLaunchKernelGGL(count_kernel, dim3(m * parts), dim3(kThreads), kHistBytes, s, x, stride, n,
+                       parts, ws);
+    if (hipGetLastError() != hipSuccess) return MX_EHIP;
+    hipLaunchKernelGGL(choose_kernel, dim3(m), dim3(kThreads), kSlots * 256, s, x, stride, n,
+                       parts, ws, temperature ? temperature + r : nullptr,
+                       top_k ? top_k + r : nullptr, top_p ? top_p + r : nullptr,
+                       min_p ? min_p + r : nullptr, uniform + r, tokens + r,
+                       logprob ? logprob + r : nullptr, kept ? kept + r : nullptr);
+    if (hipGetLastError() != hipSuccess) return MX_EHIP;
+  }
+  return MX_OK;
 }
 
 }  // namespace mx
