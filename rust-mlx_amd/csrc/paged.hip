@@ -202,13 +202,16 @@ __global__ __launch_bounds__(kQkThreads) void append_kernel(
 // k-slots that the same lane supplies as P^T for O^T = V^T P^T.  So scores never
 // leave their lane, and K and V come from memory straight into operands.  P is
 // split in two bf16 parts: the matrix cores have time, and P keeps 16 bits.
-constexpr int kDecodeTarget = 512;  // chunks wanted: two workgroups a compute unit
-
+constexpr int kDecodeMaxChunks = 2048 + 1;  // of one row: twice decode_target and the rounding
 template <bool F8>
 struct DecodeTile {
   static constexpr int kKeys = F8 ? 64 : 32;  // a lane's 16 bytes of V: 16 or 8 keys
   static constexpr int kUnit = 4 * kKeys;
 };
+// Workgroups that a compute unit holds, by registers.
+constexpr int decode_occupancy(int head_dim) { return head_dim == 256 ? 2 : head_dim == 128 ? 3 : 4; }
+// Chunks wanted: as many as run at once.
+int decode_target(const PageDims& d) { return 256 * decode_occupancy(d.head_dim); }
 
 // The length of a row's context, or -1 for a padding row.
 __device__ __forceinline__ int row_len(const int32_t* __restrict__ seqs,
@@ -216,38 +219,53 @@ __device__ __forceinline__ int row_len(const int32_t* __restrict__ seqs,
                                        int rows) {
   if (r >= rows) return -1;
   const int seq = seqs ? seqs[r] : r;
-  if (unsigned(seq) >= unsigned(d.sequences)) return -1;
-  const int64_t most = int64_t(d.table_width) << d.page_log2;
   const int len = lens[r];
-  return len < 0 ? 0 : (len > most ? int(most) : len);
+  if (unsigned(seq) >= unsigned(d.sequences)) return -1;
+  const int most = int(min(int64_t(d.table_width) << d.page_log2, int64_t(0x7fffffff)));
+  return len < 0 ? 0 : min(len, most);
 }
 
-__device__ __forceinline__ int wave_sum(int v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+__device__ __forceinline__ int units_of(int len, int unit) {
+  return len > 0 ? (len + unit - 1) / unit : 0;
 }
 
-// Units of a chunk: the smallest with at most kDecodeTarget chunks beside the rounding of each row.
-__device__ __forceinline__ int plan_chunk(const int32_t* seqs, const int32_t* lens,
-                                          const PageDims& d, int rows, int unit) {
+// The plan, formed by every wave: the most units of a chunk (a row's chunks are even), the
+// fewest that give at most `target` chunks (or two rounds of them, where they are long) where
+// some number up to twice the even share does; `len0`: the lengths of the first 64 rows, a lane each.
+struct Plan {
+  int chunk_units, len0;
+};
+__device__ __forceinline__ Plan make_plan(const int32_t* seqs, const int32_t* lens,
+                                          const PageDims& d, int rows, int unit, int target) {
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int r = 0; r < rows; r += 64) {
-    const int len = row_len(seqs, lens, d, r + lane, rows);
-    total += wave_sum(len > 0 ? (len + unit - 1) / unit : 0);
-  }
-  const int64_t c = (total * d.kv_heads + kDecodeTarget - 1) / kDecodeTarget;
-  return c < 1 ? 1 : int(c);
+  Plan p;
+  p.len0 = row_len(seqs, lens, d, lane, rows);
+  auto sum = [&](auto&& of) {
+    int64_t total = __builtin_amdgcn_readlane(wave_scan(of(units_of(p.len0, unit))), 63);
+    for (int r = 64; r < rows; r += 64)
+      total += __builtin_amdgcn_readlane(
+          wave_scan(of(units_of(row_len(seqs, lens, d, r + lane, rows), unit))), 63);
+    return total * d.kv_heads;
+  };
+  const int64_t total = sum([](int u) { return u; });
+  if (total >= 16 * int64_t(target)) target *= 2;  // long chunks: a second round evens out the units' speeds
+  const int64_t share = (total + target - 1) / target;
+  const int c0 = share < 1 ? 1 : int(share), step = (c0 + 7) / 8;
+  int c = c0;
+  while (c < 2 * c0 && sum([&](int u) { return (u + c - 1) / c; }) > target) c += step;
+  p.chunk_units = c;
+  return p;
 }
 
 template <int HD, bool F8>
-__global__ __launch_bounds__(256, 2) void decode_kernel(
+__global__ __launch_bounds__(256, decode_occupancy(HD)) void decode_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
     const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
     const int32_t* __restrict__ table, const void* __restrict__ k_cache,
     const void* __restrict__ v_cache, const float* __restrict__ k_scale,
-    const float* __restrict__ v_scale, PageDims d, float scale, float* __restrict__ o_part,
-    float* __restrict__ ml_part, uint16_t* __restrict__ out) {
+    const float* __restrict__ v_scale, PageDims d, float scale, int target,
+    float* __restrict__ o_part, float* __restrict__ ml_part, int2* __restrict__ row_chunks,
+    uint16_t* __restrict__ out) {
   constexpr int KT = DecodeTile<F8>::kKeys, kUnit = DecodeTile<F8>::kUnit;
   constexpr int T = KT / 16;        // score tiles
   constexpr int KG = KT / 4;        // keys of a lane quarter
@@ -261,50 +279,41 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(
   __shared__ __align__(16) uint16_t qs[16 * QLD];
   __shared__ float mls[2][4][16];
   extern __shared__ __align__(16) float os[];  // [4 waves][group][OLD]
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int col = lane & 15, g = lane >> 4;
   const int group = d.heads / d.kv_heads;
   // this workgroup's (row, chunk, kv head)
   const int item = blockIdx.x, kvh = item % d.kv_heads;
   const int want = item / d.kv_heads;
-  const int cu = plan_chunk(seqs, lens, d, rows, kUnit);
-  int row = -1, chunk = 0, before = 0, len = 0;
+  const Plan plan = make_plan(seqs, lens, d, rows, kUnit, target);
+  const int cu = plan.chunk_units;
+  int row = -1, chunk = 0, chunks = 0, before = 0, len = 0;
   for (int r = 0; r < rows; r += 64) {
-    const int l = row_len(seqs, lens, d, r + lane, rows);
-    const int units = l > 0 ? (l + kUnit - 1) / kUnit : 0;
-    const int n = (units + cu - 1) / cu;
-    int sum = n;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(sum, o, 64);
-      sum += lane >= o ? v : 0;
-    }
+    const int l = r == 0 ? plan.len0 : row_len(seqs, lens, d, r + lane, rows);
+    const int n = (units_of(l, kUnit) + cu - 1) / cu;
+    const int sum = wave_scan(n);
     const uint64_t past = __ballot(before + sum > want);
     if (past) {
       const int f = __builtin_ctzll(past);
       row = r + f;
-      len = __shfl(l, f, 64);
-      chunk = want - (before + __shfl(sum, f, 64) - __shfl(n, f, 64));
+      len = __builtin_amdgcn_readlane(l, f);
+      chunks = __builtin_amdgcn_readlane(n, f);
+      before += __builtin_amdgcn_readlane(sum, f) - chunks;
+      chunk = want - before;
+      if (chunk == 0 && kvh == 0 && t == 0)  // for the launch that joins
+        row_chunks[row] = make_int2(before, chunks);
       break;
     }
-    before += __shfl(sum, 63, 64);
+    before += __builtin_amdgcn_readlane(sum, 63);
   }
   if (row < 0) return;  // uniform: past the last chunk
   const int seq = seqs ? seqs[row] : row;
-  const int k0 = chunk * cu * kUnit;
-  const int k1 = min(len, k0 + cu * kUnit);  // k0 < len
+  // units / chunks each, the first ones one more
+  const int units = units_of(len, kUnit), few = units / chunks, more_units = units % chunks;
+  const int k0 = (chunk * few + min(chunk, more_units)) * kUnit;
+  const int k1 = min(len, k0 + (few + (chunk < more_units)) * kUnit);  // k0 < k1
   const bool whole = k0 == 0 && k1 == len;
   const int last_page = (len - 1) >> d.page_log2;
-
-  // q heads into LDS (rows past the group zero)
-  for (int i = t; i < 16 * HD / 8; i += 256) {
-    const int h = i / (HD / 8), piece = i % (HD / 8);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (h < group)
-      v = *reinterpret_cast<const uint4*>(
-          q + (int64_t(row) * d.heads + kvh * group + h) * HD + 8 * piece);
-    *reinterpret_cast<uint4*>(qs + h * QLD + 8 * piece) = v;
-  }
-  __syncthreads();
 
   const char* kc = static_cast<const char*>(k_cache);
   const char* vc = static_cast<const char*>(v_cache);
@@ -353,9 +362,19 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(
     load_k(tile);
     load_v(tile);
   }
+  // q heads into LDS (rows past the group zero), under the first tile's way
+  for (int i = t; i < 16 * HD / 8; i += 256) {
+    const int h = i / (HD / 8), piece = i % (HD / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (h < group)
+      v = *reinterpret_cast<const uint4*>(
+          q + (int64_t(row) * d.heads + kvh * group + h) * HD + 8 * piece);
+    *reinterpret_cast<uint4*>(qs + h * QLD + 8 * piece) = v;
+  }
+  __syncthreads();
   for (; tile < k1; tile += kUnit) {
-    // q is read again for every tile: held, its 32 registers would spill at 256 dims
-    if constexpr (HD == 256) asm volatile("" ::: "memory");
+    // q is read again for every tile where its registers (up to 32) would spill, held
+    if constexpr (HD == 256 || (HD == 128 && F8)) asm volatile("" ::: "memory");
     // valid keys of this lane quarter
     const int nk = pv < 0 ? 0 : min(max(k1 - (tile + vrow), 0), KG);
     floatx4_t sc[T];
@@ -510,62 +529,91 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(
   }
 }
 
-// Joins the chunks of one (row, head), four waves taking every fourth one, in a
-// fixed order; rows without keys become 0, rows of one chunk are done already.
-template <int HD>
-__global__ __launch_bounds__(256) void decode_join_kernel(
+// Joins the chunks of DW dims of one (row, head) in a fixed order; rows without
+// keys become 0, rows of one chunk are done already.  Each wave takes every NW-th
+// chunk, eight at a time, whose sums are on their way while the weights form.
+template <int HD, int DW, int NW>
+__global__ __launch_bounds__(64 * NW) void decode_join_kernel(
     const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
     const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
-    const float* __restrict__ v_scale, PageDims d, int unit, const float* __restrict__ o_part,
-    const float* __restrict__ ml_part, uint16_t* __restrict__ out) {
-  constexpr int DPL = HD / 64;
-  __shared__ float ls[4];
-  __shared__ float os[4][HD];
-  const int head = blockIdx.x % d.heads, row = blockIdx.x / d.heads;
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const float* __restrict__ v_scale, PageDims d, const int2* __restrict__ row_chunks,
+    const float* __restrict__ o_part, const float* __restrict__ ml_part,
+    uint16_t* __restrict__ out) {
+  constexpr int DB = HD / DW, DPL = DW / 64;
+  typedef float vec __attribute__((ext_vector_type(DPL)));
+  __shared__ float ws[kDecodeMaxChunks];
+  __shared__ float red[2][NW];
+  __shared__ vec os[NW][64];
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+  const int dim = DW * (blockIdx.x % DB) + DPL * lane;
+  const int head = blockIdx.x / DB % d.heads, row = blockIdx.x / DB / d.heads;
   const int group = d.heads / d.kv_heads, kvh = head / group;
   const int len = row_len(seqs, lens, d, row, rows);
+  const int2 rc = row_chunks[row];  // meaningful where there are keys
   if (len < 0) return;
-  uint16_t* dst = out + (int64_t(row) * d.heads + head) * HD;
+  uint16_t* dst = out + (int64_t(row) * d.heads + head) * HD + dim;
   if (len == 0) {
-    if (t < HD) dst[t] = 0;
+    if (wave == 0)
+      for (int i = 0; i < DPL; ++i) dst[i] = 0;
     return;
   }
-  const int cu = plan_chunk(seqs, lens, d, rows, unit);
-  const int units = (len + unit - 1) / unit, n = (units + cu - 1) / cu;
-  if (n == 1) return;
-  int64_t before = 0;
-  for (int r = 0; r < row; r += 64) {
-    const int l = r + lane < row ? row_len(seqs, lens, d, r + lane, rows) : 0;
-    before += wave_sum(l > 0 ? ((l + unit - 1) / unit + cu - 1) / cu : 0);
-  }
-  const int64_t step = int64_t(d.kv_heads) * group;
-  const int64_t part0 = before * step + head;
+  const int n = rc.y;  // 2 .. kDecodeMaxChunks
+  if (n <= 1) return;
+  const int64_t part0 = int64_t(rc.x) * d.heads + head;  // chunk c's partial: c heads further on
+  auto part_of = [&](int c) {
+    return *reinterpret_cast<const vec*>(o_part + (part0 + int64_t(c) * d.heads) * HD + dim);
+  };
+  vec v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = part_of(min(wave + NW * i, n - 1));
   float M = neg_inf();
-  for (int c = lane; c < n; c += 64) M = fmaxf(M, ml_part[(part0 + c * step) * 2]);
+  for (int c = t; c < n; c += 64 * NW) M = fmaxf(M, ml_part[(part0 + int64_t(c) * d.heads) * 2]);
   for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  const float ref = M == neg_inf() ? 0.0f : M;
-  float L = 0.0f, O[DPL];
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) O[i] = 0.0f;
-#pragma unroll 4
-  for (int c = wave; c < n; c += 4) {
-    const int64_t p = part0 + c * step;
-    const float e = __builtin_amdgcn_exp2f(ml_part[p * 2] - ref);
-    L = fmaf_(ml_part[p * 2 + 1], e, L);
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) O[i] = fmaf_(o_part[p * HD + 64 * i + lane], e, O[i]);
-  }
-  if (lane == 0) ls[wave] = L;
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) os[wave][64 * i + lane] = O[i];
+  if (lane == 0) red[0][wave] = M;
   __syncthreads();
-  if (t >= HD) return;
-  const float l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
-  float y = (os[0][t] + os[1][t]) + (os[2][t] + os[3][t]);
-  y = l == 0.0f ? 0.0f : y / l * (v_scale ? v_scale[kvh] : 1.0f);
-  if (d.gated) y *= gate_of(bf16_to_f32(qkv[int64_t(row) * qkv_stride + int64_t(head) * 2 * HD + HD + t]));
-  dst[t] = f32_to_bf16(y);
+#pragma unroll
+  for (int w = 0; w < NW; ++w) M = fmaxf(M, red[0][w]);
+  const float ref = M == neg_inf() ? 0.0f : M;
+  float L = 0.0f;
+  for (int c = t; c < n; c += 64 * NW) {
+    const float2 ml = *reinterpret_cast<const float2*>(ml_part + (part0 + int64_t(c) * d.heads) * 2);
+    const float e = __builtin_amdgcn_exp2f(ml.x - ref);
+    ws[c] = e;
+    L = fmaf_(ml.y, e, L);
+  }
+  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+  if (lane == 0) red[1][wave] = L;
+  __syncthreads();
+  vec O = 0.0f;
+  for (int c0 = wave; c0 < n; c0 += 8 * NW) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c0 + NW * i < n) {  // uniform
+        const float e = ws[c0 + NW * i];
+        for (int k = 0; k < DPL; ++k) O[k] = fmaf_(v[i][k], e, O[k]);
+      }
+    if (c0 + 8 * NW < n) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = part_of(min(c0 + NW * (8 + i), n - 1));
+    }
+  }
+  os[wave][lane] = O;
+  __syncthreads();
+  if (wave != 0) return;
+  L = red[1][0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    L += red[1][w];
+    O += os[w][lane];
+  }
+  const float inv = (L == 0.0f ? 0.0f : 1.0f / L) * (v_scale ? v_scale[kvh] : 1.0f);
+  const uint16_t* gp = qkv + int64_t(row) * qkv_stride + int64_t(head) * 2 * HD + HD + dim;
+#pragma unroll
+  for (int k = 0; k < DPL; ++k) {
+    float y = L == 0.0f ? 0.0f : O[k] * inv;
+    if (d.gated) y *= gate_of(bf16_to_f32(gp[k]));
+    dst[k] = f32_to_bf16(y);
+  }
 }
 
 int decode_unit(const PageDims& d) {
@@ -577,7 +625,8 @@ int64_t decode_items(int rows, const PageDims& d) {
   const int64_t unit = decode_unit(d);
   const int64_t most = ((int64_t(d.table_width) << d.page_log2) + unit - 1) / unit;
   const int64_t all = int64_t(rows) * d.kv_heads;
-  return all * most < kDecodeTarget + all ? all * most : kDecodeTarget + all;
+  const int64_t target = 2 * decode_target(d);
+  return all * most < target + all ? all * most : target + all;
 }
 
 }  // namespace
@@ -606,7 +655,8 @@ int paged_append(const uint16_t* qkv, int64_t qkv_stride, int rows, const int32_
 }
 
 size_t paged_decode_workspace(int rows, const PageDims& d) {
-  return size_t(decode_items(rows, d)) * (d.heads / d.kv_heads) * (d.head_dim + 2) * 4;
+  return size_t(decode_items(rows, d)) * (d.heads / d.kv_heads) * (d.head_dim + 2) * 4 +
+         size_t(rows) * 8;
 }
 
 int paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int rows,
@@ -620,6 +670,12 @@ int paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int
   float* o_part = static_cast<float*>(workspace);
   float* ml_part = o_part + items * group * d.head_dim;
   const int lds = 4 * group * (d.head_dim + 4) * 4;
+  int2* row_chunks = reinterpret_cast<int2*>(ml_part + items * group * 2);
+  const int target = decode_target(d);
+#define MX_JOIN(HH, DW, NW)                                                                      \
+  hipLaunchKernelGGL((decode_join_kernel<HH, DW, NW>), dim3(unsigned(joins * (HH / DW))),        \
+                     dim3(64 * NW), 0, s, qkv, qkv_stride, rows, seqs, lens,                     \
+                     d.f8 ? v_scale : nullptr, d, row_chunks, o_part, ml_part, out)
 #define MX_DECODE(HH, FF)                                                                        \
   if (d.head_dim == HH && d.f8 == FF) {                                                          \
     const auto fn = decode_kernel<HH, FF>;                                                       \
@@ -627,17 +683,20 @@ int paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int
                             hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)      \
       return MX_EHIP;                                                                            \
     hipLaunchKernelGGL(fn, dim3(unsigned(items)), dim3(256), lds, s, q, qkv, qkv_stride, rows,   \
-                       seqs, lens, table, k_cache, v_cache, k_scale, v_scale, d, scale, o_part,  \
-                       ml_part, out);                                                            \
+                       seqs, lens, table, k_cache, v_cache, k_scale, v_scale, d, scale, target,  \
+                       o_part, ml_part, row_chunks, out);                                        \
     if (hipGetLastError() != hipSuccess) return MX_EHIP;                                         \
-    hipLaunchKernelGGL((decode_join_kernel<HH>), dim3(unsigned(joins)), dim3(256), 0, s, qkv,    \
-                       qkv_stride, rows, seqs, lens, FF ? v_scale : nullptr, d, decode_unit(d),  \
-                       o_part, ml_part, out);                                                    \
+    /* few rows have many chunks each */                                                         \
+    if (joins <= 64)                                                                             \
+      MX_JOIN(HH, 64, 16);                                                                       \
+    else                                                                                         \
+      MX_JOIN(HH, HH, 4);                                                                          \
     return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;                                    \
   }
   MX_DECODE(64, false) MX_DECODE(128, false) MX_DECODE(256, false)
   MX_DECODE(64, true) MX_DECODE(128, true) MX_DECODE(256, true)
 #undef MX_DECODE
+#undef MX_JOIN
   return MX_EUNSUPPORTED;
 }
 

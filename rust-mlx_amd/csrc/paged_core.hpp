@@ -53,11 +53,27 @@ __device__ __forceinline__ float gate_of(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
 }
 
-// Sixteen bytes a lane from memory to LDS: lane l's land at lds + 16 l (lds: the same for the wave).
-__device__ __forceinline__ void copy_to_lds(const char* src, char* lds) {
-  __builtin_amdgcn_global_load_lds(
-      src, reinterpret_cast<__attribute__((address_space(3))) void*>(reinterpret_cast<uintptr_t>(lds)),
-      16, 0, 0);
+// Sixteen bytes a lane from memory to LDS: lane l's land at lds + 16 l (lds: the same for the
+// wave), once the wave has waited for its vector memory (copies_done).  Written out because
+// the compiler takes every later LDS read for one of these bytes and waits for the copy at
+// once; here a tile's copy runs under the work on the tile before.
+__device__ __forceinline__ void copy_to_lds(const char* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(src), "s"(lds)
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Sums over the lanes up to each one (all 64 lanes active), in registers.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0's and 2's last to 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31's to rows 2 and 3
+  return v;
 }
 
 // The page id of table entry `index` of `seq`, or -1 where it names no page of the cache.

@@ -63,24 +63,21 @@ __device__ __forceinline__ bool find_block(const int32_t* __restrict__ starts,
       count = max(min(starts[s + 1], rows) - first, 0);
     }
     const int n = int((int64_t(count) * group + kPairs - 1) / kPairs);
-    int sum = n;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(sum, o, 64);
-      sum += lane >= o ? v : 0;
-    }
+    const int sum = wave_scan(n);
     const uint64_t past = __ballot(before + sum > want);
     if (past) {
       const int f = __builtin_ctzll(past);
-      out->seq = s0 + f;
-      out->first = __shfl(first, f, 64);
-      out->count = __shfl(count, f, 64);
-      out->pair0 = (before + __shfl(sum, f, 64) - 1 - want) * kPairs;
+      // uniform values, into scalar registers
+      out->seq = __builtin_amdgcn_readfirstlane(s0 + f);
+      out->first = __builtin_amdgcn_readlane(first, f);
+      out->count = __builtin_amdgcn_readlane(count, f);
+      out->pair0 = (before + __builtin_amdgcn_readlane(sum, f) - 1 - want) * kPairs;
       const int64_t most = int64_t(d.table_width) << d.page_log2;
-      const int len = lens[s0 + f];
+      const int len = lens[out->seq];
       out->len = len < 0 ? 0 : (len > most ? int(most) : len);
       return true;
     }
-    before += __shfl(sum, 63, 64);
+    before += __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
 }
@@ -112,7 +109,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
   constexpr int NVV = HD * VP / 256;   // V pieces a thread copies
   constexpr int RPW = KT / 4;          // K rows a wave copies (8 or 16: one page)
   extern __shared__ __align__(16) char lds[];  // two stages of [K | V^T]
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int col = lane & 31, h = lane >> 5;
   const int group = d.heads / d.kv_heads;
   const int item = blockIdx.x;
@@ -160,60 +157,57 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
   const float sl2 = scale * kLog2e * (F8 && k_scale ? k_scale[kvh] : 1.0f);
   const int64_t head_at = (int64_t(kvh) << d.page_log2) * HD;
 
-  // page ids: of the wave's K rows, and of this lane's V piece; all four 16-key
-  // parts of a tile are checked by every wave
-  auto id_at = [&](int key) { return page_at(table, d, b.seq, min(key >> d.page_log2, last_page)); };
-  // bit i: keys 16 i .. 16 i + 15 of the tile lie in a page
-  auto parts_of = [&](int tile) {
-    const int part = lane & (KT / 16 - 1);
-    return uint32_t(__ballot(id_at(tile + 16 * part) >= 0)) & ((1u << (KT / 16)) - 1u);
+  // Page ids of a tile: of the wave's K rows, of this lane's V pieces, and, on lanes
+  // 0 .. KT/16 - 1, of its 16-key parts.  They are read two tiles ahead, the copy one.
+  struct Ids {
+    int k, v, part;
   };
+  constexpr int VL = F8 ? VP / 2 : VP;  // lanes that copy one V^T row
+  const int vdim = wave * (HD / 4) + lane / VL;
+  // the lane's keys of the rows that it copies: the same piece of every row
+  const int vkey = F8 ? 16 * (lane % VL) : 8 * ((lane % VL) ^ v_swizzle<HD>(vdim));
+  auto id_at = [&](int key) { return page_at(table, d, b.seq, min(key >> d.page_log2, last_page)); };
+  auto ids_of = [&](int tile) {
+    return Ids{id_at(tile + RPW * wave), id_at(tile + vkey),
+               id_at(tile + 16 * (lane & (KT / 16 - 1)))};
+  };
+  constexpr uint32_t kAllParts = (1u << (KT / 16)) - 1u;
 
   // One tile's copy.  Slot i of a stage's K part is piece i % KP of row i / KP
   // and holds that row's piece (i % KP) ^ swizzle(row); V^T alike.
   constexpr int kStage = stage_bytes<HD>();
   constexpr int kVAt = KT * HD * 2;
+  const uint32_t lds_at = uint32_t(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) char*)lds));
   uint4 kreg[F8 ? NK / 2 : 1], vreg[F8 ? NVV / 2 : 1];
-  auto copy = [&](int tile, int stage) {
-    char* ks = lds + stage * kStage;
-    char* vs = ks + kVAt;
-    const int kid = max(id_at(tile + RPW * wave), 0);
+  auto copy = [&](int tile, int stage, const Ids& id) {
+    const int kid = __builtin_amdgcn_readfirstlane(max(id.k, 0));
+    const int vid = max(id.v, 0);
+    const char* kbase =
+        kc + (kid * d.page_stride + head_at + int64_t((tile + RPW * wave) & (page - 1)) * HD) * E;
+    const char* vbase = vc + (vid * d.page_stride + head_at + (int64_t(vdim) << d.page_log2) +
+                              ((tile + vkey) & (page - 1))) * E;
     if constexpr (!F8) {
-      const char* kbase =
-          kc + (kid * d.page_stride + head_at + int64_t((tile + RPW * wave) & (page - 1)) * HD) * E;
+      const uint32_t ks = lds_at + stage * kStage + RPW * wave * KP * 16;
+      const uint32_t vs = lds_at + stage * kStage + kVAt + wave * (HD / 4) * VP * 16;
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
         const int slot = 64 * i + lane, r = slot / KP, p = slot % KP;
-        const int row = RPW * wave + r;
-        copy_to_lds(kbase + (r * HD + 8 * (p ^ k_swizzle<HD>(row))) * E,
-                    ks + (RPW * wave * KP + 64 * i) * 16);
+        copy_to_lds(kbase + (r * HD + 8 * (p ^ k_swizzle<HD>(RPW * wave + r))) * E, ks + 1024 * i);
       }
-      const int dim0 = wave * (HD / 4) + lane / VP;
-      const int piece = (lane % VP) ^ v_swizzle<HD>(dim0);  // the same for every dim of this lane
-      const int vid = max(id_at(tile + 8 * piece), 0);
-      const char* vbase = vc + (vid * d.page_stride + head_at + (int64_t(dim0) << d.page_log2) +
-                                ((tile + 8 * piece) & (page - 1))) * E;
 #pragma unroll
       for (int i = 0; i < NVV; ++i)
-        copy_to_lds(vbase + (int64_t(64 / VP * i) << d.page_log2) * E,
-                    vs + (wave * (HD / 4) * VP + 64 * i) * 16);
+        copy_to_lds(vbase + (int64_t(64 / VP * i) << d.page_log2) * E, vs + 1024 * i);
     } else {
       // 16 e4m3 values at a time: two neighbouring pieces
-      const char* kbase =
-          kc + kid * d.page_stride + head_at + int64_t((tile + RPW * wave) & (page - 1)) * HD;
 #pragma unroll
       for (int i = 0; i < NK / 2; ++i) {
         const int slot = 64 * i + lane, r = slot / (KP / 2), p = slot % (KP / 2);
         kreg[i] = *reinterpret_cast<const uint4*>(kbase + r * HD + 16 * p);
       }
-      const int dim0 = wave * (HD / 4) + lane / (VP / 2), p = lane % (VP / 2);
-      const int vid = max(id_at(tile + 16 * p), 0);
-      const char* vbase = vc + vid * d.page_stride + head_at + (int64_t(dim0) << d.page_log2) +
-                          ((tile + 16 * p) & (page - 1));
 #pragma unroll
       for (int i = 0; i < NVV / 2; ++i)
-        vreg[i] =
-            *reinterpret_cast<const uint4*>(vbase + (int64_t(64 / (VP / 2) * i) << d.page_log2));
+        vreg[i] = *reinterpret_cast<const uint4*>(vbase + (int64_t(64 / VL * i) << d.page_log2));
     }
   };
   auto store = [&](int stage) {
@@ -229,7 +223,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
       }
 #pragma unroll
       for (int i = 0; i < NVV / 2; ++i) {
-        const int dim = wave * (HD / 4) + 64 / (VP / 2) * i + lane / (VP / 2), p = lane % (VP / 2);
+        const int dim = vdim + 64 / VL * i, p = lane % VL;
         const int sw = v_swizzle<HD>(dim);
         *reinterpret_cast<uint4*>(vs + (dim * VP + ((2 * p) ^ sw)) * 16) = widen8(vreg[i].x, vreg[i].y);
         *reinterpret_cast<uint4*>(vs + (dim * VP + ((2 * p + 1) ^ sw)) * 16) = widen8(vreg[i].z, vreg[i].w);
@@ -244,49 +238,55 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
 
+  Ids now = ids_of(tile0 * KT), next = ids_of((tile0 + 1) * KT);
   if (tile0 < tile1) {
-    copy(tile0 * KT, 0);
+    copy(tile0 * KT, 0, now);
     store(0);
   }
   const int krow = (col & 0x13) | ((col & 4) << 1) | ((col & 8) >> 1);  // bits 2 and 3 exchanged
   for (int ti = tile0; ti < tile1; ++ti) {
     const int tile = ti * KT, stage = (ti - tile0) & 1;
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile is in LDS
-    __syncthreads();                     // everyone's is; the other stage is consumed
-    const uint32_t parts = parts_of(tile);
-    const int kend = min(b.len, kall);
-    const bool ragged = tile + KT > kend || parts != (1u << (KT / 16)) - 1u;
+    copies_done();    // this wave's part of the tile is in LDS, and `next` is here
+    __syncthreads();  // everyone's is; the other stage is consumed
+    const uint32_t parts = uint32_t(__ballot(now.part >= 0)) & kAllParts;
+    const bool ragged = tile + KT > kall || parts != kAllParts;
     char* ks = lds + stage * kStage;
     char* vs = ks + kVAt;
     if (ragged) {  // uniform: V of positions that are no keys may be anything, and becomes 0
       for (int i = t; i < HD * VP; i += 256) {
         const int dim = i / VP, key0 = 8 * ((i % VP) ^ v_swizzle<HD>(dim));
-        const int n = (parts >> (key0 >> 4)) & 1 ? min(max(kend - tile - key0, 0), 8) : 0;
+        const int n = (parts >> (key0 >> 4)) & 1 ? min(max(kall - tile - key0, 0), 8) : 0;
         if (n == 8) continue;
         uint16_t* p = reinterpret_cast<uint16_t*>(vs + i * 16);
         for (int j = n; j < 8; ++j) p[j] = 0;
       }
       __syncthreads();
     }
-    if (ti + 1 < tile1) copy((ti + 1) * KT, stage ^ 1);
+    now = next;
+    if (ti + 1 < tile1) {
+      copy((ti + 1) * KT, stage ^ 1, now);
+      next = ids_of((ti + 2) * KT);
+    }
     if (tile <= high) {
       floatx16_t sc[KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[kb][r] = 0.0f;
-        const int row = 32 * kb + krow;
-        const char* krp = ks + row * KP * 16;
-        const int sw = k_swizzle<HD>(row);
+      const char* krp = ks + krow * KP * 16;
+      int swap = h ^ k_swizzle<HD>(krow);  // of krow + 32 alike
+      asm("" : "+v"(swap));                // formed anew for every tile: held, the addresses spill
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const uint4 a = *reinterpret_cast<const uint4*>(krp + ((2 * s + h) ^ sw) * 16);
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const uint4 a =
+              *reinterpret_cast<const uint4*>(krp + ((2 * s) ^ swap) * 16 + kb * (32 * KP * 16));
           sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                            __builtin_bit_cast(bf16x8_t, qb[s]),
                                                            sc[kb], 0, 0, 0);
         }
-      }
-      if (tile + KT - 1 > low || parts != (1u << (KT / 16)) - 1u) {
+      if (tile + KT - 1 > low || parts != kAllParts) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -302,10 +302,11 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sc[kb][r]);
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * sl2;
-      const float mn = fmaxf(m_run, mt);
-      const float ref = mn == neg_inf() ? 0.0f : mn;  // no key yet: every weight is 0
-      if (__any(mn != m_run)) {
-        const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
+      // The reference follows the maximum in steps of at least 8 (a factor of 256, far from any
+      // limit of fp32 or bf16), so that most tiles rescale nothing.
+      if (__any(mt > m_run + 8.0f || m_run == neg_inf())) {
+        const float mn = fmaxf(m_run, mt);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - (mn == neg_inf() ? 0.0f : mn));
         l_run *= alpha;
 #pragma unroll
         for (int n = 0; n < ND; ++n)
@@ -313,6 +314,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
           for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
         m_run = mn;
       }
+      const float ref = m_run == neg_inf() ? 0.0f : m_run;  // no key yet: every weight is 0
       uint32_t pb[KB * 8];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -323,15 +325,15 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
           l_run += x + y;
           pb[8 * kb + r / 2] = pack2(x, y);
         }
+      const int vswap = h ^ v_swizzle<HD>(col);  // of col + 32 n alike
 #pragma unroll
       for (int s = 0; s < 2 * KB; ++s) {
         const bf16x8_t p = __builtin_bit_cast(
             bf16x8_t, make_uint4(pb[4 * s], pb[4 * s + 1], pb[4 * s + 2], pb[4 * s + 3]));
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
-          const int dim = 32 * n + col;
-          const uint4 a =
-              *reinterpret_cast<const uint4*>(vs + (dim * VP + ((2 * s + h) ^ v_swizzle<HD>(dim))) * 16);
+          const uint4 a = *reinterpret_cast<const uint4*>(
+              vs + (col * VP + ((2 * s) ^ vswap)) * 16 + n * (32 * VP * 16));
           o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), p, o[n],
                                                          0, 0, 0);
         }
