@@ -63,7 +63,17 @@ __device__ __forceinline__ void copy_to_lds(const char* src, uint32_t lds) {
                : "v"(src), "s"(lds)
                : "memory");
 }
-__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits until at most `N` of the wave's vector memory operations, the latest, are under way.
+template <int N>
+__device__ __forceinline__ void copies_done() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+// The larger of this lane's value and that of the lane 32 away.
+__device__ __forceinline__ float max_across_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+  return fmaxf(u2f(r[0]), u2f(r[1]));
+}
 
 // Sums over the lanes up to each one (all 64 lanes active), in registers.
 __device__ __forceinline__ int wave_scan(int v) {

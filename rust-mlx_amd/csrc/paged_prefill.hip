@@ -25,6 +25,9 @@
 //
 // With few workgroups the keys are split over several, and a second launch
 // joins their partials.
+#include <type_traits>
+#include <utility>
+
 #include "paged_core.hpp"
 
 namespace mx {
@@ -33,7 +36,9 @@ namespace {
 
 using namespace pg;
 
-constexpr int kPairs = 128;  // pairs of a workgroup: 32 a wave
+constexpr int NW = 4;            // waves of a workgroup
+constexpr int D = 2;             // stages of a tile in LDS
+constexpr int kPairs = 32 * NW;  // its pairs
 
 // Keys of a tile: two stages of K and V fit twice into a compute unit's LDS.
 template <int HD>
@@ -43,6 +48,19 @@ constexpr int tile_keys() {
 template <int HD>
 constexpr int stage_bytes() {
   return 2 * tile_keys<HD>() * HD * 2;  // K and V
+}
+
+// Lambdas that hold registers by reference: a call would put them into memory.
+#define MX_LAMBDA __attribute__((always_inline))
+
+// f(integral_constant<int, 0>) .. f(integral_constant<int, N - 1>)
+template <class F, int... I>
+__device__ __forceinline__ void each_(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  each_(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
 }
 
 // The sequence and block of query block `want`; a sequence's blocks in reverse
@@ -82,6 +100,24 @@ __device__ __forceinline__ bool find_block(const int32_t* __restrict__ starts,
   return false;
 }
 
+// The query block, kv head and split of a workgroup.  Workgroups go to the eight XCDs in turn
+// (id mod 8).  Those of one kv head and split read the same keys, whatever their block, so with
+// eight such pairs or more each XCD takes whole pairs, and its L2 what they read.
+struct Item {
+  int block, kvh, split;
+};
+__host__ __device__ __forceinline__ bool by_xcd(int kv_heads, int splits) {
+  return kv_heads * splits >= 8;
+}
+__device__ __forceinline__ Item item_of(int id, int kv_heads, int splits) {
+  const int pairs = kv_heads * splits;
+  if (!by_xcd(kv_heads, splits))
+    return Item{id / pairs, id % kv_heads, id / kv_heads % splits};
+  const int each = (pairs + 7) / 8, j = id >> 3;  // pairs of an XCD
+  const int pair = (id & 7) + 8 * (j % each);
+  return Item{j / each, pair % kv_heads, pair / kv_heads};  // split >= splits: none
+}
+
 template <int HD>
 __device__ __forceinline__ int k_swizzle(int row) {
   return HD >= 128 ? (row & 15) : (row & 7);
@@ -92,7 +128,7 @@ __device__ __forceinline__ int v_swizzle(int dim) {
 }
 
 template <int HD, bool F8>
-__global__ __launch_bounds__(256, 2) void prefill_kernel(
+__global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
     const int32_t* __restrict__ starts, const int32_t* __restrict__ lens,
     const int32_t* __restrict__ table, const void* __restrict__ k_cache,
@@ -105,18 +141,19 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
   constexpr int ND = HD / 32;          // 32-dim operands of the output
   constexpr int KP = HD / 8;           // 16-byte pieces of a K row in LDS
   constexpr int VP = KT / 8;           // 16-byte pieces of a V^T row
-  constexpr int NK = KT * KP / 256;    // K pieces a thread copies: 16 keys a wave's quarter
-  constexpr int NVV = HD * VP / 256;   // V pieces a thread copies
-  constexpr int RPW = KT / 4;          // K rows a wave copies (8 or 16: one page)
-  extern __shared__ __align__(16) char lds[];  // two stages of [K | V^T]
+  constexpr int NK = KT * KP / (64 * NW);   // K pieces a thread copies
+  static_assert(!F8 || NK % 2 == 0, "two pieces of e4m3 at a time");
+  constexpr int NVV = HD * VP / (64 * NW);  // V pieces a thread copies
+  constexpr int RPW = KT / NW;              // K rows a wave copies (at most 16: one page)
+  extern __shared__ __align__(16) char lds[];  // [D] of K, then [D] of V^T
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int col = lane & 31, h = lane >> 5;
   const int group = d.heads / d.kv_heads;
-  const int item = blockIdx.x;
-  const int kvh = item % d.kv_heads, rest = item / d.kv_heads;
-  const int split = rest % splits;
+  const Item it = item_of(blockIdx.x, d.kv_heads, splits);
+  if (it.split >= splits) return;
+  const int kvh = it.kvh, split = it.split;
   Block b;
-  if (!find_block(starts, lens, d, rows, group, rest / splits, &b)) return;  // uniform
+  if (!find_block(starts, lens, d, rows, group, it.block, &b)) return;  // uniform
   const int prior = b.len - b.count;  // the first row's position (negative: rows without one)
   const int pairs = b.count * group;
   const int last_pair = min(b.pair0 + kPairs, pairs) - 1;
@@ -140,15 +177,11 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
     for (int s = 0; s < KS; ++s)
       qb[s] = alive ? *reinterpret_cast<const uint4*>(src + 16 * s) : make_uint4(0, 0, 0, 0);
   }
-  // the wave's pairs see at least the keys up to low, at most those up to high
-  int low = alive ? limit : 0x7fffffff, high = limit;
+  // the wave's pairs see at least the keys up to low
+  int low = alive ? limit : 0x7fffffff;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    low = min(low, __shfl_xor(low, o, 64));
-    high = max(high, __shfl_xor(high, o, 64));
-  }
+  for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o, 64));
   low = __builtin_amdgcn_readfirstlane(low);
-  high = __builtin_amdgcn_readfirstlane(high);
 
   const char* kc = static_cast<const char*>(k_cache);
   const char* vc = static_cast<const char*>(v_cache);
@@ -157,63 +190,74 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
   const float sl2 = scale * kLog2e * (F8 && k_scale ? k_scale[kvh] : 1.0f);
   const int64_t head_at = (int64_t(kvh) << d.page_log2) * HD;
 
-  // Page ids of a tile: of the wave's K rows, of this lane's V pieces, and, on lanes
-  // 0 .. KT/16 - 1, of its 16-key parts.  They are read two tiles ahead, the copy one.
+  // Page ids of a tile's 16-key parts, through scalar loads (they have a counter of their
+  // own, so waiting for one waits for no copy), read one tile ahead of the copy.
+  constexpr int PT = KT / 16;
   struct Ids {
-    int k, v, part;
+    int part[PT];
   };
   constexpr int VL = F8 ? VP / 2 : VP;  // lanes that copy one V^T row
-  const int vdim = wave * (HD / 4) + lane / VL;
+  const int vdim = wave * (HD / NW) + lane / VL;
   // the lane's keys of the rows that it copies: the same piece of every row
   const int vkey = F8 ? 16 * (lane % VL) : 8 * ((lane % VL) ^ v_swizzle<HD>(vdim));
-  auto id_at = [&](int key) { return page_at(table, d, b.seq, min(key >> d.page_log2, last_page)); };
-  auto ids_of = [&](int tile) {
-    return Ids{id_at(tile + RPW * wave), id_at(tile + vkey),
-               id_at(tile + 16 * (lane & (KT / 16 - 1)))};
+  auto ids_of = [&](int tile) MX_LAMBDA {
+    Ids id;
+#pragma unroll
+    for (int i = 0; i < PT; ++i)
+      id.part[i] = page_at(table, d, b.seq, min((tile + 16 * i) >> d.page_log2, last_page));
+    return id;
   };
-  constexpr uint32_t kAllParts = (1u << (KT / 16)) - 1u;
+  constexpr uint32_t kAllParts = (1u << PT) - 1u;
+  auto bits_of = [&](const Ids& id) MX_LAMBDA {  // bit i: keys 16 i .. 16 i + 15 lie in a page
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) m |= (id.part[i] >= 0 ? 1u : 0u) << i;
+    return m;
+  };
 
-  // One tile's copy.  Slot i of a stage's K part is piece i % KP of row i / KP
-  // and holds that row's piece (i % KP) ^ swizzle(row); V^T alike.
-  constexpr int kStage = stage_bytes<HD>();
-  constexpr int kVAt = KT * HD * 2;
+  // One tile's copies.  Slot i of a K stage is piece i % KP of row i / KP and
+  // holds that row's piece (i % KP) ^ swizzle(row); V^T alike.
+  constexpr int kPart = KT * HD * 2;  // bytes of a K (or V^T) stage
   const uint32_t lds_at = uint32_t(reinterpret_cast<uintptr_t>(
       (__attribute__((address_space(3))) char*)lds));
   uint4 kreg[F8 ? NK / 2 : 1], vreg[F8 ? NVV / 2 : 1];
-  auto copy = [&](int tile, int stage, const Ids& id) {
-    const int kid = __builtin_amdgcn_readfirstlane(max(id.k, 0));
-    const int vid = max(id.v, 0);
-    const char* kbase =
-        kc + (kid * d.page_stride + head_at + int64_t((tile + RPW * wave) & (page - 1)) * HD) * E;
-    const char* vbase = vc + (vid * d.page_stride + head_at + (int64_t(vdim) << d.page_log2) +
-                              ((tile + vkey) & (page - 1))) * E;
+  // from where this lane copies a tile's K and V
+  auto k_from = [&](int tile, const Ids& id) MX_LAMBDA {
+    int kid = id.part[0];
+#pragma unroll
+    for (int i = 1; i < PT; ++i) kid = (RPW * wave) >> 4 == i ? id.part[i] : kid;
+    return kc + (max(kid, 0) * d.page_stride + head_at +
+                 int64_t((tile + RPW * wave) & (page - 1)) * HD) * E;
+  };
+  auto v_from = [&](int tile, const Ids& id) MX_LAMBDA {
+    int vid = id.part[0];
+#pragma unroll
+    for (int i = 1; i < PT; ++i) vid = vkey >> 4 == i ? id.part[i] : vid;
+    return vc + (max(vid, 0) * d.page_stride + head_at + (int64_t(vdim) << d.page_log2) +
+                 ((tile + vkey) & (page - 1))) * E;
+  };
+  // piece i of a wave's copies, to LDS, or of e4m3 (16 values: two pieces of LDS) to registers
+  constexpr int CK = F8 ? NK / 2 : NK, CV = F8 ? NVV / 2 : NVV;
+  auto copy_k = [&](const char* from, int stage, int i) MX_LAMBDA {
     if constexpr (!F8) {
-      const uint32_t ks = lds_at + stage * kStage + RPW * wave * KP * 16;
-      const uint32_t vs = lds_at + stage * kStage + kVAt + wave * (HD / 4) * VP * 16;
-#pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const int slot = 64 * i + lane, r = slot / KP, p = slot % KP;
-        copy_to_lds(kbase + (r * HD + 8 * (p ^ k_swizzle<HD>(RPW * wave + r))) * E, ks + 1024 * i);
-      }
-#pragma unroll
-      for (int i = 0; i < NVV; ++i)
-        copy_to_lds(vbase + (int64_t(64 / VP * i) << d.page_log2) * E, vs + 1024 * i);
+      const int slot = 64 * i + lane, r = slot / KP, p = slot % KP;
+      copy_to_lds(from + (r * HD + 8 * (p ^ k_swizzle<HD>(RPW * wave + r))) * E,
+                  lds_at + stage * kPart + RPW * wave * KP * 16 + 1024 * i);
     } else {
-      // 16 e4m3 values at a time: two neighbouring pieces
-#pragma unroll
-      for (int i = 0; i < NK / 2; ++i) {
-        const int slot = 64 * i + lane, r = slot / (KP / 2), p = slot % (KP / 2);
-        kreg[i] = *reinterpret_cast<const uint4*>(kbase + r * HD + 16 * p);
-      }
-#pragma unroll
-      for (int i = 0; i < NVV / 2; ++i)
-        vreg[i] = *reinterpret_cast<const uint4*>(vbase + (int64_t(64 / VL * i) << d.page_log2));
+      const int slot = 64 * i + lane, r = slot / (KP / 2), p = slot % (KP / 2);
+      kreg[i] = *reinterpret_cast<const uint4*>(from + r * HD + 16 * p);
     }
   };
-  auto store = [&](int stage) {
+  auto copy_v = [&](const char* from, int stage, int i) MX_LAMBDA {
+    const char* src = from + (int64_t(64 / VL * i) << d.page_log2) * E;
+    if constexpr (!F8)
+      copy_to_lds(src, lds_at + (D + stage) * kPart + wave * (HD / NW) * VP * 16 + 1024 * i);
+    else
+      vreg[i] = *reinterpret_cast<const uint4*>(src);
+  };
+  auto store_k = [&](int stage) MX_LAMBDA {
     if constexpr (F8) {
-      char* ks = lds + stage * kStage;
-      char* vs = ks + kVAt;
+      char* ks = lds + stage * kPart;
 #pragma unroll
       for (int i = 0; i < NK / 2; ++i) {
         const int slot = 64 * i + lane, r = slot / (KP / 2), p = slot % (KP / 2);
@@ -221,6 +265,11 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
         *reinterpret_cast<uint4*>(ks + (row * KP + ((2 * p) ^ sw)) * 16) = widen8(kreg[i].x, kreg[i].y);
         *reinterpret_cast<uint4*>(ks + (row * KP + ((2 * p + 1) ^ sw)) * 16) = widen8(kreg[i].z, kreg[i].w);
       }
+    }
+  };
+  auto store_v = [&](int stage) MX_LAMBDA {
+    if constexpr (F8) {
+      char* vs = lds + (D + stage) * kPart;
 #pragma unroll
       for (int i = 0; i < NVV / 2; ++i) {
         const int dim = vdim + 64 / VL * i, p = lane % VL;
@@ -238,22 +287,86 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
 
-  Ids now = ids_of(tile0 * KT), next = ids_of((tile0 + 1) * KT);
-  if (tile0 < tile1) {
-    copy(tile0 * KT, 0, now);
-    store(0);
-  }
+  // Tile ti's K and V lie in stages ti % D.  Two workgroups (or four waves more of this one) share
+  // each matrix unit: while one forms its exponentials, the other has the products.  Forming a
+  // tile's exponentials under the next tile's products within one wave was no faster (HD 128,
+  // 8192 tokens: 608 us against 565), the two waves do that already.
+  constexpr int kCopies = F8 ? 0 : CK + CV;  // of a step, by a wave
+  constexpr int R = HD == 256 ? 2 : 4;       // operands read ahead of their products
+  // The order as it is written: left alone, the compiler reads each operand just before its
+  // product.  With 256 dims it has no registers for that, and its own order is faster (141 us
+  // against 191 for 512 rows on 12001 keys), and so it is with e4m3 (146 against 152 for four
+  // prompts of up to 2047 on up to 3001).
+  auto keep_order = [] {
+    if constexpr (HD < 256 && !F8) __builtin_amdgcn_sched_barrier(0);
+  };
   const int krow = (col & 0x13) | ((col & 4) << 1) | ((col & 8) >> 1);  // bits 2 and 3 exchanged
+  const int kswap = h ^ k_swizzle<HD>(krow);  // of krow + 32 alike
+  const int vswap = h ^ v_swizzle<HD>(col);   // of col + 32 n alike
+  // operands of product i of the scores, and of P V
+  auto k_operand = [&](int stage, int i) MX_LAMBDA {
+    return *reinterpret_cast<const uint4*>(lds + stage * kPart + krow * (KP * 16) +
+                                           ((2 * (i / KB)) ^ kswap) * 16 +
+                                           (i % KB) * (32 * KP * 16));
+  };
+  auto v_operand = [&](int stage, int i) MX_LAMBDA {
+    return *reinterpret_cast<const uint4*>(lds + (D + stage) * kPart + col * (VP * 16) +
+                                           ((2 * (i / ND)) ^ vswap) * 16 +
+                                           (i % ND) * (32 * VP * 16));
+  };
+  auto score = [&](int i, const uint4& a, floatx16_t (&sc)[KB]) MX_LAMBDA {
+    sc[i % KB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                         __builtin_bit_cast(bf16x8_t, qb[i / KB]),
+                                                         sc[i % KB], 0, 0, 0);
+  };
+  // all scores of the tile in K stage `stage`, with between(i) after product i
+  auto scores = [&](int stage, floatx16_t (&sc)[KB], auto&& between) MX_LAMBDA {
+    uint4 a[R];
+    each<R>([&](auto i) MX_LAMBDA { a[i] = k_operand(stage, i); });
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[kb][r] = 0.0f;
+    each<KS * KB>([&](auto i) MX_LAMBDA {
+      keep_order();
+      score(i, a[i % R], sc);
+      if constexpr (i + R < KS * KB) a[i % R] = k_operand(stage, i + R);
+      between(i);
+    });
+    keep_order();
+  };
+  // Tiles past the last one are copied like it, into stages that nobody reads: every step
+  // has the same copies, so waiting for all but the latest is waiting for their number.
+  const int last = (tile1 - 1) * KT;
+  uint32_t queue = 0;  // parts of the tiles from the present one on, PT bits each
+  Ids id;
+  if (tile0 < tile1) {
+    id = ids_of(tile0 * KT);
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i) {
+      const int at = min((tile0 + i) * KT, last);
+      queue |= bits_of(id) << (PT * i);
+      const char* kf = k_from(at, id);
+      const char* vf = v_from(at, id);
+      each<CK>([&](auto j) MX_LAMBDA { copy_k(kf, i, j); });
+      each<CV>([&](auto j) MX_LAMBDA { copy_v(vf, i, j); });
+      store_k(i);
+      store_v(i);
+      id = ids_of(min((tile0 + i + 1) * KT, last));
+    }
+  }
+  int stage = 0;
   for (int ti = tile0; ti < tile1; ++ti) {
-    const int tile = ti * KT, stage = (ti - tile0) & 1;
-    copies_done();    // this wave's part of the tile is in LDS, and `next` is here
-    __syncthreads();  // everyone's is; the other stage is consumed
-    const uint32_t parts = uint32_t(__ballot(now.part >= 0)) & kAllParts;
+    const int tile = ti * KT;
+    // this wave's part of the tile is in LDS ...
+    copies_done<(D - 2) * kCopies>();
+    __syncthreads();  // ... and everyone's; the stage of the tile before is free
+    const uint32_t parts = queue & kAllParts;
+    queue >>= PT;
     const bool ragged = tile + KT > kall || parts != kAllParts;
-    char* ks = lds + stage * kStage;
-    char* vs = ks + kVAt;
+    char* vs = lds + (D + stage) * kPart;
     if (ragged) {  // uniform: V of positions that are no keys may be anything, and becomes 0
-      for (int i = t; i < HD * VP; i += 256) {
+      for (int i = t; i < HD * VP; i += 64 * NW) {
         const int dim = i / VP, key0 = 8 * ((i % VP) ^ v_swizzle<HD>(dim));
         const int n = (parts >> (key0 >> 4)) & 1 ? min(max(kall - tile - key0, 0), 8) : 0;
         if (n == 8) continue;
@@ -262,85 +375,93 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
       }
       __syncthreads();
     }
-    now = next;
-    if (ti + 1 < tile1) {
-      copy((ti + 1) * KT, stage ^ 1, now);
-      next = ids_of((ti + 2) * KT);
+    const int ahead = stage == 0 ? D - 1 : stage - 1;  // of tile ti + D - 1
+    queue |= bits_of(id) << (PT * (D - 2));
+    const int at = min((ti + D - 1) * KT, last);
+    const char* kf = k_from(at, id);
+    const char* vf = v_from(at, id);
+    // Issued together the copies hold up every wave of the workgroup at once, for as long as the
+    // memory path takes for all of them, so they are spread over the scores' products; with 256
+    // dims there are no registers for their addresses meanwhile.
+    auto copy = [&](auto i) MX_LAMBDA {
+      if constexpr (i < CK)
+        copy_k(kf, ahead, i);
+      else
+        copy_v(vf, ahead, i - CK);
+    };
+    if constexpr (HD == 256) each<CK + CV>(copy);
+    floatx16_t sc[KB];
+    scores(stage, sc, [&](auto i) MX_LAMBDA {
+      if constexpr (HD < 256) {
+        constexpr int n = KS * KB, first = i * (CK + CV) / n, end = (i + 1) * (CK + CV) / n;
+        each<end - first>([&](auto j) MX_LAMBDA { copy(std::integral_constant<int, first + j>{}); });
+      }
+    });
+    uint4 a[R];
+    each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(stage, i); });
+    if (tile + KT - 1 > low || parts != kAllParts) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = 32 * kb + 16 * (r >> 3) + 8 * h + (r & 7);
+          const bool in = tile + key <= limit && (parts >> (2 * kb + (r >> 3)) & 1);
+          sc[kb][r] = in ? sc[kb][r] : neg_inf();
+        }
     }
-    if (tile <= high) {
-      floatx16_t sc[KB];
+    float mt = sc[0][0];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+    for (int i = 1; i < 16 * KB; ++i) mt = fmaxf(mt, sc[i / 16][i % 16]);
+    mt = max_across_halves(mt) * sl2;
+    // The reference follows the maximum in steps of at least 8 (a factor of 256, far from any
+    // limit of fp32 or bf16), so that most tiles rescale nothing.
+    if (__any(mt > m_run + 8.0f || m_run == neg_inf())) {
+      const float mn = fmaxf(m_run, mt);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (mn == neg_inf() ? 0.0f : mn));
+      l_run *= alpha;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sc[kb][r] = 0.0f;
-      const char* krp = ks + krow * KP * 16;
-      int swap = h ^ k_swizzle<HD>(krow);  // of krow + 32 alike
-      asm("" : "+v"(swap));                // formed anew for every tile: held, the addresses spill
+      for (int n = 0; n < ND; ++n)
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const uint4 a =
-              *reinterpret_cast<const uint4*>(krp + ((2 * s) ^ swap) * 16 + kb * (32 * KP * 16));
-          sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                           __builtin_bit_cast(bf16x8_t, qb[s]),
-                                                           sc[kb], 0, 0, 0);
-        }
-      if (tile + KT - 1 > low || parts != kAllParts) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = 32 * kb + 16 * (r >> 3) + 8 * h + (r & 7);
-            const bool in = tile + key <= limit && (parts >> (2 * kb + (r >> 3)) & 1);
-            sc[kb][r] = in ? sc[kb][r] : neg_inf();
-          }
-      }
-      float mt = sc[0][0];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sc[kb][r]);
-      mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * sl2;
-      // The reference follows the maximum in steps of at least 8 (a factor of 256, far from any
-      // limit of fp32 or bf16), so that most tiles rescale nothing.
-      if (__any(mt > m_run + 8.0f || m_run == neg_inf())) {
-        const float mn = fmaxf(m_run, mt);
-        const float alpha = __builtin_amdgcn_exp2f(m_run - (mn == neg_inf() ? 0.0f : mn));
-        l_run *= alpha;
-#pragma unroll
-        for (int n = 0; n < ND; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
-        m_run = mn;
-      }
-      const float ref = m_run == neg_inf() ? 0.0f : m_run;  // no key yet: every weight is 0
-      uint32_t pb[KB * 8];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float x = __builtin_amdgcn_exp2f(fmaf_(sc[kb][r], sl2, -ref));
-          const float y = __builtin_amdgcn_exp2f(fmaf_(sc[kb][r + 1], sl2, -ref));
-          l_run += x + y;
-          pb[8 * kb + r / 2] = pack2(x, y);
-        }
-      const int vswap = h ^ v_swizzle<HD>(col);  // of col + 32 n alike
-#pragma unroll
-      for (int s = 0; s < 2 * KB; ++s) {
-        const bf16x8_t p = __builtin_bit_cast(
-            bf16x8_t, make_uint4(pb[4 * s], pb[4 * s + 1], pb[4 * s + 2], pb[4 * s + 3]));
-#pragma unroll
-        for (int n = 0; n < ND; ++n) {
-          const uint4 a = *reinterpret_cast<const uint4*>(
-              vs + (col * VP + ((2 * s) ^ vswap)) * 16 + n * (32 * VP * 16));
-          o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), p, o[n],
-                                                         0, 0, 0);
-        }
-      }
+        for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
+      m_run = mn;
     }
-    if (ti + 1 < tile1) store(stage ^ 1);
+    const float ref = m_run == neg_inf() ? 0.0f : m_run;  // no key yet: every weight is 0
+    uint32_t pb[KB * 8];
+    auto pair = [&](auto j) MX_LAMBDA {
+      constexpr int kb = j / 8, r = 2 * (j % 8);
+      const float x = __builtin_amdgcn_exp2f(fmaf_(sc[kb][r], sl2, -ref));
+      const float y = __builtin_amdgcn_exp2f(fmaf_(sc[kb][r + 1], sl2, -ref));
+      l_run += x + y;
+      pb[j] = pack2(x, y);
+    };
+    // P V of 16 keys takes four pairs; the next four form between its products
+    each<4>(pair);
+    constexpr int kP = 2 * KB * ND;
+    each<kP>([&](auto i) MX_LAMBDA {
+      constexpr int s = i / ND, n = i % ND;
+      keep_order();
+      o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          __builtin_bit_cast(bf16x8_t, a[i % R]),
+          __builtin_bit_cast(bf16x8_t, make_uint4(pb[4 * s], pb[4 * s + 1], pb[4 * s + 2],
+                                                  pb[4 * s + 3])),
+          o[n], 0, 0, 0);
+      if constexpr (i + R < kP) a[i % R] = v_operand(stage, i + R);
+      if constexpr (s + 1 < 2 * KB) {
+        constexpr int first = 4 * n / ND, end = 4 * (n + 1) / ND;
+        each<end - first>([&](auto j) MX_LAMBDA {
+          pair(std::integral_constant<int, 4 * (s + 1) + first + j>{});
+        });
+      }
+    });
+    keep_order();
+    // read here, the ids are there after the barrier; before, they would hold up the first
+    // products, whose LDS reads wait on the same counter
+    id = ids_of(min((ti + D) * KT, last));
+    store_k(ahead);
+    store_v(ahead);
+    stage = stage == D - 1 ? 0 : stage + 1;
   }
+  copies_done<0>();  // none lands in LDS that is no longer this workgroup's
   if (!alive) return;
   l_run += __shfl_xor(l_run, 32, 64);
   if (whole) {
@@ -379,43 +500,58 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(
   }
 }
 
-// Joins the splits of 128 pairs of a query block in order, a wave a pair at a time.
+// Joins the splits (at most 64) of some pairs of a query block in order, a wave a pair at a time.
+constexpr int kJoinPairs = 8;
 template <int HD>
 __global__ __launch_bounds__(256) void prefill_join_kernel(
     const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
     const int32_t* __restrict__ starts, const int32_t* __restrict__ lens,
     const float* __restrict__ v_scale, PageDims d, int splits, const float* __restrict__ o_part,
     const float* __restrict__ ml_part, uint16_t* __restrict__ out) {
-  constexpr int KT = tile_keys<HD>(), DPL = HD / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int KT = tile_keys<HD>(), DPL = HD / 64, JW = kPairs / kJoinPairs;
+  typedef float vec __attribute__((ext_vector_type(DPL)));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = d.heads / d.kv_heads;
   const int kvh = blockIdx.x % d.kv_heads;
   Block b;
-  if (!find_block(starts, lens, d, rows, group, int(blockIdx.x / d.kv_heads / 8), &b)) return;
+  if (!find_block(starts, lens, d, rows, group, int(blockIdx.x / d.kv_heads / JW), &b)) return;
   const int prior = b.len - b.count, pairs = b.count * group;
   const int last_pair = min(b.pair0 + kPairs, pairs) - 1;
   const int kall = max(prior + last_pair / group + 1, 0);
   const int tiles = (kall + KT - 1) / KT, per = (tiles + splits - 1) / splits;
   if (per >= tiles) return;  // one split (or none) wrote the result
   const int n = (tiles + per - 1) / per;
-  const int first = int(blockIdx.x / d.kv_heads) % 8 * (kPairs / 8);  // an eighth of the block
-  for (int i = first + wave; i < first + kPairs / 8; i += 4) {
+  const int first = int(blockIdx.x / d.kv_heads) % JW * kJoinPairs;
+  for (int i = first + wave; i < first + kJoinPairs; i += 4) {
     const int pair = b.pair0 + i;
     if (pair > last_pair) return;
     const int token = pair / group, head = kvh * group + pair - token * group;
     const int64_t row = b.first + token, part = (row * d.heads + head) * splits;
-    float M = neg_inf();
-    for (int c = 0; c < n; ++c) M = fmaxf(M, ml_part[(part + c) * 2]);
-    const float ref = M == neg_inf() ? 0.0f : M;
-    float L = 0.0f, O[DPL];
+    // eight splits' sums on their way while the weights form, a lane a split
+    vec v[8];
 #pragma unroll
-    for (int k = 0; k < DPL; ++k) O[k] = 0.0f;
-#pragma unroll 4
-    for (int c = 0; c < n; ++c) {
-      const float e = __builtin_amdgcn_exp2f(ml_part[(part + c) * 2] - ref);
-      L = fmaf_(ml_part[(part + c) * 2 + 1], e, L);
+    for (int c = 0; c < 8; ++c)
+      v[c] = *reinterpret_cast<const vec*>(o_part + (part + min(c, n - 1)) * HD + DPL * lane);
+    const float2 ml = *reinterpret_cast<const float2*>(ml_part + (part + min(lane, n - 1)) * 2);
+    float M = ml.x;
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float e = lane < n ? __builtin_amdgcn_exp2f(ml.x - (M == neg_inf() ? 0.0f : M)) : 0.0f;
+    float L = ml.y * e;
+    for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+    vec O = 0.0f;
+    for (int c0 = 0; c0 < n; c0 += 8) {
 #pragma unroll
-      for (int k = 0; k < DPL; ++k) O[k] = fmaf_(o_part[(part + c) * HD + DPL * lane + k], e, O[k]);
+      for (int c = 0; c < 8; ++c)
+        if (c0 + c < n) {  // uniform
+          const float w = u2f(__builtin_amdgcn_readlane(int(f2u(e)), c0 + c));
+          for (int k = 0; k < DPL; ++k) O[k] = fmaf_(v[c][k], w, O[k]);
+        }
+      if (c0 + 8 < n) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          v[c] = *reinterpret_cast<const vec*>(o_part + (part + min(c0 + 8 + c, n - 1)) * HD +
+                                               DPL * lane);
+      }
     }
     const float inv = (L == 0.0f ? 0.0f : 1.0f / L) * (v_scale ? v_scale[kvh] : 1.0f);
 #pragma unroll
@@ -428,28 +564,35 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(
   }
 }
 
-// The most query blocks (times kv heads) that any starts give.
-int64_t prefill_blocks(int rows, const PageDims& d) {
-  const int group = d.heads / d.kv_heads;
-  const int64_t n = int64_t(rows) * group / kPairs + (d.sequences < rows ? d.sequences : rows);
-  return n * d.kv_heads;
-}
-
-// Workgroups that share a block's keys: as many as bring the launch to two a
-// compute unit, each with at least four tiles of the longest possible context.
-int prefill_splits(int rows, const PageDims& d) {
-  const int64_t blocks = prefill_blocks(rows, d);
-  const int64_t want = 512 / (blocks < 1 ? 1 : blocks);
+// How a call is laid out: the most query blocks that any starts give, and the workgroups that
+// share a block's keys.
+struct Layout {
+  int64_t blocks;
+  int splits;
+};
+Layout layout_of(int rows, const PageDims& d) {
+  Layout l;
+  l.blocks = int64_t(rows) * (d.heads / d.kv_heads) / kPairs + (d.sequences < rows ? d.sequences : rows);
+  // as many splits as bring the launch to two workgroups a compute unit, each with at least four
+  // tiles of the longest possible context; in eights with the kv heads where that is possible,
+  // for whole XCDs (512 rows on 12001 keys, two kv heads: 8 splits 147 us, 7 splits 162)
+  const int64_t all = l.blocks * d.kv_heads, want = 512 / (all < 1 ? 1 : all);
   const int64_t room = (int64_t(d.table_width) << d.page_log2) / 256;
   int64_t s = want < room ? want : room;
-  s = s > 64 ? 64 : s;
-  return s < 1 ? 1 : int(s);
+  s = s > 64 ? 64 : s < 1 ? 1 : s;
+  l.splits = int(s);
+  for (int64_t e = s; s > 1 && e < 2 * s && e <= room; ++e)
+    if (e * d.kv_heads % 8 == 0) {
+      l.splits = int(e);
+      break;
+    }
+  return l;
 }
 
 }  // namespace
 
 size_t paged_prefill_workspace(int rows, const PageDims& d) {
-  const int s = prefill_splits(rows, d);
+  const int s = layout_of(rows, d).splits;
   return s == 1 ? 0 : size_t(rows) * d.heads * s * (d.head_dim + 2) * 4;
 }
 
@@ -458,27 +601,32 @@ int paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, in
                   const void* k_cache, const void* v_cache, const float* k_scale,
                   const float* v_scale, const PageDims& d, float scale, void* workspace,
                   uint16_t* out, hipStream_t s) {
-  const int splits = prefill_splits(rows, d);
-  const int64_t blocks = prefill_blocks(rows, d);
-  if (blocks * splits > 0x7fffffff || blocks * 8 > 0x7fffffff) return MX_EUNSUPPORTED;
+  const Layout l = layout_of(rows, d);
+  const int splits = l.splits;
+  const int64_t blocks = l.blocks * d.kv_heads, joins = blocks * (kPairs / kJoinPairs);
+  // XCDs take whole pairs of kv head and split; without enough of them, every workgroup in turn
+  const int64_t grid = by_xcd(d.kv_heads, splits)
+                           ? l.blocks * 8 * ((int64_t(d.kv_heads) * splits + 7) / 8)
+                           : blocks * splits;
+  if (grid > 0x7fffffff || joins > 0x7fffffff) return MX_EUNSUPPORTED;
   float* o_part = static_cast<float*>(workspace);
   float* ml_part = o_part + size_t(rows) * d.heads * splits * d.head_dim;
-#define MX_PREFILL(HH, FF)                                                                        \
-  if (d.head_dim == HH && d.f8 == FF) {                                                           \
-    const auto fn = prefill_kernel<HH, FF>;                                                       \
-    constexpr int lb = 2 * stage_bytes<HH>();                                                     \
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn),                                    \
-                            hipFuncAttributeMaxDynamicSharedMemorySize, lb) != hipSuccess)        \
-      return MX_EHIP;                                                                             \
-    hipLaunchKernelGGL(fn, dim3(unsigned(blocks* splits)), dim3(256), lb, s, q, qkv, qkv_stride,  \
-                       rows, starts, lens, table, k_cache, v_cache, k_scale, v_scale, d, scale,   \
-                       splits, o_part, ml_part, out);                                             \
-    if (hipGetLastError() != hipSuccess) return MX_EHIP;                                          \
-    if (splits == 1) return MX_OK;                                                                \
-    hipLaunchKernelGGL((prefill_join_kernel<HH>), dim3(unsigned(blocks * 8)), dim3(256), 0, s,    \
-                       qkv, qkv_stride, rows, starts, lens, FF ? v_scale : nullptr, d, splits,    \
-                       o_part, ml_part, out);                                                     \
-    return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;                                     \
+  const float* vs = d.f8 ? v_scale : nullptr;
+#define MX_PREFILL(HH, FF)                                                                       \
+  if (d.head_dim == HH && d.f8 == FF) {                                                          \
+    const auto fn = prefill_kernel<HH, FF>;                                                      \
+    constexpr int lb = D * stage_bytes<HH>();                                                    \
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn),                                   \
+                            hipFuncAttributeMaxDynamicSharedMemorySize, lb) != hipSuccess)       \
+      return MX_EHIP;                                                                            \
+    hipLaunchKernelGGL(fn, dim3(unsigned(grid)), dim3(64 * NW), lb, s, q, qkv, qkv_stride, rows, \
+                       starts, lens, table, k_cache, v_cache, k_scale, v_scale, d, scale,        \
+                       splits, o_part, ml_part, out);                                            \
+    if (hipGetLastError() != hipSuccess) return MX_EHIP;                                         \
+    if (splits == 1) return MX_OK;                                                               \
+    hipLaunchKernelGGL((prefill_join_kernel<HH>), dim3(unsigned(joins)), dim3(256), 0, s, qkv,   \
+                       qkv_stride, rows, starts, lens, vs, d, splits, o_part, ml_part, out);     \
+    return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;                                    \
   }
   MX_PREFILL(64, false) MX_PREFILL(128, false) MX_PREFILL(256, false)
   MX_PREFILL(64, true) MX_PREFILL(128, true) MX_PREFILL(256, true)
