@@ -506,9 +506,9 @@ mx_status mx_attn_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_str
  * finite.
  *
  * head_dim 64, 128 or 256; 1..16 q heads per kv head; page_size 16, 32, 64, 128
- * or 256 (MX_EUNSUPPORTED otherwise).  q, qkv rows (qkv_stride % 8 == 0), out,
- * workspaces and both caches are 16-byte aligned.  The pointers and the stream belong
- * to the current device.  A workspace serves one call at a time: calls that
+ * or 256 (MX_EUNSUPPORTED otherwise).  q, qkv rows (qkv_stride % 8 == 0), norms,
+ * out, workspaces and both caches are 16-byte aligned.  The pointers and the
+ * stream belong to the current device.  A workspace serves one call at a time: calls that
  * may overlap (two streams, two captured graphs) need one each. */
 typedef struct mx_page_dims {
   int32_t heads;        /* q heads */

@@ -628,10 +628,10 @@ MX_ABI mx_status mx_attn_paged_append(const uint16_t* qkv, int64_t qkv_stride, i
   const int64_t width =
       (int64_t(d.heads) * (d.gated ? 2 : 1) + 2 * int64_t(d.kv_heads)) * d.head_dim;
   MX_CHECK(qkv_stride >= width, MX_EINVAL, "mx_attn_paged_append: qkv_stride shorter than a row");
-  MX_CHECK(aligned16(qkv) && qkv_stride % 8 == 0 && aligned16(q_out) && aligned16(k_cache) &&
-               aligned16(v_cache),
+  MX_CHECK(aligned16(qkv) && qkv_stride % 8 == 0 && aligned16(q_norm) && aligned16(k_norm) &&
+               aligned16(q_out) && aligned16(k_cache) && aligned16(v_cache),
            MX_EUNSUPPORTED,
-           "mx_attn_paged_append: qkv rows, q_out and the cache must be 16-byte aligned");
+           "mx_attn_paged_append: qkv rows, norms, q_out and the cache must be 16-byte aligned");
   return finish(paged_append(qkv, qkv_stride, rows, seqs, pos, rope_pos, r, q_norm, k_norm, eps,
                              table, d, k_scale, v_scale, q_out, k_cache, v_cache,
                              hipStream_t(stream)),

@@ -17,12 +17,12 @@ using namespace pg;
 // all in fp32 with one rounding, to bf16 or, divided by the kv head's scale, to
 // e4m3.  The angle is formed in 64 bits as a fraction of a turn, so positions
 // of millions keep their low bits; its sine and cosine are then fp32 series
-// around the nearest quarter turn, once per row and workgroup.
+// around the nearest quarter turn, once per row and wave.
 //
-// Bytes bound it.  The first workgroups of the grid take the q and k heads of
-// one row each, eight values a lane; the others take one kv head's V of 32 rows
-// each: they pass through LDS so that neighbouring lanes store neighbouring
-// positions of a page, where V lies transposed.
+// Bytes bound it.  The first workgroups of the grid take one kv head's V of 32
+// rows each: they pass through LDS so that neighbouring lanes store neighbouring
+// positions of a page, where V lies transposed.  The waves of the others take q
+// and k heads of a row, eight values a lane, several at a time, without meeting.
 constexpr int kQkThreads = 256;
 constexpr int kVRows = 32;
 
@@ -55,104 +55,155 @@ __global__ __launch_bounds__(kQkThreads) void append_kernel(
     const uint16_t* __restrict__ k_norm, float eps, const int32_t* __restrict__ table, PageDims d,
     const float* __restrict__ k_scale, const float* __restrict__ v_scale,
     uint16_t* __restrict__ q_out, void* __restrict__ k_cache, void* __restrict__ v_cache,
-    int groups, int64_t qk_blocks) {
+    int groups, int each, int v_blocks) {
   constexpr int LPH = HD / 8;           // lanes per head
-  constexpr int HPB = kQkThreads / LPH; // heads per workgroup
-  __shared__ float trig[2][128];
-  __shared__ float pairs[kQkThreads][9];  // nine: lanes of a wave start in different banks
-  __shared__ uint16_t vbuf[kVRows][HD + 2];
+  constexpr int HPW = 64 / LPH;         // heads of a group, which a wave takes at once
+  constexpr int PLD = 12;               // a lane's eight values in LDS, padded
+  constexpr int AHEAD = 4;              // groups on their way
+  __shared__ float trigs[kQkThreads / 64][2][128];
+  constexpr int VLD = HD + 2;
+  __shared__ __align__(16) union {
+    float pairs[kQkThreads * PLD];
+    uint16_t v[kVRows * VLD];
+  } buf;
+  float* pairs = buf.pairs;
   const int t = threadIdx.x;
   const int page = 1 << d.page_log2;
   const int q_width = d.gated ? 2 * HD : HD;
-  const int64_t b = blockIdx.x;
-  if (b < qk_blocks) {
-    const int row = int(b / groups), group = int(b % groups);
+  if (int(blockIdx.x) >= v_blocks) {
+    // a wave takes `each` groups of heads of one row
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+    const int per_row = (groups + each - 1) / each;
+    const int64_t b = int64_t(int(blockIdx.x) - v_blocks) * (kQkThreads / 64) + wave;
+    if (b >= int64_t(rows) * per_row) return;
+    const int row = int(b / per_row), g0 = int(b % per_row) * each, g1 = min(groups, g0 + each);
+    float(&trig)[2][128] = trigs[wave];
     const int seq = seqs ? seqs[row] : row;
-    if (unsigned(seq) >= unsigned(d.sequences)) return;  // a padding row (uniform)
-    const int head = group * HPB + t / LPH, piece = t % LPH;
-    const bool alive = head < d.heads + d.kv_heads, is_q = head < d.heads;
-    const int kvh = head - d.heads;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (alive) {
-      const uint16_t* src = qkv + int64_t(row) * qkv_stride +
-                            (is_q ? int64_t(head) * q_width
-                                  : int64_t(d.heads) * q_width + int64_t(kvh) * HD) + 8 * piece;
-      raw = *reinterpret_cast<const uint4*>(src);
-    }
+    const int p = pos[row];
+    const int piece = t % LPH, heads = d.heads + d.kv_heads;
+    const uint16_t* src = qkv + int64_t(row) * qkv_stride + 8 * piece;
+    auto load = [&](int group) {
+      const int head = group * HPW + lane / LPH;
+      if (group >= g1 || head >= heads) return make_uint4(0, 0, 0, 0);
+      const int64_t at = head < d.heads ? int64_t(head) * q_width
+                                        : int64_t(d.heads) * q_width + int64_t(head - d.heads) * HD;
+      return *reinterpret_cast<const uint4*>(src + at);
+    };
+    uint4 raws[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) raws[i] = load(g0 + i);
     const int half = rope.rotary_dim / 2;
-    if (t < half) {
-      const double p = double(rope_pos[int64_t(rope.pair_axis[t]) * rows + row]);
-      sincos_turn(p * rope.inv_freq[t] * 0.15915494309189533577, &trig[1][t], &trig[0][t]);
-    }
-    float y[8];
-    const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[2 * i] = u2f(w4[i] << 16);
-      y[2 * i + 1] = u2f(w4[i] & 0xffff0000u);
-    }
-    const uint16_t* norm = is_q ? q_norm : k_norm;
-    if (norm && alive) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf_(y[i], y[i], ss);
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-      const float inv = 1.0f / __builtin_sqrtf(ss * (1.0f / HD) + eps);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * (bf16_to_f32(norm[8 * piece + i]) + 1.0f);
-    }
-    // every value's partner of the rotation, half a rotary width away
-#pragma unroll
-    for (int i = 0; i < 8; ++i) pairs[t][i] = y[i];
-    __syncthreads();
-    if (!alive) return;
-    const int head0 = t - piece;  // the head's first lane
+    uint4 qn = make_uint4(0, 0, 0, 0), kn = qn;  // norm weights: the same piece of every head
+    if (q_norm) qn = *reinterpret_cast<const uint4*>(q_norm + 8 * piece);
+    if (k_norm) kn = *reinterpret_cast<const uint4*>(k_norm + 8 * piece);
+    if (unsigned(seq) >= unsigned(d.sequences)) return;  // a padding row (uniform)
+    const int pid = p >= 0 && (p >> d.page_log2) < d.table_width
+                        ? page_at(table, d, seq, p >> d.page_log2)
+                        : -1;
+    for (int i = lane; i < half; i += 64)
+      sincos_turn(double(rope_pos[int64_t(rope.pair_axis[i]) * rows + row]) * rope.inv_freq[i] *
+                      0.15915494309189533577,
+                  &trig[1][i], &trig[0][i]);
+    wave_sync();
+    // The lane's eight places are the same in every head, and so are their sines (signed for
+    // the sum) and their partners' place, half a rotary width away in a lane of this wave.
+    float cs[8], sn[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int c = 8 * piece + i;
-      if (c < 2 * half) {
-        const int pi = c < half ? c : c - half;
-        const int other = c < half ? c + half : c - half;
-        const float x = pairs[head0 + (other >> 3)][other & 7];
-        y[i] = c < half ? y[i] * trig[0][pi] - x * trig[1][pi]
-                        : y[i] * trig[0][pi] + x * trig[1][pi];
-      }
+      cs[i] = c < 2 * half ? trig[0][c < half ? c : c - half] : 1.0f;
+      sn[i] = c < half ? -trig[1][c] : c < 2 * half ? trig[1][c - half] : 0.0f;
     }
-    if (is_q) {
-      *reinterpret_cast<uint4*>(q_out + (int64_t(row) * d.heads + head) * HD + 8 * piece) =
-          make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
-      return;
-    }
-    const int p = pos[row];
-    if (p < 0 || (p >> d.page_log2) >= d.table_width) return;
-    const int pid = page_at(table, d, seq, p >> d.page_log2);
-    if (pid < 0) return;
-    const int64_t at =
-        pid * d.page_stride + (int64_t(kvh) * page + (p & (page - 1))) * HD + 8 * piece;
-    if constexpr (F8) {
-      const float s = k_scale ? k_scale[kvh] : 1.0f;
-      uint32_t o[2] = {0, 0};
+    const int partner =
+        (t - piece + (8 * piece < half ? 8 * piece + half : 8 * piece - half) / 8) * PLD;
+    auto widen = [](const uint4& v, float (&y)[8]) {
+      const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i >> 2] |= uint32_t(narrow(y[i] / s)) << (8 * (i & 3));
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(k_cache) + at) = make_uint2(o[0], o[1]);
-    } else {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(k_cache) + at) =
-          make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
+      for (int i = 0; i < 4; ++i) {
+        y[2 * i] = u2f(w4[i] << 16);
+        y[2 * i + 1] = u2f(w4[i] & 0xffff0000u);
+      }
+    };
+    auto put = [&](int group, const uint4& raw) {
+      const int head = group * HPW + lane / LPH;
+      const bool is_q = head < d.heads;
+      const int kvh = head - d.heads;
+      float y[8];
+      widen(raw, y);
+      if (is_q ? q_norm != nullptr : k_norm != nullptr) {
+        float w[8];
+        widen(is_q ? qn : kn, w);
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf_(y[i], y[i], ss);
+        ss = group_sum<LPH>(ss);
+        const float inv = 1.0f / __builtin_sqrtf(ss * (1.0f / HD) + eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * (w[i] + 1.0f);
+      }
+      if (half > 0) {
+        wave_sync();
+        float4* mine = reinterpret_cast<float4*>(pairs + t * PLD);
+        mine[0] = make_float4(y[0], y[1], y[2], y[3]);
+        mine[1] = make_float4(y[4], y[5], y[6], y[7]);
+        wave_sync();
+        if (half % 8 == 0) {  // a lane's eight values have another lane's eight for partners
+          if (8 * piece < 2 * half) {
+            const float4* op = reinterpret_cast<const float4*>(pairs + partner);
+            const float4 o0 = op[0], o1 = op[1];
+            const float x[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = fmaf_(x[i], sn[i], y[i] * cs[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int c = 8 * piece + i, other = c < half ? c + half : c - half;
+            if (c < 2 * half)
+              y[i] = fmaf_(pairs[(t - piece + (other >> 3)) * PLD + (other & 7)], sn[i], y[i] * cs[i]);
+          }
+        }
+      }
+      if (head >= heads) return;
+      if (is_q) {
+        *reinterpret_cast<uint4*>(q_out + (int64_t(row) * d.heads + head) * HD + 8 * piece) =
+            make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
+        return;
+      }
+      if (pid < 0) return;
+      const int64_t at =
+          pid * d.page_stride + (int64_t(kvh) * page + (p & (page - 1))) * HD + 8 * piece;
+      if constexpr (F8) {
+        const float s = k_scale ? k_scale[kvh] : 1.0f;
+        uint32_t o[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i >> 2] |= uint32_t(narrow(y[i] / s)) << (8 * (i & 3));
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(k_cache) + at) = make_uint2(o[0], o[1]);
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(k_cache) + at) =
+            make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
+      }
+    };
+    for (int g = g0; g < g1; g += AHEAD) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (g + i >= g1) break;
+        put(g + i, raws[i]);
+        raws[i] = load(g + AHEAD + i);
+      }
     }
     return;
   }
   // V of kVRows rows and one kv head
-  const int64_t vb = b - qk_blocks;
-  const int kvh = int(vb % d.kv_heads);
-  const int row0 = int(vb / d.kv_heads) * kVRows;
+  const int kvh = int(blockIdx.x) % d.kv_heads;
+  const int row0 = int(blockIdx.x) / d.kv_heads * kVRows;
   const int64_t col = int64_t(d.heads) * q_width + int64_t(d.kv_heads + kvh) * HD;
   for (int i = t; i < kVRows * LPH; i += kQkThreads) {
     const int r = i / LPH, piece = i % LPH;
     if (row0 + r < rows) {
       const uint4 v =
           *reinterpret_cast<const uint4*>(qkv + int64_t(row0 + r) * qkv_stride + col + 8 * piece);
-      uint32_t* dst = reinterpret_cast<uint32_t*>(&vbuf[r][8 * piece]);  // rows are 4-byte aligned
+      uint32_t* dst = reinterpret_cast<uint32_t*>(buf.v + r * VLD + 8 * piece);  // 4-byte aligned
       dst[0] = v.x;
       dst[1] = v.y;
       dst[2] = v.z;
@@ -170,7 +221,7 @@ __global__ __launch_bounds__(kQkThreads) void append_kernel(
   float s = 1.0f;
   if constexpr (F8) s = v_scale ? v_scale[kvh] : 1.0f;
   for (int c = t / kVRows; c < HD / 2; c += kQkThreads / kVRows) {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(&vbuf[r][2 * c]);
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(buf.v + r * VLD + 2 * c);
     const int64_t o = at + (int64_t(2 * c) << d.page_log2);
     if constexpr (F8) {
       uint8_t* dst = static_cast<uint8_t*>(v_cache);
@@ -636,16 +687,22 @@ int paged_append(const uint16_t* qkv, int64_t qkv_stride, int rows, const int32_
                  const uint16_t* q_norm, const uint16_t* k_norm, float eps, const int32_t* table,
                  const PageDims& d, const float* k_scale, const float* v_scale, uint16_t* q_out,
                  void* k_cache, void* v_cache, hipStream_t s) {
-  const int per = kQkThreads / (d.head_dim / 8);
+  const int per = 64 / (d.head_dim / 8);
   const int groups = (d.heads + d.kv_heads + per - 1) / per;
-  const int64_t qk = int64_t(rows) * groups;
-  const int64_t blocks = qk + int64_t((rows + kVRows - 1) / kVRows) * d.kv_heads;
+  // as many groups of a row a wave as leave 3072 waves (12 a compute unit): the more, the fewer
+  // sines are formed twice (4093 rows of 40 heads of 128: 24.6 us, 26.9 with twice the waves)
+  const int64_t all = int64_t(rows) * groups;
+  const int each = int(all / 3072 < 1 ? 1 : all / 3072 < groups ? all / 3072 : groups);
+  const int64_t vb = int64_t((rows + kVRows - 1) / kVRows) * d.kv_heads;
+  const int64_t waves = int64_t(rows) * ((groups + each - 1) / each);
+  const int64_t blocks = vb + (waves + kQkThreads / 64 - 1) / (kQkThreads / 64);
   if (blocks > 0x7fffffff) return MX_EUNSUPPORTED;
 #define MX_APPEND(HH, FF)                                                                       \
   if (d.head_dim == HH && d.f8 == FF) {                                                         \
     hipLaunchKernelGGL((append_kernel<HH, FF>), dim3(unsigned(blocks)), dim3(kQkThreads), 0, s, \
                        qkv, qkv_stride, rows, seqs, pos, rope_pos, rope, q_norm, k_norm, eps,   \
-                       table, d, k_scale, v_scale, q_out, k_cache, v_cache, groups, qk);        \
+                       table, d, k_scale, v_scale, q_out, k_cache, v_cache, groups, each,       \
+                       int(vb));                                                                \
     return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;                                   \
   }
   MX_APPEND(64, false) MX_APPEND(128, false) MX_APPEND(256, false)

@@ -69,6 +69,21 @@ __device__ __forceinline__ void copies_done() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
+// Sums over groups of N neighbouring lanes (8, 16 or 32), in every lane of the group.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return u2f(uint32_t(__builtin_amdgcn_mov_dpp(int(f2u(v)), CTRL, 0xf, 0xf, true)));
+}
+template <int N>
+__device__ __forceinline__ float group_sum(float v) {
+  v += dpp<0xb1>(v);                     // quad_perm 1 0 3 2
+  v += dpp<0x4e>(v);                     // quad_perm 2 3 0 1
+  v += dpp<0x141>(v);                    // row_half_mirror: the other four of eight
+  if (N >= 16) v += dpp<0x140>(v);       // row_mirror: the other eight of sixteen
+  if (N >= 32) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+
 // The larger of this lane's value and that of the lane 32 away.
 __device__ __forceinline__ float max_across_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);

@@ -78,7 +78,7 @@ def test_null_pointers_and_rows(mx):
 
 def test_alignment_strides_and_scales(mx):
     d = dims(mx)
-    for name, what in (("append", "qkv out k v"), ("decode", "q k v ws"), ("prefill", "q k v ws out")):
+    for name, what in (("append", "qkv out k v qn kn"), ("decode", "q k v ws"), ("prefill", "q k v ws out")):
         for m in what.split():
             assert calls(mx, d, **{m: P + 8})[name]() == mx.MX_EUNSUPPORTED, (name, m)
     assert calls(mx, d, stride=20 * 128 - 8)["append"]() == mx.MX_EINVAL
