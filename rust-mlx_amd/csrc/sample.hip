@@ -47,23 +47,77 @@ constexpr int kHistBytes = 65536 * 2;
 static_assert(kWavePieces * kWaves >= kPartPieces, "a part fits its waves");
 static_assert((kSampleMaxVocab / kPiece + 2) / kPartPieces + 1 <= kMaxParts, "parts of the longest row");
 
-// The workspace: counters of every part, then their segment bits, then their largest keys.
+// The workspace: counters of every part, then their segment bits, then their first places.
 struct Parts {
   uint16_t* counts;  // [part][65536], segments without a bit are not written
   uint32_t* bits;    // [part][32]
-  uint32_t* top;     // [part]
+  uint32_t* top;     // [part]: the first place that occurs
 };
 
-// bf16 bits as a 16-bit key that orders like the values; NaN counts as -inf, -0 as 0.
-__device__ __forceinline__ uint32_t key_of(uint32_t b) {
-  b = (b & 0x7fffu) > 0x7f80u ? 0xff80u : b;
-  b = b == 0x8000u ? 0u : b;
-  return b & 0x8000u ? b ^ 0xffffu : b | 0x8000u;
+// The place of a bf16 value among all, largest first: +inf at 0x7f, -inf at 0xff80, 0 and -0 at
+// 0x7fff; NaN lands before or behind them.
+constexpr uint32_t kInfPlace = 0x7fu, kNegInfPlace = 0xff80u;
+__device__ __forceinline__ uint32_t place_of(uint32_t b) {
+  const uint32_t d = b ^ (b & 0x8000u ? 0u : 0x7fffu);
+  return d == 0x8000u ? 0x7fffu : d;
 }
-__device__ __forceinline__ float value_of(uint32_t key) {
-  return bf16_to_f32(uint16_t(key & 0x8000u ? key ^ 0x8000u : key ^ 0xffffu));
+__device__ __forceinline__ float value_at(uint32_t place) {
+  return bf16_to_f32(uint16_t(place & 0x8000u ? place : place ^ 0x7fffu));
 }
-constexpr uint32_t kNegInfKey = 0x007fu;
+
+// e^x for x <= 0 in 64 bits: x = n ln 2 + r, the series of e^r to r^13 / 13!
+// (|r| <= ln 2 / 2: 2e-17 of it is left out), scaled by 2^n.  0 below the
+// smallest double, and for NaN; exactly 1 at 0.
+__device__ __forceinline__ double weight_of(double x) {
+  const double n = __builtin_rint(x * 1.4426950408889634074);
+  double r = __builtin_fma(-n, 0x1.62e42ff000000p-1, x);  // ln 2 to 32 bits: n times it is exact
+  r = __builtin_fma(-n, -0x1.718432a1b0e26p-35, r);         // and the rest
+  double p = 1.6059043836821613e-10;  // 1 / 13!
+  p = __builtin_fma(p, r, 2.0876756987868099e-09);
+  p = __builtin_fma(p, r, 2.5052108385441720e-08);
+  p = __builtin_fma(p, r, 2.7557319223985893e-07);
+  p = __builtin_fma(p, r, 2.7557319223985888e-06);
+  p = __builtin_fma(p, r, 2.4801587301587302e-05);
+  p = __builtin_fma(p, r, 1.9841269841269841e-04);
+  p = __builtin_fma(p, r, 1.3888888888888889e-03);
+  p = __builtin_fma(p, r, 8.3333333333333332e-03);
+  p = __builtin_fma(p, r, 4.1666666666666664e-02);
+  p = __builtin_fma(p, r, 1.6666666666666666e-01);
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  return x > -746.0 ? __builtin_ldexp(p, int(n)) : 0.0;
+}
+
+// Sums over the lanes up to each one (all 64 lanes active), in registers.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t shifted(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xf, true));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double shifted(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = shifted<CTRL, ROWS>(uint32_t(u)), hi = shifted<CTRL, ROWS>(uint32_t(u >> 32));
+  return __builtin_bit_cast(double, lo | hi << 32);
+}
+template <class T>
+__device__ __forceinline__ T scan(T v) {
+  v += shifted<0x111, 0xf>(v);  // from 1, 2, 4, 8 lanes below in the row of 16
+  v += shifted<0x112, 0xf>(v);
+  v += shifted<0x114, 0xf>(v);
+  v += shifted<0x118, 0xf>(v);
+  v += shifted<0x142, 0xa>(v);  // rows 0 and 2 to rows 1 and 3
+  v += shifted<0x143, 0xc>(v);  // the first two rows to the others
+  return v;
+}
+__device__ __forceinline__ uint32_t at_lane(uint32_t v, int l) {
+  return uint32_t(__builtin_amdgcn_readlane(int(v), l));
+}
+__device__ __forceinline__ double at_lane(double v, int l) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, uint64_t(at_lane(uint32_t(u), l)) |
+                                        uint64_t(at_lane(uint32_t(u >> 32), l)) << 32);
+}
 
 // A row in blocks of eight at 16-byte borders: block b holds tokens 8 b - lead .. + 7.
 struct Row {
@@ -100,7 +154,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(const uint16_t* __restr
                                                          int64_t stride, int n, int parts,
                                                          Parts ws) {
   extern __shared__ __align__(16) uint32_t hist[];  // 32768 words, two counters each
-  __shared__ uint32_t bits[32], best_of;
+  __shared__ uint32_t bits[32], top;
   const int row = blockIdx.x / parts, part = blockIdx.x % parts;
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   const Row r(logits + int64_t(row) * stride, n);
@@ -113,21 +167,22 @@ __global__ __launch_bounds__(kThreads) void count_kernel(const uint16_t* __restr
   for (int i = t; i < 32768 / 4; i += kThreads)
     reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
   if (t < 32) bits[t] = 0;
-  if (t == 32) best_of = 0;
+  if (t == 32) top = 0xffffu;
   __syncthreads();
-  uint32_t best = 0;
+  uint32_t least = 0xffffu;
 #pragma unroll
   for (int i = 0; i < kWavePieces; ++i)
     if (p0 + wave + kWaves * i < p1) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t k = key_of(token_of(v[i], j)), d = 0xffffu - k;
-        best = max(best, k);
-        if (k > kNegInfKey) atomicAdd(&hist[d >> 1], d & 1 ? 0x10000u : 1u);
+        const uint32_t d = place_of(token_of(v[i], j));
+        const bool counts = d - kInfPlace < kNegInfPlace - kInfPlace;  // not NaN, not -inf
+        least = min(least, counts ? d : 0xffffu);
+        if (counts) atomicAdd(&hist[d >> 1], d & 1 ? 0x10000u : 1u);
       }
     }
-  for (int o = 32; o > 0; o >>= 1) best = max(best, uint32_t(__shfl_xor(int(best), o, 64)));
-  if (lane == 0) atomicMax(&best_of, best);
+  for (int o = 32; o > 0; o >>= 1) least = min(least, uint32_t(__shfl_xor(int(least), o, 64)));
+  if (lane == 0) atomicMin(&top, least);
   __syncthreads();
   // eight counters a lane, eight lanes a segment
   uint16_t* counts = ws.counts + int64_t(blockIdx.x) * 65536;
@@ -143,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(const uint16_t* __restr
   }
   __syncthreads();
   if (t < 32) ws.bits[int64_t(blockIdx.x) * 32 + t] = bits[t];
-  if (t == 32) ws.top[blockIdx.x] = best_of;
+  if (t == 32) ws.top[blockIdx.x] = top;
 }
 
 // ---------------------------------------------------------------------------
@@ -173,10 +228,10 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
   const uint16_t* counts = ws.counts + int64_t(row) * parts * 65536;
   for (int i = t; i < parts * 32; i += kThreads) sh.bits[i] = ws.bits[int64_t(row) * parts * 32 + i];
   if (wave == kWaves - 1) {
-    uint32_t best = lane < parts ? ws.top[int64_t(row) * parts + lane] : 0;
-    for (int o = 32; o > 0; o >>= 1) best = max(best, uint32_t(__shfl_xor(int(best), o, 64)));
+    uint32_t first = lane < parts ? ws.top[int64_t(row) * parts + lane] : 0xffffu;
+    for (int o = 32; o > 0; o >>= 1) first = min(first, uint32_t(__shfl_xor(int(first), o, 64)));
     if (lane == 0) {
-      sh.top = best;
+      sh.top = first;
       sh.above = 0;
     }
   }
@@ -187,7 +242,7 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
   const float u = uniform[row];
   __syncthreads();
   const uint32_t top = sh.top;
-  if (top <= kNegInfKey) {  // uniform: nothing exceeds -inf
+  if (top >= kNegInfPlace) {  // uniform: nothing exceeds -inf
     if (t == 0) {
       tokens[row] = 0;
       if (kept) kept[row] = 0;
@@ -196,13 +251,10 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
     return;
   }
   const bool greedy = !(temp > 0.0f);
-  const double lmax = double(value_of(top)), td = greedy ? 1.0 : double(temp);
-  // the weight of a value by its place below 0xffff
-  auto weight = [&](uint32_t d) {
-    const uint32_t key = 0xffffu - d;
-    if (key == top) return 1.0;
-    const double w = exp((double(value_of(key)) - lmax) / td);
-    return w > 0.0 ? w : 0.0;  // also where both are infinite
+  const double lmax = double(value_at(top)), per_t = greedy ? 1.0 : 1.0 / double(temp);
+  auto weight = [&](uint32_t place) {
+    if (place == top) return 1.0;
+    return weight_of((double(value_at(place)) - lmax) * per_t);  // 0 also where both are infinite
   };
   // lane's counter of a segment over all parts (of one that found no room in LDS)
   auto gather = [&](int seg) {
@@ -294,24 +346,18 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
     if ((lane & 15) == 0 && above) atomicAdd(&sh.above, above);
     __syncthreads();
     // prefixes over the segments
-    double m_in = sh.mass[t];
-    uint32_t c_in = sh.count[t];
-    for (int o = 1; o < 64; o <<= 1) {
-      const double m = __shfl_up(m_in, o, 64);
-      const uint32_t c = __shfl_up(c_in, o, 64);
-      if (lane >= o) {
-        m_in += m;
-        c_in += c;
-      }
-    }
+    double m_in = scan(sh.mass[t]);
+    uint32_t c_in = scan(sh.count[t]);
     if (lane == 63) {
       sh.wmass[wave] = m_in;
       sh.wcount[wave] = c_in;
     }
     __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-      m_in += sh.wmass[w];
-      c_in += sh.wcount[w];
+    const double m_w = scan(lane < kWaves ? sh.wmass[lane] : 0.0);
+    const uint32_t c_w = scan(lane < kWaves ? sh.wcount[lane] : 0u);
+    if (wave > 0) {
+      m_in += at_lane(m_w, wave - 1);
+      c_in += at_lane(c_w, wave - 1);
     }
     sh.mass[t] = m_in;
     sh.count[t] = c_in;
@@ -336,31 +382,23 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
         c = s == kNone ? 0 : s < kSlots ? sums[s * 64 + lane] : gather(seg);
         w = c ? weight(uint32_t(seg) * 64 + lane) : 0.0;
         c = w > 0.0 ? c : 0;
-        ci = c;
-        mi = double(c) * w;
-        for (int o = 1; o < 64; o <<= 1) {
-          const double m = __shfl_up(mi, o, 64);
-          const uint32_t k = __shfl_up(ci, o, 64);
-          if (lane >= o) {
-            mi += m;
-            ci += k;
-          }
-        }
+        ci = scan(c);
+        mi = scan(double(c) * w);
         mi += seg ? sh.mass[seg - 1] : 0.0;
         ci += seg ? sh.count[seg - 1] : 0;
       };
       // the lane of the open segment that holds rank `want` (from 1), or the last with tokens
       auto lane_of = [&](uint64_t past) {
         if (!past) past = 1ull << (63 - __builtin_clzll(__ballot(c != 0) | 1ull));
-        return __builtin_ctzll(past);
+        return __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
       };
       // the mass of the first `want` tokens (1 <= want <= c_all)
       auto mass_of = [&](uint32_t want) {
         if (want >= c_all) return m_all;
         open(find([&](int s) { return sh.count[s] >= want; }));
         const int f = lane_of(__ballot(ci >= want));
-        const uint32_t over = __shfl(ci, f, 64) - want;  // tokens of the value past the rank
-        return __shfl(mi, f, 64) - double(over) * __shfl(w, f, 64);
+        const uint32_t over = at_lane(ci, f) - want;  // tokens of the value past the rank
+        return at_lane(mi, f) - double(over) * at_lane(w, f);
       };
       uint32_t keep = c_all;
       if (k > 0 && uint32_t(k) < keep) keep = uint32_t(k);
@@ -372,12 +410,12 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
         const double target = double(p) * mass;
         open(find([&](int s) { return sh.mass[s] >= target; }));
         const int f = lane_of(__ballot(mi >= target && c != 0));
-        const uint32_t cf = __shfl(c, f, 64);
-        const double wf = __shfl(w, f, 64);
-        const double before = __shfl(mi, f, 64) - double(cf) * wf;
+        const uint32_t cf = at_lane(c, f);
+        const double wf = at_lane(w, f);
+        const double before = at_lane(mi, f) - double(cf) * wf;
         double q = __builtin_ceil((target - before) / wf);
         q = q < 1.0 ? 1.0 : (q > double(cf) ? double(cf) : q);
-        keep = min(keep, uint32_t(__shfl(ci, f, 64)) - cf + uint32_t(q));
+        keep = min(keep, at_lane(ci, f) - cf + uint32_t(q));
       }
       if (floor_w > 0.0) keep = min(keep, sh.above);
       keep = max(keep, 1u);
@@ -386,22 +424,22 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
       int seg = find([&](int s) { return sh.mass[s] > at; });
       open(seg);
       int f = lane_of(__ballot(mi > at && c != 0));
-      uint32_t cf = __shfl(c, f, 64);
-      double wf = __shfl(w, f, 64);
-      const double before = __shfl(mi, f, 64) - double(cf) * wf;
+      uint32_t cf = at_lane(c, f);
+      double wf = at_lane(w, f);
+      const double before = at_lane(mi, f) - double(cf) * wf;
       double q = __builtin_floor((at - before) / wf);
       q = q < 0.0 ? 0.0 : (q > double(cf - 1) ? double(cf - 1) : q);
       uint32_t rank = uint32_t(q);  // among the value's tokens
-      if (uint32_t(__shfl(ci, f, 64)) - cf + rank >= keep) {  // a rounding past the last kept token
+      if (at_lane(ci, f) - cf + rank >= keep) {  // a rounding past the last kept token
         seg = find([&](int s) { return sh.count[s] >= keep; });
         open(seg);
         f = lane_of(__ballot(ci >= keep));
-        cf = __shfl(c, f, 64);
-        wf = __shfl(w, f, 64);
-        rank = keep - 1 - (uint32_t(__shfl(ci, f, 64)) - cf);
+        cf = at_lane(c, f);
+        wf = at_lane(w, f);
+        rank = keep - 1 - (at_lane(ci, f) - cf);
       }
       if (lane == 0) {
-        sh.chosen = 0xffffu - (uint32_t(seg) * 64 + f);
+        sh.chosen = uint32_t(seg) * 64 + f;
         sh.rank = rank;
         if (kept) kept[row] = int32_t(keep);
         if (logprob) logprob[row] = float(log(wf / mass));
@@ -416,24 +454,20 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
   // the part that holds the rank-th of the value's tokens (ids in order)
   if (wave == 0) {
     wave_sync();
-    const uint32_t d = 0xffffu - sh.chosen, seg = d >> 6, rank = sh.rank;
+    const uint32_t d = sh.chosen, seg = d >> 6, rank = sh.rank;
     uint32_t c = 0;
     if (lane < parts && (sh.bits[lane * 32 + (seg >> 5)] >> (seg & 31) & 1))
       c = counts[int64_t(lane) * 65536 + d];
-    uint32_t sum = c;
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t v = __shfl_up(sum, o, 64);
-      sum += lane >= o ? v : 0;
-    }
+    const uint32_t sum = scan(c);
     const int f = __builtin_ctzll(__ballot(sum > rank) | (1ull << 63));
-    const uint32_t before = uint32_t(__shfl(sum, f, 64)) - uint32_t(__shfl(c, f, 64));
+    const uint32_t before = at_lane(sum, f) - at_lane(c, f);
     if (lane == 0) {
       sh.part = min(uint32_t(f), uint32_t(parts - 1));
       sh.rank = rank - before;
     }
   }
   __syncthreads();
-  const uint32_t chosen = sh.chosen, rank = sh.rank;
+  const uint32_t place = sh.chosen, rank = sh.rank;
   const Row r(logits + int64_t(row) * stride, n);
   const int each = (r.pieces() + parts - 1) / parts;
   const int p0 = int(sh.part) * each, np = min(r.pieces(), p0 + each) - p0;
@@ -447,24 +481,20 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
     if (wave + kWaves * i >= np) continue;
     uint32_t c = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c += key_of(token_of(v[i], j)) == chosen;
-    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+    for (int j = 0; j < 8; ++j) c += place_of(token_of(v[i], j)) == place;
+    c = at_lane(scan(c), 63);
     if (lane == 0) sh.pieces[wave + kWaves * i] = c;
   }
   __syncthreads();
   // the piece that holds it: two a lane
   const uint32_t a = 2 * lane < np ? sh.pieces[2 * lane] : 0;
   const uint32_t b = 2 * lane + 1 < np ? sh.pieces[2 * lane + 1] : 0;
-  uint32_t sum = a + b;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t x = __shfl_up(sum, o, 64);
-    sum += lane >= o ? x : 0;
-  }
+  const uint32_t sum = scan(a + b);
   const uint64_t past = __ballot(sum > rank);
   if (!past) return;  // unreachable: the part's counters say that it is there
   const int f = __builtin_ctzll(past);
-  uint32_t before = uint32_t(__shfl(sum, f, 64)) - uint32_t(__shfl(a + b, f, 64));
-  const uint32_t af = __shfl(a, f, 64);
+  uint32_t before = at_lane(sum, f) - at_lane(a + b, f);
+  const uint32_t af = at_lane(a, f);
   const int piece = before + af > rank ? 2 * f : 2 * f + 1;
   if (piece & 1) before += af;
 #pragma unroll
@@ -472,16 +502,12 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
     if (piece != wave + kWaves * i) continue;  // uniform: one wave's one piece
     uint32_t own = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) own += key_of(token_of(v[i], j)) == chosen;
-    uint32_t upto = own;
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t x = __shfl_up(upto, o, 64);
-      upto += lane >= o ? x : 0;
-    }
+    for (int j = 0; j < 8; ++j) own += place_of(token_of(v[i], j)) == place;
+    const uint32_t upto = scan(own);
     uint32_t at = before + upto - own;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (key_of(token_of(v[i], j)) == chosen) {
+      if (place_of(token_of(v[i], j)) == place) {
         if (at == rank) tokens[row] = uint32_t(r.first(p0 + piece, lane) + j);
         ++at;
       }
