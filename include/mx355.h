@@ -501,12 +501,11 @@ mx_status mx_attn_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_str
  * position p of sequence s lies at p % page_size of page
  * table[s][p / page_size].  An entry outside [0, pages) holds no positions:
  * appends to it write nothing, attention leaves its positions out.  Sequences
- * may share pages (a common prefix); what no sequence's length covers may hold
- * anything, NaN too.  The values of positions that a length covers must be
- * finite.
+ * may share pages (a common prefix).  What a row does not see may hold anything,
+ * infinities and NaN too: positions past a length, and of later rows.
  *
  * head_dim 64, 128 or 256; 1..16 q heads per kv head; page_size 16, 32, 64, 128
- * or 256 (MX_EUNSUPPORTED otherwise).  q, qkv rows (qkv_stride % 8 == 0), norms,
+ * or 256; at most 2^30 positions a sequence (MX_EUNSUPPORTED otherwise).  q, qkv rows (qkv_stride % 8 == 0), norms,
  * out, workspaces and both caches are 16-byte aligned.  The pointers and the
  * stream belong to the current device.  A workspace serves one call at a time: calls that
  * may overlap (two streams, two captured graphs) need one each. */

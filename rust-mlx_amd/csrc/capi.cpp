@@ -562,8 +562,8 @@ const char* check_pages(const mx_page_dims* dims, PageDims* d, int* code) {
   if ((1 << log2) != dims->page_size) return "page_size must be 16, 32, 64, 128 or 256";
   if (dims->dtype != MX_DT_BF16 && dims->dtype != MX_DT_F8E4M3)
     return "dtype must be MX_DT_BF16 or MX_DT_F8E4M3";
-  if ((int64_t(dims->table_width) << log2) > 0x7fffffff)
-    return "table_width * page_size must stay below 2^31";
+  if ((int64_t(dims->table_width) << log2) > (1 << 30))
+    return "table_width * page_size must be at most 2^30";
   *code = MX_EINVAL;
   if (dims->page_stride < int64_t(dims->kv_heads) * dims->page_size * dims->head_dim ||
       dims->page_stride % 16 != 0)
@@ -690,6 +690,8 @@ MX_ABI mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, i
       rc != MX_OK)
     return rc;
   MX_CHECK(rows >= 0, MX_EINVAL, "mx_attn_paged_prefill: negative rows");
+  MX_CHECK(int64_t(rows) * d.heads <= 0x7fffffff, MX_EUNSUPPORTED,
+           "mx_attn_paged_prefill: rows * heads must stay below 2^31");
   if (rows == 0) return MX_OK;
   MX_CHECK(q && starts && lens && table && k_cache && v_cache && out &&
                (workspace || paged_prefill_workspace(rows, d) == 0),

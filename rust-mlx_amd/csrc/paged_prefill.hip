@@ -183,6 +183,8 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o, 64));
   low = __builtin_amdgcn_readfirstlane(low);
 
+  const int sees_all = prior + b.pair0 / group;  // the last key that every pair of the block sees
+
   const char* kc = static_cast<const char*>(k_cache);
   const char* vc = static_cast<const char*>(v_cache);
   constexpr int E = F8 ? 1 : 2;
@@ -426,6 +428,41 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
       m_run = mn;
     }
     const float ref = m_run == neg_inf() ? 0.0f : m_run;  // no key yet: every weight is 0
+    // Where a pair does not see all of the tile, its p of 0 must not meet an infinite or NaN value:
+    // such values go to the sums of the pairs that see them (they stay infinite or NaN whatever
+    // their weight) and become 0 for the product.
+    if (tile + KT - 1 > sees_all) {  // uniform
+      char* vs = lds + (D + stage) * kPart;
+      auto odd = [](uint32_t w) MX_LAMBDA {
+        return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+      };
+      bool some = false;
+      for (int i = t; i < HD * VP; i += 64 * NW) {
+        const uint4 v = *reinterpret_cast<const uint4*>(vs + i * 16);
+        some |= odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w);
+      }
+      if (__syncthreads_or(some)) {
+        for (int key = 0; key < KT; ++key) {
+          const bool in = tile + key <= limit && (parts >> (key >> 4) & 1);
+#pragma unroll
+          for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int dim = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
+              const uint16_t v = *reinterpret_cast<const uint16_t*>(
+                  vs + (dim * VP + ((key >> 3) ^ v_swizzle<HD>(dim))) * 16 + (key & 7) * 2);
+              if (in && (v & 0x7f80u) == 0x7f80u) o[n][r] += bf16_to_f32(v);
+            }
+        }
+        __syncthreads();
+        for (int i = t; i < HD * VP * 8; i += 64 * NW) {
+          uint16_t* v = reinterpret_cast<uint16_t*>(vs) + i;
+          if ((*v & 0x7f80u) == 0x7f80u) *v = 0;
+        }
+        __syncthreads();
+        each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(stage, i); });
+      }
+    }
     uint32_t pb[KB * 8];
     auto pair = [&](auto j) MX_LAMBDA {
       constexpr int kb = j / 8, r = 2 * (j % 8);

@@ -227,6 +227,35 @@ def test_prefill_missing_pages(mx, f8):
     assert (got[60:] == 0).all()
 
 
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("heads,kv,hd,total", [(8, 2, 128, 150), (16, 2, 256, 77), (4, 4, 64, 200)])
+def test_what_later_rows_hold_stays_unseen(mx, heads, kv, hd, total, f8):
+    """Infinite and NaN keys and values of a prompt's own later positions: earlier rows are as if they were
+    other numbers; the rows that see one are not finite where they must not be."""
+    c = Paged(mx, heads, kv, hd, 32, [total], f8, seed=20)
+    rng = np.random.default_rng(21)
+    q = to_bf(0.5 * rng.standard_normal((total, heads, hd)))
+    ref, mag = attend(c, 0, bf(q).astype(np.float64), np.arange(total) + 1)
+    at = total - 40  # inside the last blocks' tiles
+    nan = 0x7F if f8 else 0x7FC0
+    kc, vc = c.kview(), c.vview()
+    for p, d, bits in ((at, 3, nan), (at + 7, hd - 1, nan if f8 else 0x7F80), (at + 20, 9, nan if f8 else 0xFF80)):
+        vc[c.table[0, p // 32], 0, d, p % 32] = bits
+    kc[c.table[0, (total - 1) // 32], 0, (total - 1) % 32, 5] = nan  # the last key
+    c.k[:, :kc[0].size], c.v[:, :vc[0].size] = kc.reshape(c.pages, -1), vc.reshape(c.pages, -1)
+    c.upload()
+    got = run_prefill(mx, c, q, [0, total], [total])
+    group = heads // kv
+    seen = np.zeros(got.shape, bool)  # outputs that one of them reaches (kv head 0's)
+    seen[at:, :group, 3] = seen[at + 7:, :group, hd - 1] = seen[at + 20:, :group, 9] = True
+    seen[total - 1, :group] = True
+    g = bf(got).astype(np.float64)
+    assert not np.isfinite(g[seen]).any()
+    if not f8:
+        assert (g[at + 7:-1, :group, hd - 1] == np.inf).all() and (g[at + 20:-1, :group, 9] == -np.inf).all()
+    close(np.where(seen, 0, got).astype(np.uint16), np.where(seen, 0, ref), np.where(seen, 0, mag), False)
+
+
 def reference_append(x, c, pos, rope_pos, inv_freq, pair_axis, rot, qn, kn, eps=1e-6):
     """Normalised and rotated q and k, and v, in 64 bits."""
     rows, hd, h, kv = len(x), c.hd, c.heads, c.kv
