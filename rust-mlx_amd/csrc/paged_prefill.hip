@@ -189,7 +189,17 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   const char* vc = static_cast<const char*>(v_cache);
   constexpr int E = F8 ? 1 : 2;
   const int page = 1 << d.page_log2, last_page = max(b.len - 1, 0) >> d.page_log2;
-  const float sl2 = scale * kLog2e * (F8 && k_scale ? k_scale[kvh] : 1.0f);
+  float sl2 = scale * kLog2e * (F8 && k_scale ? k_scale[kvh] : 1.0f);
+  // A tile's maximum is taken before the product with sl2, and masked scores of -inf stay below
+  // everything only under a positive one: the sign of a kv head's scale, or its zero, goes to q.
+  if constexpr (F8) {
+    const uint32_t flip = sl2 < 0.0f ? 0x80008000u : 0u, keep = sl2 == 0.0f ? 0u : 0xffffffffu;
+    sl2 = sl2 < 0.0f ? -sl2 : sl2 == 0.0f ? 1.0f : sl2;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      qb[s] = make_uint4((qb[s].x & keep) ^ flip, (qb[s].y & keep) ^ flip, (qb[s].z & keep) ^ flip,
+                         (qb[s].w & keep) ^ flip);
+  }
   const int64_t head_at = (int64_t(kvh) << d.page_log2) * HD;
 
   // Page ids of a tile's 16-key parts, through scalar loads (they have a counter of their
@@ -289,10 +299,10 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
 
-  // Tile ti's K and V lie in stages ti % D.  Two workgroups (or four waves more of this one) share
-  // each matrix unit: while one forms its exponentials, the other has the products.  Forming a
-  // tile's exponentials under the next tile's products within one wave was no faster (HD 128,
-  // 8192 tokens: 608 us against 565), the two waves do that already.
+  // Tile ti's K and V lie in stages ti % D.  Two workgroups share each matrix unit: while a wave of
+  // one forms its exponentials, one of the other has the products.  Forming a tile's exponentials
+  // under the next tile's products within one wave was no faster (HD 128, 8192 tokens: 608 us
+  // against 565), the two workgroups do that already.
   constexpr int kCopies = F8 ? 0 : CK + CV;  // of a step, by a wave
   constexpr int R = HD == 256 ? 2 : 4;       // operands read ahead of their products
   // The order as it is written: left alone, the compiler reads each operand just before its

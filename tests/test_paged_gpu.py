@@ -256,6 +256,26 @@ def test_what_later_rows_hold_stays_unseen(mx, heads, kv, hd, total, f8):
     close(np.where(seen, 0, got).astype(np.uint16), np.where(seen, 0, ref), np.where(seen, 0, mag), False)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(12, 3, 64), (6, 3, 128), (6, 3, 256)])
+def test_scales_of_either_sign_and_zero(mx, heads, kv, hd):
+    """A kv head's scale may be negative, or 0 (then every position weighs the same).  At 64 dims scores
+    reach over more than 128 octaves, past what fp32 would forgive a maximum of the wrong sign.  Their
+    error, at worst hd 2^-24 sum |q k| / sqrt(hd) = hd^1.5 2^-24 0.64 |q| with |q| = 16 (64 / hd)^1.5, is
+    under 2^-11.6: the bound of the other tests holds."""
+    total = 170
+    c = Paged(mx, heads, kv, hd, 16, [total], True, seed=22)
+    c.ks *= np.array([-1, 0, 1], np.float32)
+    c.vs *= np.array([1, -1, 0], np.float32)
+    c.upload()
+    rng = np.random.default_rng(23)
+    q = to_bf(16 * (64 / hd) ** 1.5 * rng.standard_normal((total, heads, hd)))
+    ref, mag = attend(c, 0, bf(q).astype(np.float64), np.arange(total) + 1)
+    close(run_prefill(mx, c, q, [0, total], [total]), ref, mag, False)
+    few = [0, 1, 33, total - 1]
+    got = run_decode(mx, c, np.ascontiguousarray(q[few]), [i + 1 for i in few], seqs=[0] * len(few))
+    close(got, ref[few], mag[few], True)
+
+
 def reference_append(x, c, pos, rope_pos, inv_freq, pair_axis, rot, qn, kn, eps=1e-6):
     """Normalised and rotated q and k, and v, in 64 bits."""
     rows, hd, h, kv = len(x), c.hd, c.heads, c.kv
