@@ -689,10 +689,10 @@ int paged_append(const uint16_t* qkv, int64_t qkv_stride, int rows, const int32_
                  void* k_cache, void* v_cache, hipStream_t s) {
   const int per = 64 / (d.head_dim / 8);
   const int groups = (d.heads + d.kv_heads + per - 1) / per;
-  // as many groups of a row a wave as leave 3072 waves (12 a compute unit): the more, the fewer
-  // sines are formed twice (4093 rows of 40 heads of 128: 24.6 us, 26.9 with twice the waves)
-  const int64_t all = int64_t(rows) * groups;
-  const int each = int(all / 3072 < 1 ? 1 : all / 3072 < groups ? all / 3072 : groups);
+  // as many groups of a row a wave as leave 12 waves a compute unit: the more, the fewer sines
+  // are formed twice (4093 rows of 40 heads of 128: 24.6 us, 26.9 with twice the waves)
+  const int64_t share = int64_t(rows) * groups / (12 * 256);
+  const int each = int(share < 1 ? 1 : share < groups ? share : groups);
   const int64_t vb = int64_t((rows + kVRows - 1) / kVRows) * d.kv_heads;
   const int64_t waves = int64_t(rows) * ((groups + each - 1) / each);
   const int64_t blocks = vb + (waves + kQkThreads / 64 - 1) / (kQkThreads / 64);
