@@ -63,6 +63,16 @@ __device__ __forceinline__ void copy_to_lds(const char* src, uint32_t lds) {
                : "v"(src), "s"(lds)
                : "memory");
 }
+// The same from src + off, src the same for the wave.
+__device__ __forceinline__ void copy_to_lds(const char* src, uint32_t off, uint32_t lds) {
+  const uint64_t at = reinterpret_cast<uint64_t>(src);
+  const uint64_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(at))));
+  const uint64_t hi = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(at >> 32))));
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(hi << 32 | lo), "s"(lds)
+               : "memory");
+}
 // Waits until at most `N` of the wave's vector memory operations, the latest, are under way.
 template <int N>
 __device__ __forceinline__ void copies_done() {

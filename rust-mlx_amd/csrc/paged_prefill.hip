@@ -250,10 +250,12 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   };
   // piece i of a wave's copies, to LDS, or of e4m3 (16 values: two pieces of LDS) to registers
   constexpr int CK = F8 ? NK / 2 : NK, CV = F8 ? NVV / 2 : NVV;
+  // K piece `lane` of the wave's rows, in bytes from the first; piece 64 i + lane differs in the
+  // bits of its 1 KB and of the rows' part in the exchange
+  const uint32_t koff = lane / KP * (HD * 2) + 16 * ((lane % KP) ^ k_swizzle<HD>(RPW * wave + lane / KP));
   auto copy_k = [&](const char* from, int stage, int i) MX_LAMBDA {
     if constexpr (!F8) {
-      const int slot = 64 * i + lane, r = slot / KP, p = slot % KP;
-      copy_to_lds(from + (r * HD + 8 * (p ^ k_swizzle<HD>(RPW * wave + r))) * E,
+      copy_to_lds(from, koff ^ (1024 * i | 16 * k_swizzle<HD>(64 / KP * i)),
                   lds_at + stage * kPart + RPW * wave * KP * 16 + 1024 * i);
     } else {
       const int slot = 64 * i + lane, r = slot / (KP / 2), p = slot % (KP / 2);
@@ -393,21 +395,18 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     const char* kf = k_from(at, id);
     const char* vf = v_from(at, id);
     // Issued together the copies hold up every wave of the workgroup at once, for as long as the
-    // memory path takes for all of them, so they are spread over the scores' products; with 256
-    // dims there are no registers for their addresses meanwhile.
+    // memory path takes for all of them, so they are spread over the scores' products (512 rows
+    // on 12001 keys, 256 dims: 124 us against 133).
     auto copy = [&](auto i) MX_LAMBDA {
       if constexpr (i < CK)
         copy_k(kf, ahead, i);
       else
         copy_v(vf, ahead, i - CK);
     };
-    if constexpr (HD == 256) each<CK + CV>(copy);
     floatx16_t sc[KB];
     scores(stage, sc, [&](auto i) MX_LAMBDA {
-      if constexpr (HD < 256) {
-        constexpr int n = KS * KB, first = i * (CK + CV) / n, end = (i + 1) * (CK + CV) / n;
-        each<end - first>([&](auto j) MX_LAMBDA { copy(std::integral_constant<int, first + j>{}); });
-      }
+      constexpr int n = KS * KB, first = i * (CK + CV) / n, end = (i + 1) * (CK + CV) / n;
+      each<end - first>([&](auto j) MX_LAMBDA { copy(std::integral_constant<int, first + j>{}); });
     });
     uint4 a[R];
     each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(stage, i); });
