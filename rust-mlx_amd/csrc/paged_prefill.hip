@@ -75,10 +75,11 @@ __device__ __forceinline__ bool find_block(const int32_t* __restrict__ starts,
   int before = 0;
   for (int s0 = 0; s0 < d.sequences; s0 += 64) {
     const int s = s0 + lane;
-    int first = 0, count = 0;
+    int first = 0, count = 0, len = 0;
     if (s < d.sequences) {
       first = min(max(starts[s], 0), rows);
       count = max(min(starts[s + 1], rows) - first, 0);
+      len = lens[s];
     }
     const int n = int((int64_t(count) * group + kPairs - 1) / kPairs);
     const int sum = wave_scan(n);
@@ -91,7 +92,7 @@ __device__ __forceinline__ bool find_block(const int32_t* __restrict__ starts,
       out->count = __builtin_amdgcn_readlane(count, f);
       out->pair0 = (before + __builtin_amdgcn_readlane(sum, f) - 1 - want) * kPairs;
       const int64_t most = int64_t(d.table_width) << d.page_log2;
-      const int len = lens[out->seq];
+      len = __builtin_amdgcn_readlane(len, f);
       out->len = len < 0 ? 0 : (len > most ? int(most) : len);
       return true;
     }
@@ -164,9 +165,9 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   const bool whole = tile0 == 0 && tile1 == tiles;  // also a block without keys
   if (tile0 >= tile1 && !(split == 0 && tiles == 0)) return;
 
-  // this lane's pair
-  const int pair = b.pair0 + 32 * wave + col;
-  const bool alive = pair < pairs;
+  // this lane's pair; lanes past the last pair take that, see nothing and write nothing
+  const bool alive = b.pair0 + 32 * wave + col < pairs;
+  const int pair = min(b.pair0 + 32 * wave + col, pairs - 1);
   const int token = pair / group, head = kvh * group + pair - token * group;
   const int64_t qrow = b.first + token;
   const int limit = alive ? prior + token : -1;  // the last key that the pair sees
@@ -174,8 +175,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   {
     const uint16_t* src = q + (qrow * d.heads + head) * HD + 8 * h;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-      qb[s] = alive ? *reinterpret_cast<const uint4*>(src + 16 * s) : make_uint4(0, 0, 0, 0);
+    for (int s = 0; s < KS; ++s) qb[s] = *reinterpret_cast<const uint4*>(src + 16 * s);
   }
   // the wave's pairs see at least the keys up to low
   int low = alive ? limit : 0x7fffffff;
