@@ -305,6 +305,10 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   // one forms its exponentials, one of the other has the products.  Forming a tile's exponentials
   // under the next tile's products within one wave was no faster (HD 128, 8192 tokens: 608 us
   // against 565), the two workgroups do that already.
+  // With 256 dims of e4m3 the registers hold a tile's K or V on their way, not both: K is widened
+  // after the scores, V after P V (512 rows on 12001 keys: 152 us, both after P V 181; with 128
+  // dims both together are faster, four prompts of up to 2047 on up to 3001: 147 us against 151).
+  constexpr bool kHalves = F8 && HD == 256;
   constexpr int kCopies = F8 ? 0 : CK + CV;  // of a step, by a wave
   constexpr int R = HD == 256 ? 2 : 4;       // operands read ahead of their products
   // The order as it is written: left alone, the compiler reads each operand just before its
@@ -405,9 +409,14 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     };
     floatx16_t sc[KB];
     scores(stage, sc, [&](auto i) MX_LAMBDA {
-      constexpr int n = KS * KB, first = i * (CK + CV) / n, end = (i + 1) * (CK + CV) / n;
+      constexpr int nc = kHalves ? CK : CK + CV;
+      constexpr int n = KS * KB, first = i * nc / n, end = (i + 1) * nc / n;
       each<end - first>([&](auto j) MX_LAMBDA { copy(std::integral_constant<int, first + j>{}); });
     });
+    if constexpr (kHalves) {
+      store_k(ahead);
+      each<CV>([&](auto i) MX_LAMBDA { copy_v(vf, ahead, i); });
+    }
     uint4 a[R];
     each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(stage, i); });
     if (tile + KT - 1 > low || parts != kAllParts) {
@@ -453,11 +462,13 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
       if (__syncthreads_or(some)) {
         for (int key = 0; key < KT; ++key) {
           const bool in = tile + key <= limit && (parts >> (key >> 4) & 1);
+          int half = h;  // addresses formed for each key: kept over the keys they would take
+          asm volatile("" : "+v"(half));  // a register for every sum, in the loop over tiles too
 #pragma unroll
           for (int n = 0; n < ND; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int dim = 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
+              const int dim = 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
               const uint16_t v = *reinterpret_cast<const uint16_t*>(
                   vs + (dim * VP + ((key >> 3) ^ v_swizzle<HD>(dim))) * 16 + (key & 7) * 2);
               if (in && (v & 0x7f80u) == 0x7f80u) o[n][r] += bf16_to_f32(v);
@@ -503,7 +514,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     // read here, the ids are there after the barrier; before, they would hold up the first
     // products, whose LDS reads wait on the same counter
     id = ids_of(min((ti + D) * KT, last));
-    store_k(ahead);
+    if constexpr (!kHalves) store_k(ahead);
     store_v(ahead);
     stage = stage == D - 1 ? 0 : stage + 1;
   }
