@@ -21,10 +21,16 @@
 //
 // Tiles are copied to LDS one ahead (e4m3 through registers, where it is
 // widened once for all waves).  16-byte pieces of a row are exchanged by the
-// row's number, so that operand reads of 16 rows meet no bank twice.
+// row's number, so that operand reads of 8 rows meet no bank twice (of 16 rows
+// at 128 dims too: 562 us against 555 for 8192 tokens, the bits cost more).
 //
 // With few workgroups the keys are split over several, and a second launch
 // joins their partials.
+//
+// The matrix cores and the vector ALUs bound it together, under a falling clock:
+// 8192 tokens of 32 q / 8 kv heads of 128 take 555 to 580 us (950 to 990 TFLOP/s).
+// 512 rows of 16 / 2 heads of 256 on 12001 keys take 124 us, 17 of them to join
+// eight splits; there the registers bound it, see R and kHalves.
 #include <type_traits>
 #include <utility>
 
@@ -110,13 +116,21 @@ struct Item {
 __host__ __device__ __forceinline__ bool by_xcd(int kv_heads, int splits) {
   return kv_heads * splits >= 8;
 }
-__device__ __forceinline__ Item item_of(int id, int kv_heads, int splits) {
+// Where all workgroups run at once, the second 256 beside the first on the same compute units,
+// those take the blocks from the last one on: a sequence's blocks have fewer and fewer keys, and
+// so a long one shares its unit with a short one (four prompts of up to 2047 rows on up to 3001,
+// e4m3: 144 us against 152).
+__device__ __forceinline__ Item item_of(int id, int grid, int kv_heads, int splits) {
   const int pairs = kv_heads * splits;
-  if (!by_xcd(kv_heads, splits))
-    return Item{id / pairs, id % kv_heads, id / kv_heads % splits};
-  const int each = (pairs + 7) / 8, j = id >> 3;  // pairs of an XCD
-  const int pair = (id & 7) + 8 * (j % each);
-  return Item{j / each, pair % kv_heads, pair / kv_heads};  // split >= splits: none
+  const bool xcd = by_xcd(kv_heads, splits);
+  const int each = (pairs + 7) / 8;  // pairs of an XCD
+  const int j = id >> 3, pair = xcd ? (id & 7) + 8 * (j % each) : id % pairs;
+  int block = xcd ? j / each : id / pairs;
+  if (grid > 256 && grid <= 512) {
+    const int a_block = xcd ? 8 * each : pairs, blocks = grid / a_block, first = 256 / a_block;
+    if (block >= first) block = blocks - 1 - (block - first);
+  }
+  return Item{block, pair % kv_heads, pair / kv_heads};  // split >= splits: none
 }
 
 template <int HD>
@@ -150,7 +164,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int col = lane & 31, h = lane >> 5;
   const int group = d.heads / d.kv_heads;
-  const Item it = item_of(blockIdx.x, d.kv_heads, splits);
+  const Item it = item_of(blockIdx.x, gridDim.x, d.kv_heads, splits);
   if (it.split >= splits) return;
   const int kvh = it.kvh, split = it.split;
   Block b;
@@ -312,9 +326,9 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   constexpr int kCopies = F8 ? 0 : CK + CV;  // of a step, by a wave
   constexpr int R = HD == 256 ? 2 : 4;       // operands read ahead of their products
   // The order as it is written: left alone, the compiler reads each operand just before its
-  // product.  With 256 dims it has no registers for that, and its own order is faster (141 us
-  // against 191 for 512 rows on 12001 keys), and so it is with e4m3 (146 against 152 for four
-  // prompts of up to 2047 on up to 3001).
+  // product.  With 256 dims it has no registers for that, and its own order is faster (124 us
+  // against 125 for 512 rows on 12001 keys; operands four ahead 132), and so it is with e4m3 (151
+  // against 157 for four prompts of up to 2047 on up to 3001, before their blocks' order).
   auto keep_order = [] {
     if constexpr (HD < 256 && !F8) __builtin_amdgcn_sched_barrier(0);
   };
@@ -632,7 +646,7 @@ Layout layout_of(int rows, const PageDims& d) {
   l.blocks = int64_t(rows) * (d.heads / d.kv_heads) / kPairs + (d.sequences < rows ? d.sequences : rows);
   // as many splits as bring the launch to two workgroups a compute unit, each with at least four
   // tiles of the longest possible context; in eights with the kv heads where that is possible,
-  // for whole XCDs (512 rows on 12001 keys, two kv heads: 8 splits 147 us, 7 splits 162)
+  // for whole XCDs (512 rows on 12001 keys, two kv heads: 8 splits 126 us, 7 splits 138)
   const int64_t all = l.blocks * d.kv_heads, want = 512 / (all < 1 ? 1 : all);
   const int64_t room = (int64_t(d.table_width) << d.page_log2) / 256;
   int64_t s = want < room ? want : room;
