@@ -538,7 +538,8 @@ typedef struct mx_rope_axes {
  * one rounding; v as it is.  Row r is position pos[r] of sequence seqs[r]
  * (seqs NULL: sequence r).  An e4m3 cache takes round(clamp(value / scale,
  * +-448)); k_scale / v_scale: device fp32 [kv_heads], NULL for 1 (and ignored
- * for bf16).  rope_pos: int32 [axes][rows].  A row whose sequence is not in
+ * for bf16), finite, of either sign (attention takes 0 too; here it divides, so
+ * values of 0 become NaN).  rope_pos: int32 [axes][rows].  A row whose sequence is not in
  * [0, sequences) is padding: nothing of it is written; a position outside the
  * table writes q_out only.  Rows must not name the same position twice.
  * Replaces, for paged caches, the norms, RoPE and KvCache::update of
