@@ -394,8 +394,8 @@ mx_status mx_argmax_bf16(const uint16_t* logits, int32_t rows, int32_t n, uint32
  * top_k[r] tokens the shortest prefix with at least top_p[r] of their mass is
  * kept, of that the tokens with w_j >= min_p[r]; token 0 of the order always
  * is.  The token is the first whose prefix mass exceeds uniform[r] times the
- * kept mass.  Counts are exact and masses 64-bit sums, so a row's token
- * depends on its own inputs only, bit for bit.
+ * kept mass, from uniform 1 on the last one kept.  Counts are exact and masses
+ * 64-bit sums, so a row's token depends on its own inputs only, bit for bit.
  * All per-row arrays are on the device.  NULL, or: temperature NULL = 1, <= 0
  * or NaN = greedy; top_k NULL or <= 0 = off; top_p NULL, >= 1 or NaN = off, <= 0
  * keeps one token; min_p NULL, <= 0 or NaN = off.  uniform is cut to [0, 1],

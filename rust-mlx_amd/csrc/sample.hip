@@ -6,13 +6,13 @@
 //   top-p  the shortest prefix with a mass of at least p times the first k's
 //   min-p  those with w_j >= min_p
 // n is the shortest of them (at least one token), and the sampled token is the
-// first whose prefix mass exceeds u times the mass of n.
+// first whose prefix mass exceeds u times the mass of n (the n-th from u = 1 on).
 //
 // bf16 has 65536 values, so a row is known by how often each occurs, and needs an
 // exponential per occurring value instead of one per token, without any sort.
 // Counts are exact and masses are sums of few products in 64 bits, so neither the
-// order of the atomics nor the launch shape can change a token, and a u next to a
-// border falls on the side that the definition says.
+// order of the atomics nor the launch shape can change a token: a u within the
+// sums' rounding of a border falls on one side of it, always the same.
 //
 // Launch 1 counts: a workgroup takes a part of a row (at most 65024 tokens, so
 // 16-bit counters suffice: 128 KB of LDS for all values) and writes the segments
@@ -109,6 +109,16 @@ __device__ __forceinline__ T scan(T v) {
   v += shifted<0x118, 0xf>(v);
   v += shifted<0x142, 0xa>(v);  // rows 0 and 2 to rows 1 and 3
   v += shifted<0x143, 0xc>(v);  // the first two rows to the others
+  return v;
+}
+// The largest of the lanes up to each one (none negative).
+__device__ __forceinline__ double scan_max(double v) {
+  v = fmax(v, shifted<0x111, 0xf>(v));
+  v = fmax(v, shifted<0x112, 0xf>(v));
+  v = fmax(v, shifted<0x114, 0xf>(v));
+  v = fmax(v, shifted<0x118, 0xf>(v));
+  v = fmax(v, shifted<0x142, 0xa>(v));
+  v = fmax(v, shifted<0x143, 0xc>(v));
   return v;
 }
 __device__ __forceinline__ uint32_t at_lane(uint32_t v, int l) {
@@ -346,28 +356,34 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
     }
     if ((lane & 15) == 0 && above) atomicAdd(&sh.above, above);
     __syncthreads();
-    // prefixes over the segments
+    // Prefixes over the segments.  Rounding depends on the order of a sum, which differs from lane to
+    // lane in the scan: only the prefixes of occurring segments count, each raised to the largest
+    // before it, and the waves' totals add up one after another.  So the prefixes never fall and an
+    // empty segment has exactly its predecessor's: the first to pass a bound is one with tokens.
+    const uint32_t c_own = sh.count[t];
     double m_in = scan(sh.mass[t]);
-    uint32_t c_in = scan(sh.count[t]);
+    m_in = scan_max(c_own ? m_in : 0.0);
+    uint32_t c_in = scan(c_own);
     if (lane == 63) {
       sh.wmass[wave] = m_in;
       sh.wcount[wave] = c_in;
     }
     __syncthreads();
-    const double m_w = scan(lane < kWaves ? sh.wmass[lane] : 0.0);
+    const double m_w = lane < kWaves ? sh.wmass[lane] : 0.0;
     const uint32_t c_w = scan(lane < kWaves ? sh.wcount[lane] : 0u);
-    if (wave > 0) {
-      m_in += at_lane(m_w, wave - 1);
-      c_in += at_lane(c_w, wave - 1);
-    }
+    double m_before = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves - 1; ++w) m_before += w < wave ? at_lane(m_w, w) : 0.0;
+    m_in += m_before;
+    if (wave > 0) c_in += at_lane(c_w, wave - 1);
     sh.mass[t] = m_in;
     sh.count[t] = c_in;
     __syncthreads();
     if (wave == 0) {
       const double m_all = sh.mass[kSegments - 1];
       const uint32_t c_all = sh.count[kSegments - 1];
-      // the first segment whose prefix passes (the last with tokens where none does): over the
-      // waves' last segments, then within one wave's
+      // the first segment whose prefix passes (the last with tokens where none does): over every
+      // 16th segment, then within sixteen
       auto find = [&](auto&& passes) {
         uint64_t b = __ballot(passes(16 * lane + 15));
         if (!b) b = __ballot(sh.count[16 * lane + 15] >= c_all);
@@ -431,7 +447,8 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(
       double q = __builtin_floor((at - before) / wf);
       q = q < 0.0 ? 0.0 : (q > double(cf - 1) ? double(cf - 1) : q);
       uint32_t rank = uint32_t(q);  // among the value's tokens
-      if (at_lane(ci, f) - cf + rank >= keep) {  // a rounding past the last kept token
+      // all of the mass, or a rounding past the last kept token: that token
+      if (u >= 1.0f || at_lane(ci, f) - cf + rank >= keep) {
         seg = find([&](int s) { return sh.count[s] >= keep; });
         open(seg);
         f = lane_of(__ballot(ci >= keep));
