@@ -502,7 +502,9 @@ mx_status mx_attn_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_str
  * table[s][p / page_size].  An entry outside [0, pages) holds no positions:
  * appends to it write nothing, attention leaves its positions out.  Sequences
  * may share pages (a common prefix).  What a row does not see may hold anything,
- * infinities and NaN too: positions past a length, and of later rows.
+ * infinities and NaN too: positions past a length, and of later rows.  An
+ * infinite value that it does see makes its output infinite, NaN beside a NaN
+ * or one of the other sign (in a prompt also where its weight is 0 in fp32).
  *
  * head_dim 64, 128 or 256; 1..16 q heads per kv head; page_size 16, 32, 64, 128
  * or 256; at most 2^30 positions a sequence (MX_EUNSUPPORTED otherwise).  q, qkv rows (qkv_stride % 8 == 0), norms,

@@ -1,4 +1,6 @@
 // The paged cache: rows appended to it, and attention of one new token a row over it.
+#include <type_traits>
+
 #include "paged_core.hpp"
 
 namespace mx {
@@ -315,6 +317,21 @@ __device__ __forceinline__ Plan make_plan(const int32_t* seqs, const int32_t* le
   return p;
 }
 
+// The sum of the infinite and NaN values among positions k0 .. k1 - 1 of one dim (at: from a page's
+// start to that dim's first position), 0 where there is none.
+__device__ __forceinline__ float sum_of_odd(const uint16_t* __restrict__ v_cache,
+                                            const int32_t* __restrict__ table, const PageDims& d,
+                                            int seq, int k0, int k1, int64_t at) {
+  float sum = 0.0f;
+  for (int key = k0; key < k1; ++key) {
+    const int pid = page_at(table, d, seq, key >> d.page_log2);
+    if (pid < 0) continue;
+    const uint16_t v = v_cache[pid * d.page_stride + at + (key & ((1 << d.page_log2) - 1))];
+    if ((v & 0x7f80u) == 0x7f80u) sum += bf16_to_f32(v);
+  }
+  return sum;
+}
+
 template <int HD, bool F8>
 __global__ __launch_bounds__(256, decode_occupancy(HD)) void decode_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
@@ -558,7 +575,8 @@ __global__ __launch_bounds__(256, decode_occupancy(HD)) void decode_kernel(
   __syncthreads();
   const float vs = F8 && v_scale ? v_scale[kvh] : 1.0f;
   const int64_t part0 = (int64_t(item / d.kv_heads) * d.kv_heads + kvh) * group;
-  for (int i = t; i < group * HD; i += 256) {
+  // output i of the chunk; true where it is NaN under weights that are not.  again: where it was
+  auto output = [&](int i, auto again) {
     const int h = i / HD, c = i % HD;
     float M = mls[0][0][h];
 #pragma unroll
@@ -570,6 +588,13 @@ __global__ __launch_bounds__(256, decode_occupancy(HD)) void decode_kernel(
       const float e = __builtin_amdgcn_exp2f(mls[0][w][h] - ref);
       L = fmaf_(mls[1][w][h], e, L);
       O = fmaf_(os[(w * group + h) * OLD + c], e, O);
+    }
+    const bool odd = O != O && L == L;
+    if constexpr (again) {
+      if (!odd) return false;
+      const float sum = sum_of_odd(static_cast<const uint16_t*>(v_cache), table, d, seq, k0, k1,
+                                   (int64_t(kvh) * HD + c) << d.page_log2);
+      if (sum != 0.0f) O = sum;
     }
     if (whole) {
       float y = L == 0.0f ? 0.0f : O / L * vs;
@@ -584,7 +609,17 @@ __global__ __launch_bounds__(256, decode_occupancy(HD)) void decode_kernel(
         ml_part[(part0 + h) * 2 + 1] = L;
       }
     }
-  }
+    return odd;
+  };
+  bool odd = false;
+  for (int i = t; i < group * HD; i += 256) odd |= output(i, std::false_type{});
+  // An infinite value times a p whose low part is 0 or negative, or times a weight that has become
+  // 0, is NaN, where a positive weight leaves it infinite.  Such outputs are formed once more, from
+  // the values that are no numbers alone: nothing before has to look for them.  (e4m3 has no
+  // infinity.)
+  if constexpr (!F8)
+    if (odd)
+      for (int i = t; i < group * HD; i += 256) output(i, std::true_type{});
 }
 
 // Joins the chunks of DW dims of one (row, head) in a fixed order; rows without
@@ -648,7 +683,8 @@ __global__ __launch_bounds__(64 * NW) void decode_join_kernel(
     for (int i = 0; i < 8; ++i)
       if (c0 + NW * i < n) {  // uniform
         const float e = ws[c0 + NW * i];
-        for (int k = 0; k < DPL; ++k) O[k] = fmaf_(v[i][k], e, O[k]);
+        // (an infinite sum stays one, however small its chunk's weight)
+        for (int k = 0; k < DPL; ++k) O[k] = fmaf_(v[i][k], __builtin_isinf(v[i][k]) ? 1.0f : e, O[k]);
       }
     if (c0 + 8 * NW < n) {
 #pragma unroll
