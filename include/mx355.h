@@ -404,9 +404,9 @@ mx_status mx_argmax_bf16(const uint16_t* logits, int32_t rows, int32_t n, uint32
  * nothing exceeds -inf gives token 0, kept 0 and logprob -inf.  logprob
  * (optional): log of the token's share of the kept mass, fp32; kept
  * (optional): the number of tokens kept.  n <= 1048576.  workspace:
- * mx_sample_workspace_bytes(rows, n) bytes (0 bytes: NULL will do), 16-byte
- * aligned, one call at a time.  No reference counterpart (its server decodes
- * greedily). */
+ * mx_sample_workspace_bytes(rows, n) bytes, which do for any call of no more
+ * rows and tokens too, 16-byte aligned, one call at a time.  No reference
+ * counterpart (its server decodes greedily). */
 size_t mx_sample_workspace_bytes(int32_t rows, int32_t n);
 mx_status mx_sample_bf16(const uint16_t* logits, int64_t stride, int32_t rows, int32_t n,
                          const float* temperature, const int32_t* top_k, const float* top_p,

@@ -361,8 +361,7 @@ MX_ABI mx_status mx_sample_bf16(const uint16_t* logits, int64_t stride, int32_t 
   MX_CHECK(rows >= 0 && n > 0 && stride >= n, MX_EINVAL, "mx_sample_bf16: bad shape");
   MX_CHECK(n <= kSampleMaxVocab, MX_EUNSUPPORTED, "mx_sample_bf16: at most 1048576 logits a row");
   if (rows == 0) return MX_OK;
-  MX_CHECK(logits && uniform && tokens && (workspace || sample_workspace(rows, n) == 0), MX_EINVAL,
-           "mx_sample_bf16: null pointer");
+  MX_CHECK(logits && uniform && tokens && workspace, MX_EINVAL, "mx_sample_bf16: null pointer");
   MX_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, MX_EUNSUPPORTED,
            "mx_sample_bf16: the workspace must be 16-byte aligned");
   return finish(sample_bf16(logits, stride, rows, n, temperature, top_k, top_p, min_p, uniform,

@@ -550,9 +550,16 @@ int sample_batch(int rows, int parts) {
 
 }  // namespace
 
+// For any call of at most `rows` rows of at most n tokens.  Fewer rows are cut into more parts, so
+// that 32 rows may need more than 33: the most that any number of rows gives (parts of a longer row
+// are never fewer).
 size_t sample_workspace(int rows, int n) {
-  const int parts = sample_parts(rows, n);
-  return size_t(sample_batch(rows, parts)) * parts * (kHistBytes + 32 * 4 + 4);
+  int64_t most = 0;  // parts of a batch
+  for (int r = 1; r <= rows && r <= kBatchParts; ++r) {
+    const int64_t all = int64_t(r) * sample_parts(r, n);
+    most = all > most ? all : most;
+  }
+  return size_t(most < kBatchParts ? most : kBatchParts) * (kHistBytes + 32 * 4 + 4);
 }
 
 int sample_bf16(const uint16_t* logits, int64_t stride, int rows, int n, const float* temperature,
