@@ -563,8 +563,8 @@ mx_status mx_attn_paged_append(const uint16_t* qkv, int64_t qkv_stride, int32_t 
  * Lengths past the table are cut to it.  Matrix-core sums in fp32; the result
  * depends on the lengths of all rows (the keys' split follows them) to within
  * those sums' rounding, and is the same for the same inputs.  workspace:
- * mx_attn_paged_decode_workspace_bytes(rows, dims) bytes.  The paged form of
- * mx_attn_decode. */
+ * mx_attn_paged_decode_workspace_bytes(rows, dims) bytes, which do for fewer
+ * rows too.  The paged form of mx_attn_decode. */
 size_t mx_attn_paged_decode_workspace_bytes(int32_t rows, const mx_page_dims* dims);
 mx_status mx_attn_paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride,
                                int32_t rows, const int32_t* seqs, const int32_t* lens,
@@ -580,8 +580,9 @@ mx_status mx_attn_paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t q
  * positions up to its own.  Rows before position 0 see none and give zeros;
  * rows outside every sequence keep their out.  P is rounded to bf16 for the
  * second product.  Otherwise as mx_attn_paged_decode; workspace:
- * mx_attn_paged_prefill_workspace_bytes(rows, dims) bytes (0 bytes: NULL will
- * do).  The packed and paged form of mx_attn_decode's prefill form. */
+ * mx_attn_paged_prefill_workspace_bytes(rows, dims) bytes, which do for any call
+ * of no more rows with these dims too (0 bytes: NULL will do).  The packed and
+ * paged form of mx_attn_decode's prefill form. */
 size_t mx_attn_paged_prefill_workspace_bytes(int32_t rows, const mx_page_dims* dims);
 mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride,
                                 int32_t rows, const int32_t* starts, const int32_t* lens,

@@ -693,7 +693,7 @@ MX_ABI mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, i
            "mx_attn_paged_prefill: rows * heads must stay below 2^31");
   if (rows == 0) return MX_OK;
   MX_CHECK(q && starts && lens && table && k_cache && v_cache && out &&
-               (workspace || paged_prefill_workspace(rows, d) == 0),
+               (workspace || !paged_prefill_splits(rows, d)),
            MX_EINVAL, "mx_attn_paged_prefill: null pointer");
   MX_CHECK(aligned16(workspace) && aligned16(out), MX_EUNSUPPORTED,
            "mx_attn_paged_prefill: the workspace and out must be 16-byte aligned");

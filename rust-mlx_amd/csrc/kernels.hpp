@@ -235,6 +235,7 @@ int paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int
                  const float* v_scale, const PageDims& d, float scale, void* workspace,
                  uint16_t* out, hipStream_t s);
 size_t paged_prefill_workspace(int rows, const PageDims& d);
+bool paged_prefill_splits(int rows, const PageDims& d);  // does such a call use its workspace
 int paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int rows,
                   const int32_t* starts, const int32_t* lens, const int32_t* table,
                   const void* k_cache, const void* v_cache, const float* k_scale,

@@ -662,10 +662,23 @@ Layout layout_of(int rows, const PageDims& d) {
 
 }  // namespace
 
+// For any call of at most `rows` rows.  Fewer rows are split more, so that 300 rows may need more than
+// 512, and 2048 none: the most that any number of rows gives.
 size_t paged_prefill_workspace(int rows, const PageDims& d) {
-  const int s = layout_of(rows, d).splits;
-  return s == 1 ? 0 : size_t(rows) * d.heads * s * (d.head_dim + 2) * 4;
+  const int64_t group = d.heads / d.kv_heads;
+  int64_t most = 0;  // rows times splits
+  for (int64_t r = 1; r <= rows; ++r) {
+    // on to the last row that leaves the number of blocks as it is
+    if (r >= d.sequences) r = ((r * group / kPairs + 1) * kPairs - 1) / group;
+    r = r < rows ? r : rows;
+    const Layout l = layout_of(int(r), d);
+    if (l.splits == 1) break;  // and so for more rows
+    most = r * l.splits > most ? r * l.splits : most;
+  }
+  return size_t(most) * d.heads * (d.head_dim + 2) * 4;
 }
+
+bool paged_prefill_splits(int rows, const PageDims& d) { return layout_of(rows, d).splits > 1; }
 
 int paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int rows,
                   const int32_t* starts, const int32_t* lens, const int32_t* table,

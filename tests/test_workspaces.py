@@ -1,6 +1,8 @@
 """Workspace sizes of the operators for serving: a workspace for a program's largest
 batch serves every smaller one, so the sizes never fall as a call grows (no device:
 the entry points cannot see how large a workspace is)."""
+import ctypes as C
+
 import pytest
 
 
@@ -15,3 +17,27 @@ def test_sampling_workspace_never_falls_with_rows(mx, n):
 def test_sampling_workspace_never_falls_with_the_vocabulary(mx, rows):
     sizes = [mx.lib.mx_sample_workspace_bytes(rows, n) for n in range(1, 1 << 20, 511)]
     assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+
+
+def dims(mx, heads, kv, hd, page=64, sequences=1, width=196):
+    return mx.PageDimsC(heads, kv, hd, page, 1000, sequences, width, mx.MX_DT_BF16, 0, kv * page * hd)
+
+
+@pytest.mark.parametrize("sequences", [1, 5, 64, 300])
+@pytest.mark.parametrize("heads,kv,hd", [(16, 2, 256), (32, 8, 128), (28, 4, 128), (7, 1, 64), (5, 5, 128), (9, 9, 64)])
+@pytest.mark.parametrize("width", [3, 196, 4000])
+def test_prompt_workspace_never_falls_with_rows(mx, heads, kv, hd, sequences, width):
+    d = dims(mx, heads, kv, hd, sequences=sequences, width=width)
+    at = list(range(1, 1200)) + list(range(1200, 40000, 97))
+    sizes = [mx.lib.mx_attn_paged_prefill_workspace_bytes(r, C.byref(d)) for r in at]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:])), [r for r, a, b in zip(at[1:], sizes, sizes[1:]) if a > b][:9]
+    assert (sizes[0] > 0) == (width > 3)  # few rows that may see many keys are split
+    # bounded: a split call has fewer than 1024 workgroups, of 128 pairs each
+    assert mx.lib.mx_attn_paged_prefill_workspace_bytes(1 << 20, C.byref(d)) <= 1024 * 128 * (hd + 2) * 4
+
+
+@pytest.mark.parametrize("rows", [1, 8, 64, 130, 1000])
+def test_one_token_workspace_never_falls_with_rows(mx, rows):
+    d = dims(mx, 16, 2, 256)
+    f = mx.lib.mx_attn_paged_decode_workspace_bytes
+    assert f(rows, C.byref(d)) < f(rows + 1, C.byref(d))
