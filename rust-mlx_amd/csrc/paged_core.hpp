@@ -63,12 +63,14 @@ __device__ __forceinline__ void copy_to_lds(const char* src, uint32_t lds) {
                : "v"(src), "s"(lds)
                : "memory");
 }
-// The same from src + off, src the same for the wave.
+// The same from src + off, src the same for the wave.  src may come from a vector instruction (a read
+// of one lane), which has to lie five wait states before a memory instruction that uses it: the
+// compiler does not look into the block, so the block has them all.
 __device__ __forceinline__ void copy_to_lds(const char* src, uint32_t off, uint32_t lds) {
   const uint64_t at = reinterpret_cast<uint64_t>(src);
   const uint64_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(at))));
   const uint64_t hi = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(at >> 32))));
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1"
                :
                : "v"(off), "s"(hi << 32 | lo), "s"(lds)
                : "memory");
