@@ -58,8 +58,9 @@ __device__ __forceinline__ float gate_of(float x) {
 // the compiler takes every later LDS read for one of these bytes and waits for the copy at
 // once; here a tile's copy runs under the work on the tile before.
 __device__ __forceinline__ void copy_to_lds(const char* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-               :
+  uint32_t m0;  // an output, so that the compiler knows that it is written
+  asm volatile("s_mov_b32 %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               : "=&{m0}"(m0)
                : "v"(src), "s"(lds)
                : "memory");
 }
@@ -70,8 +71,9 @@ __device__ __forceinline__ void copy_to_lds(const char* src, uint32_t off, uint3
   const uint64_t at = reinterpret_cast<uint64_t>(src);
   const uint64_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(at))));
   const uint64_t hi = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(at >> 32))));
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1"
-               :
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, %3\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
+               : "=&{m0}"(m0)
                : "v"(off), "s"(hi << 32 | lo), "s"(lds)
                : "memory");
 }
