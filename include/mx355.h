@@ -578,7 +578,9 @@ mx_status mx_attn_paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t q
  * in the cache already (this call's and any cached prefix): row starts[s] + i
  * sits at position lens[s] - (starts[s + 1] - starts[s]) + i and sees the
  * positions up to its own.  Rows before position 0 see none and give zeros;
- * rows outside every sequence keep their out.  P is rounded to bf16 for the
+ * rows outside every sequence keep their out.  The table may hold sequences
+ * that have no rows in the call: they do not change how the others are shared
+ * out over the device, nor a bit of the result.  P is rounded to bf16 for the
  * second product.  Otherwise as mx_attn_paged_decode; workspace:
  * mx_attn_paged_prefill_workspace_bytes(rows, dims) bytes, which do for any call
  * of no more rows with these dims too (0 bytes: NULL will do).  The packed and

@@ -69,37 +69,89 @@ __device__ __forceinline__ void each(F&& f) {
   each_(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
 }
 
+// Rows of a sequence, which are the packed ones from `first` on, and its length, cut to the table's.
+struct Rows {
+  int first, count, len;
+};
+__device__ __forceinline__ Rows rows_of(const int32_t* __restrict__ starts,
+                                        const int32_t* __restrict__ lens, const PageDims& d,
+                                        int rows, int s) {
+  Rows r = {0, 0, 0};
+  if (s < d.sequences) {
+    r.first = min(max(starts[s], 0), rows);
+    r.count = max(min(starts[s + 1], rows) - r.first, 0);
+    const int64_t most = int64_t(d.table_width) << d.page_log2;
+    const int len = lens[s];
+    r.len = len < 0 ? 0 : (len > most ? int(most) : len);
+  }
+  return r;
+}
+__device__ __forceinline__ int blocks_of(const Rows& r, int group) {
+  return int((int64_t(r.count) * group + kPairs - 1) / kPairs);
+}
+
+// How many workgroups share the keys of a query block, with `blocks` of them: as many as bring the
+// launch to two workgroups a compute unit, each with at least four tiles of the longest possible
+// context; in eights with the kv heads where that is possible, for whole XCDs (512 rows on 12001
+// keys, two kv heads: 8 splits 126 us, 7 splits 138).  At most 64, never more with more blocks.
+__host__ __device__ __forceinline__ int splits_of(int64_t blocks, const PageDims& d) {
+  const int64_t all = blocks * d.kv_heads, room = (int64_t(d.table_width) << d.page_log2) / 256;
+  int s = all > 256 ? 1 : 512 / int(all < 1 ? 1 : all);
+  s = s > room ? int(room) : s;
+  s = s > 64 ? 64 : s < 1 ? 1 : s;
+  const int low = d.kv_heads & -d.kv_heads, step = low >= 8 ? 1 : 8 / low;  // powers of two
+  const int e = (s + step - 1) & -step;
+  return s > 1 && e < 2 * s && e <= room ? e : s;
+}
+// The fewest blocks that a call of so many rows is laid out for.
+__host__ __device__ __forceinline__ int64_t least_blocks(int rows, const PageDims& d) {
+  return (int64_t(rows) * (d.heads / d.kv_heads) + kPairs - 1) / kPairs;
+}
+
+// What follows from all sequences' rows, formed by every wave: the number of query blocks (sequences
+// without rows have none, however many the table has) and the splits; `r0`: the rows of the first 64
+// sequences, a lane each.
+struct Plan {
+  Rows r0;
+  int blocks, splits;
+};
+__device__ __forceinline__ Plan make_plan(const int32_t* __restrict__ starts,
+                                          const int32_t* __restrict__ lens, const PageDims& d,
+                                          int rows, int group) {
+  const int lane = threadIdx.x & 63;
+  Plan p;
+  p.r0 = rows_of(starts, lens, d, rows, lane);
+  int n = blocks_of(p.r0, group);
+#pragma unroll 4
+  for (int s = 64 + lane; s < d.sequences; s += 64)
+    n += blocks_of(rows_of(starts, lens, d, rows, s), group);
+  p.blocks = max(__builtin_amdgcn_readlane(wave_scan(n), 63), int(least_blocks(rows, d)));
+  p.splits = splits_of(p.blocks, d);
+  return p;
+}
+
 // The sequence and block of query block `want`; a sequence's blocks in reverse
 // order, those with the most keys first.
 struct Block {
   int seq, first, count, pair0, len;  // pair0: the block's first pair within the sequence
 };
-__device__ __forceinline__ bool find_block(const int32_t* __restrict__ starts,
+__device__ __forceinline__ bool find_block(const Plan& p, const int32_t* __restrict__ starts,
                                            const int32_t* __restrict__ lens, const PageDims& d,
                                            int rows, int group, int want, Block* out) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int s0 = 0; s0 < d.sequences; s0 += 64) {
-    const int s = s0 + lane;
-    int first = 0, count = 0, len = 0;
-    if (s < d.sequences) {
-      first = min(max(starts[s], 0), rows);
-      count = max(min(starts[s + 1], rows) - first, 0);
-      len = lens[s];
-    }
-    const int n = int((int64_t(count) * group + kPairs - 1) / kPairs);
-    const int sum = wave_scan(n);
+    const Rows r = s0 == 0 ? p.r0 : rows_of(starts, lens, d, rows, s0 + lane);
+    const int sum = wave_scan(blocks_of(r, group));
     const uint64_t past = __ballot(before + sum > want);
     if (past) {
       const int f = __builtin_ctzll(past);
       // uniform values, into scalar registers
       out->seq = __builtin_amdgcn_readfirstlane(s0 + f);
-      out->first = __builtin_amdgcn_readlane(first, f);
-      out->count = __builtin_amdgcn_readlane(count, f);
+      out->first = __builtin_amdgcn_readlane(r.first, f);
+      out->count = __builtin_amdgcn_readlane(r.count, f);
       out->pair0 = (before + __builtin_amdgcn_readlane(sum, f) - 1 - want) * kPairs;
-      const int64_t most = int64_t(d.table_width) << d.page_log2;
-      len = __builtin_amdgcn_readlane(len, f);
-      out->len = len < 0 ? 0 : (len > most ? int(most) : len);
+      out->len = __builtin_amdgcn_readlane(r.len, f);
       return true;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
@@ -116,19 +168,27 @@ struct Item {
 __host__ __device__ __forceinline__ bool by_xcd(int kv_heads, int splits) {
   return kv_heads * splits >= 8;
 }
+// Workgroups of a block: its pairs of kv head and split, in whole XCDs or, without enough of them,
+// every workgroup in turn.
+__host__ __device__ __forceinline__ int items_of(int kv_heads, int splits) {
+  const int pairs = kv_heads * splits;
+  return by_xcd(kv_heads, splits) ? 8 * ((pairs + 7) / 8) : pairs;
+}
 // Where all workgroups run at once, the second 256 beside the first on the same compute units,
 // those take the blocks from the last one on: a sequence's blocks have fewer and fewer keys, and
 // so a long one shares its unit with a short one (four prompts of up to 2047 rows on up to 3001,
 // e4m3: 144 us against 152).
-__device__ __forceinline__ Item item_of(int id, int grid, int kv_heads, int splits) {
-  const int pairs = kv_heads * splits;
-  const bool xcd = by_xcd(kv_heads, splits);
-  const int each = (pairs + 7) / 8;  // pairs of an XCD
+__device__ __forceinline__ Item item_of(int id, const Plan& p, int kv_heads) {
+  const int pairs = kv_heads * p.splits, a_block = items_of(kv_heads, p.splits);
+  const bool xcd = by_xcd(kv_heads, p.splits);
+  const int each = a_block / 8;  // pairs of an XCD
   const int j = id >> 3, pair = xcd ? (id & 7) + 8 * (j % each) : id % pairs;
   int block = xcd ? j / each : id / pairs;
-  if (grid > 256 && grid <= 512) {
-    const int a_block = xcd ? 8 * each : pairs, blocks = grid / a_block, first = 256 / a_block;
-    if (block >= first) block = blocks - 1 - (block - first);
+  if (block >= p.blocks) return Item{block, 0, p.splits};  // past the last block: none
+  const int64_t all = int64_t(p.blocks) * a_block;
+  if (all > 256 && all <= 512) {
+    const int first = 256 / a_block;
+    if (block >= first) block = p.blocks - 1 - (block - first);
   }
   return Item{block, pair % kv_heads, pair / kv_heads};  // split >= splits: none
 }
@@ -148,8 +208,8 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     const int32_t* __restrict__ starts, const int32_t* __restrict__ lens,
     const int32_t* __restrict__ table, const void* __restrict__ k_cache,
     const void* __restrict__ v_cache, const float* __restrict__ k_scale,
-    const float* __restrict__ v_scale, PageDims d, float scale, int splits,
-    float* __restrict__ o_part, float* __restrict__ ml_part, uint16_t* __restrict__ out) {
+    const float* __restrict__ v_scale, PageDims d, float scale, float* __restrict__ o_part,
+    float* __restrict__ ml_part, uint16_t* __restrict__ out) {
   constexpr int KT = tile_keys<HD>();
   constexpr int KS = HD / 16;          // steps of S^T
   constexpr int KB = KT / 32;          // 32-key operands of a tile
@@ -164,11 +224,13 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int col = lane & 31, h = lane >> 5;
   const int group = d.heads / d.kv_heads;
-  const Item it = item_of(blockIdx.x, gridDim.x, d.kv_heads, splits);
+  const Plan plan = make_plan(starts, lens, d, rows, group);
+  const int splits = plan.splits;
+  const Item it = item_of(blockIdx.x, plan, d.kv_heads);
   if (it.split >= splits) return;
   const int kvh = it.kvh, split = it.split;
   Block b;
-  if (!find_block(starts, lens, d, rows, group, it.block, &b)) return;  // uniform
+  if (!find_block(plan, starts, lens, d, rows, group, it.block, &b)) return;  // uniform
   const int prior = b.len - b.count;  // the first row's position (negative: rows without one)
   const int pairs = b.count * group;
   const int last_pair = min(b.pair0 + kPairs, pairs) - 1;
@@ -571,33 +633,44 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   }
 }
 
-// Joins the splits (at most 64) of some pairs of a query block in order, a wave a pair at a time.
+// Joins the splits (at most 64) of some pairs of a kv head in order, a wave a pair at a time.
 constexpr int kJoinPairs = 8;
 template <int HD>
 __global__ __launch_bounds__(256) void prefill_join_kernel(
     const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
     const int32_t* __restrict__ starts, const int32_t* __restrict__ lens,
-    const float* __restrict__ v_scale, PageDims d, int splits, const float* __restrict__ o_part,
+    const float* __restrict__ v_scale, PageDims d, const float* __restrict__ o_part,
     const float* __restrict__ ml_part, uint16_t* __restrict__ out) {
-  constexpr int KT = tile_keys<HD>(), DPL = HD / 64, JW = kPairs / kJoinPairs;
+  constexpr int KT = tile_keys<HD>(), DPL = HD / 64;
   typedef float vec __attribute__((ext_vector_type(DPL)));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = d.heads / d.kv_heads;
   const int kvh = blockIdx.x % d.kv_heads;
-  Block b;
-  if (!find_block(starts, lens, d, rows, group, int(blockIdx.x / d.kv_heads / JW), &b)) return;
-  const int prior = b.len - b.count, pairs = b.count * group;
-  const int last_pair = min(b.pair0 + kPairs, pairs) - 1;
-  const int kall = max(prior + last_pair / group + 1, 0);
-  const int tiles = (kall + KT - 1) / KT, per = (tiles + splits - 1) / splits;
-  if (per >= tiles) return;  // one split (or none) wrote the result
-  const int n = (tiles + per - 1) / per;
-  const int first = int(blockIdx.x / d.kv_heads) % JW * kJoinPairs;
-  for (int i = first + wave; i < first + kJoinPairs; i += 4) {
-    const int pair = b.pair0 + i;
-    if (pair > last_pair) return;
-    const int token = pair / group, head = kvh * group + pair - token * group;
-    const int64_t row = b.first + token, part = (row * d.heads + head) * splits;
+  const Plan plan = make_plan(starts, lens, d, rows, group);
+  const int splits = plan.splits;
+  const int all = rows * group, first = int(blockIdx.x / d.kv_heads) * kJoinPairs;  // below 2^31
+  for (int i = first + wave; i < min(first + kJoinPairs, all); i += 4) {
+    const int row = i / group, head = kvh * group + i - row * group;
+    // the row's sequence
+    int token = 0, pairs = 0, prior = 0;
+    for (int s0 = 0; s0 < d.sequences && pairs == 0; s0 += 64) {
+      const Rows r = s0 == 0 ? plan.r0 : rows_of(starts, lens, d, rows, s0 + lane);
+      const uint64_t here = __ballot(row >= r.first && row < r.first + r.count);
+      if (here) {
+        const int f = __builtin_ctzll(here);
+        token = row - __builtin_amdgcn_readlane(r.first, f);
+        pairs = __builtin_amdgcn_readlane(r.count, f) * group;
+        prior = __builtin_amdgcn_readlane(r.len - r.count, f);
+      }
+    }
+    if (pairs == 0) continue;  // a row outside every sequence
+    const int pair0 = (token * group + head - kvh * group) / kPairs * kPairs;  // of its block
+    const int last_pair = min(pair0 + kPairs, pairs) - 1;
+    const int kall = max(prior + last_pair / group + 1, 0);
+    const int tiles = (kall + KT - 1) / KT, per = (tiles + splits - 1) / splits;
+    if (per >= tiles) continue;  // one split (or none) wrote the result
+    const int n = (tiles + per - 1) / per;
+    const int64_t at = int64_t(row) * d.heads + head, part = at * splits;
     // eight splits' sums on their way while the weights form, a lane a split
     vec v[8];
 #pragma unroll
@@ -629,69 +702,46 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(
     for (int k = 0; k < DPL; ++k) {
       float y = L == 0.0f ? 0.0f : O[k] * inv;
       if (d.gated)
-        y *= gate_of(bf16_to_f32(qkv[row * qkv_stride + int64_t(head) * 2 * HD + HD + DPL * lane + k]));
-      out[(row * d.heads + head) * HD + DPL * lane + k] = f32_to_bf16(y);
+        y *= gate_of(bf16_to_f32(qkv[int64_t(row) * qkv_stride + int64_t(head) * 2 * HD + HD + DPL * lane + k]));
+      out[at * HD + DPL * lane + k] = f32_to_bf16(y);
     }
   }
-}
-
-// How a call is laid out: the most query blocks that any starts give, and the workgroups that
-// share a block's keys.
-struct Layout {
-  int64_t blocks;
-  int splits;
-};
-Layout layout_of(int rows, const PageDims& d) {
-  Layout l;
-  l.blocks = int64_t(rows) * (d.heads / d.kv_heads) / kPairs + (d.sequences < rows ? d.sequences : rows);
-  // as many splits as bring the launch to two workgroups a compute unit, each with at least four
-  // tiles of the longest possible context; in eights with the kv heads where that is possible,
-  // for whole XCDs (512 rows on 12001 keys, two kv heads: 8 splits 126 us, 7 splits 138)
-  const int64_t all = l.blocks * d.kv_heads, want = 512 / (all < 1 ? 1 : all);
-  const int64_t room = (int64_t(d.table_width) << d.page_log2) / 256;
-  int64_t s = want < room ? want : room;
-  s = s > 64 ? 64 : s < 1 ? 1 : s;
-  l.splits = int(s);
-  for (int64_t e = s; s > 1 && e < 2 * s && e <= room; ++e)
-    if (e * d.kv_heads % 8 == 0) {
-      l.splits = int(e);
-      break;
-    }
-  return l;
 }
 
 }  // namespace
 
 // For any call of at most `rows` rows.  Fewer rows are split more, so that 300 rows may need more than
-// 512, and 2048 none: the most that any number of rows gives.
+// 512, and 2048 none: the most that any number of rows gives, each with the fewest blocks.
 size_t paged_prefill_workspace(int rows, const PageDims& d) {
   const int64_t group = d.heads / d.kv_heads;
   int64_t most = 0;  // rows times splits
-  for (int64_t r = 1; r <= rows; ++r) {
-    // on to the last row that leaves the number of blocks as it is
-    if (r >= d.sequences) r = ((r * group / kPairs + 1) * kPairs - 1) / group;
-    r = r < rows ? r : rows;
-    const Layout l = layout_of(int(r), d);
-    if (l.splits == 1) break;  // and so for more rows
-    most = r * l.splits > most ? r * l.splits : most;
+  for (int64_t b = 1; (b - 1) * kPairs < rows * group; ++b) {
+    const int splits = splits_of(b, d);
+    if (splits == 1) break;  // and so for more blocks
+    const int64_t r = b * kPairs / group < rows ? b * kPairs / group : rows;  // the last row with b blocks
+    most = r * splits > most ? r * splits : most;
   }
   return size_t(most) * d.heads * (d.head_dim + 2) * 4;
 }
 
-bool paged_prefill_splits(int rows, const PageDims& d) { return layout_of(rows, d).splits > 1; }
+bool paged_prefill_splits(int rows, const PageDims& d) { return splits_of(least_blocks(rows, d), d) > 1; }
 
 int paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int rows,
                   const int32_t* starts, const int32_t* lens, const int32_t* table,
                   const void* k_cache, const void* v_cache, const float* k_scale,
                   const float* v_scale, const PageDims& d, float scale, void* workspace,
                   uint16_t* out, hipStream_t s) {
-  const Layout l = layout_of(rows, d);
-  const int splits = l.splits;
-  const int64_t blocks = l.blocks * d.kv_heads, joins = blocks * (kPairs / kJoinPairs);
-  // XCDs take whole pairs of kv head and split; without enough of them, every workgroup in turn
-  const int64_t grid = by_xcd(d.kv_heads, splits)
-                           ? l.blocks * 8 * ((int64_t(d.kv_heads) * splits + 7) / 8)
-                           : blocks * splits;
+  // Workgroups for any number of blocks that starts may give: the number itself is the kernel's to
+  // find.  Beyond 256 blocks of a kv head nothing is split, and more blocks have more workgroups.
+  const int64_t group = d.heads / d.kv_heads, least = least_blocks(rows, d);
+  const int64_t most = int64_t(rows) * group / kPairs + (d.sequences < rows ? d.sequences : rows);
+  int64_t grid = most * items_of(d.kv_heads, splits_of(most, d));
+  for (int64_t b = least; b < most && b * d.kv_heads <= 256; ++b) {
+    const int64_t n = b * items_of(d.kv_heads, splits_of(b, d));
+    grid = n > grid ? n : grid;
+  }
+  const int splits = splits_of(least, d);  // at most
+  const int64_t joins = (int64_t(rows) * group + kJoinPairs - 1) / kJoinPairs * d.kv_heads;
   if (grid > 0x7fffffff || joins > 0x7fffffff) return MX_EUNSUPPORTED;
   float* o_part = static_cast<float*>(workspace);
   float* ml_part = o_part + size_t(rows) * d.heads * splits * d.head_dim;
@@ -705,11 +755,11 @@ int paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, in
       return MX_EHIP;                                                                            \
     hipLaunchKernelGGL(fn, dim3(unsigned(grid)), dim3(64 * NW), lb, s, q, qkv, qkv_stride, rows, \
                        starts, lens, table, k_cache, v_cache, k_scale, v_scale, d, scale,        \
-                       splits, o_part, ml_part, out);                                            \
+                       o_part, ml_part, out);                                                    \
     if (hipGetLastError() != hipSuccess) return MX_EHIP;                                         \
     if (splits == 1) return MX_OK;                                                               \
     hipLaunchKernelGGL((prefill_join_kernel<HH>), dim3(unsigned(joins)), dim3(256), 0, s, qkv,   \
-                       qkv_stride, rows, starts, lens, vs, d, splits, o_part, ml_part, out);     \
+                       qkv_stride, rows, starts, lens, vs, d, o_part, ml_part, out);             \
     return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;                                    \
   }
   MX_PREFILL(64, false) MX_PREFILL(128, false) MX_PREFILL(256, false)

@@ -41,3 +41,11 @@ def test_one_token_workspace_never_falls_with_rows(mx, rows):
     d = dims(mx, 16, 2, 256)
     f = mx.lib.mx_attn_paged_decode_workspace_bytes
     assert f(rows, C.byref(d)) < f(rows + 1, C.byref(d))
+
+
+@pytest.mark.parametrize("rows", [1, 40, 512, 1500])
+def test_idle_rows_of_the_table_do_not_change_a_prompts_shape(mx, rows):
+    """How many workgroups share a prompt's keys follows from its rows, not from the sequences that have none."""
+    f = mx.lib.mx_attn_paged_prefill_workspace_bytes
+    sizes = {f(rows, C.byref(dims(mx, 16, 2, 256, sequences=s))) for s in (1, 2, 64, 300, 5000)}
+    assert len(sizes) == 1 and sizes.pop() > 0
