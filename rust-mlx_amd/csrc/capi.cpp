@@ -554,7 +554,7 @@ const char* check_pages(const mx_page_dims* dims, PageDims* d, int* code) {
   *code = MX_EUNSUPPORTED;
   if (dims->head_dim != 64 && dims->head_dim != 128 && dims->head_dim != 256)
     return "head_dim must be 64, 128 or 256";
-  if (dims->heads / dims->kv_heads > 16) return "at most 16 q heads per kv head";
+  if (dims->heads / dims->kv_heads > kPagedMaxGroup) return "at most 16 q heads per kv head";
   if (dims->heads > 65536) return "at most 65536 heads";
   int log2 = 4;
   while (log2 < 8 && (1 << log2) != dims->page_size) ++log2;

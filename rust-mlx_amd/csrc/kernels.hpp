@@ -209,6 +209,7 @@ int attn_combine_splits(const float* o_part, const float* ml_part, const uint16_
 constexpr int kAttnRows = 128;  // query rows per attention launch of a prefill chunk
 
 // ---- the paged cache (paged.hip, paged_prefill.hip) ----
+constexpr int kPagedMaxGroup = 16;  // q heads per kv head: columns of one matrix-core operand
 struct PageDims {
   int heads, kv_heads, head_dim;
   int page_log2;      // positions per page: 16 .. 256

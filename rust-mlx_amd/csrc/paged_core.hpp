@@ -20,7 +20,6 @@ typedef float floatx4_t __attribute__((ext_vector_type(4)));
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxGroup = 16;  // q heads per kv head
 
 __device__ __forceinline__ float neg_inf() { return u2f(0xff800000u); }
 

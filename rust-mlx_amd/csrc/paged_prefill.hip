@@ -16,8 +16,10 @@
 // leaves its lane, and the pair's maximum, sum and rescaling are one value a
 // lane.  The cache holds V transposed, so both operands are 16-byte reads.
 //
-// P is rounded to bf16 for the product: its relative error of 2^-9 is at most
-// that of the output's own rounding, and the sum that divides takes P before it.
+// P is rounded to bf16 for the product, each p by at most 2^-8 of itself, as the
+// output is; the sum that divides takes P before it.  A second part of P, as
+// attention of one token has it, would make the second product's work twice as
+// much where the matrix units are the bound.
 //
 // Tiles are copied to LDS one ahead (e4m3 through registers, where it is
 // widened once for all waves).  16-byte pieces of a row are exchanged by the
