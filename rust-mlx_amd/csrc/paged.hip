@@ -259,9 +259,9 @@ __global__ __launch_bounds__(kQkThreads) void append_kernel(
 //
 // The memory bounds it where there are many keys: 64 rows of 32 q / 8 kv heads of 128
 // on up to 16384 take 386 us and 6 to join (5.5 TB/s), 40 e4m3 rows of 28 / 4 heads on
-// up to 12001 48 and 5.  Of one row of 60001 keys (16 / 2 heads of 256, 30 us and 5), 2.7
+// up to 12001 48 and 5.  Of one row of 60001 keys (16 / 2 heads of 256, 30 us and 6), 2.7
 // us go to the plan, the first keys are there after 6.4, and 2.5 join the waves; 8 rows of
-// up to 4000 (14 and 4) are little else.
+// up to 4000 (14 and 5) are little else.
 constexpr int kDecodeMaxChunks = 2048 + 1;  // of one row: twice decode_target and the rounding
 template <bool F8>
 struct DecodeTile {

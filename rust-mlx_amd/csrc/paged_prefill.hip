@@ -30,9 +30,9 @@
 // joins their partials.
 //
 // The matrix cores and the vector ALUs bound it together, under a falling clock:
-// 8192 tokens of 32 q / 8 kv heads of 128 take 555 to 580 us (950 to 990 TFLOP/s).
-// 512 rows of 16 / 2 heads of 256 on 12001 keys take 124 us, 17 of them to join
-// eight splits; there the registers bound it, see R and kHalves.
+// 8192 tokens of 32 q / 8 kv heads of 128 take 560 to 592 us from card to card (930 to
+// 980 TFLOP/s).  512 rows of 16 / 2 heads of 256 on 12001 keys take 123 to 130 us, 17
+// of them to join eight splits; there the registers bound it, see R and kHalves.
 #include <type_traits>
 #include <utility>
 

@@ -25,7 +25,7 @@
 // read again for the id.
 //
 // The latency of few dependent steps bounds it: one row of 151936 takes 6 us to count
-// and 13 to choose, 64 rows 9 and 15 (their logits alone would take 4).  One workgroup
+// and 14 to choose, 64 rows 10 and 16 (their logits alone would take 4).  One workgroup
 // a row that counts, chooses and reads the row three times takes 76 us for 1 to 256
 // rows: each read is 19 dependent trips of one compute unit.
 #include "common.hpp"
