@@ -124,9 +124,23 @@ __device__ __forceinline__ Plan make_plan(const int32_t* __restrict__ starts,
   Plan p;
   p.r0 = rows_of(starts, lens, d, rows, lane);
   int n = blocks_of(p.r0, group);
-#pragma unroll 4
-  for (int s = 64 + lane; s < d.sequences; s += 64)
-    n += blocks_of(rows_of(starts, lens, d, rows, s), group);
+  constexpr int AHEAD = 8;  // loads on their way; past the last sequence there are no rows
+  const int all = min(starts[d.sequences], rows);
+  int done = __builtin_amdgcn_readlane(p.r0.first + p.r0.count, 63);  // rows of the sequences so far
+  for (int s0 = 64; s0 < d.sequences && done < all; s0 += 64 * AHEAD) {
+    int at[AHEAD], to[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      at[i] = starts[min(s0 + 64 * i + lane, d.sequences)];
+      to[i] = starts[min(s0 + 64 * i + lane + 1, d.sequences)];
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int first = min(max(at[i], 0), rows);
+      n += blocks_of({first, max(min(to[i], rows) - first, 0), 0}, group);
+    }
+    done = __builtin_amdgcn_readlane(to[AHEAD - 1], 63);
+  }
   p.blocks = max(__builtin_amdgcn_readlane(wave_scan(n), 63), int(least_blocks(rows, d)));
   p.splits = splits_of(p.blocks, d);
   return p;
