@@ -345,13 +345,17 @@ def _own_prompt(s):
 
 def _own_controls(s):
     mx, c = _package(), s["case"]
-    words = 0 if s["masks"] is None else s["masks"].shape[1]
-    states = 0 if s["masks"] is None else s["masks"].shape[0]
-    mx.check(mx.lib.mx_logits_control_bf16(
-        s["logits"].data_ptr(), c["vocab"], c["rows"], c["vocab"], s["tokens"].data_ptr(), s["tokens"].shape[1],
-        s["prompt_lens"].data_ptr(), s["lens"].data_ptr(), s["repetition"].data_ptr(), s["frequency"].data_ptr(),
-        s["presence"].data_ptr(), _p(s["bias_starts"]), _p(s["bias_tokens"]), _p(s["bias_values"]), _p(s["masks"]), words,
-        states, _p(s["mask_rows"]), s["out"].data_ptr(), c["vocab"], _stream()))
+    if "controls" not in s:  # the description that a program keeps
+        states, words = (0, 0) if s["masks"] is None else s["masks"].shape
+        s["controls"] = mx.LogitsControlsC(
+            tokens=s["tokens"].data_ptr(), tokens_stride=s["tokens"].shape[1], prompt_lens=s["prompt_lens"].data_ptr(),
+            lens=s["lens"].data_ptr(), sequences=c["rows"], repetition=s["repetition"].data_ptr(),
+            frequency=s["frequency"].data_ptr(), presence=s["presence"].data_ptr(), bias_starts=_p(s["bias_starts"]),
+            bias_tokens=_p(s["bias_tokens"]), bias_values=_p(s["bias_values"]),
+            bias_count=0 if s["bias_tokens"] is None else s["bias_tokens"].shape[0], masks=_p(s["masks"]),
+            mask_rows=_p(s["mask_rows"]), mask_stride=words, mask_states=states)
+    mx.check(mx.lib.mx_logits_control_bf16(s["logits"].data_ptr(), c["vocab"], c["rows"], c["vocab"],
+                                           ctypes.byref(s["controls"]), s["out"].data_ptr(), c["vocab"], _stream()))
     return {"logits": s["out"]}
 
 
