@@ -243,6 +243,24 @@ int paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, in
                   const float* v_scale, const PageDims& d, float scale, void* workspace,
                   uint16_t* out, hipStream_t s);
 
+// ---- the latent cache (latent.hip, latent_decode.hip, latent_prefill.hip) ----
+struct LatentDims {
+  int heads;
+  int nope_dim, v_dim;        // of a head, as formed from the latents
+  int latent_dim, rope_dim;   // of a position
+  int page_log2, pages, sequences, table_width;  // as in PageDims
+  bool f8;
+  int64_t page_stride;
+  static constexpr int kv_heads = 1;  // all heads read the same positions
+};
+// What attention with keys and values of every head knows of them: each head is a kv head.
+struct LatentPromptDims {
+  int heads, kv_heads;
+  int sequences;
+  int kv_rows;  // packed keys of all sequences
+  static constexpr bool gated = false;
+};
+
 // ---- MoE ----
 constexpr int kMaxRoutes = 8 * 16 + 1;
 // Work list of one MoE step: distinct routed experts (first appearance order)

@@ -29,27 +29,6 @@ using namespace pg;
 constexpr int kQkThreads = 256;
 constexpr int kVRows = 32;
 
-// sin and cos of 2 pi t
-__device__ __forceinline__ void sincos_turn(double t, float* sn, float* cs) {
-  const double f = __builtin_amdgcn_fract(t);           // [0, 1)
-  const double quarter = __builtin_rint(f * 4.0);       // 0 .. 4
-  const float r = float((f - quarter * 0.25) * 6.283185307179586477);  // |r| <= pi / 4
-  const float z = r * r;
-  float s = fmaf_(z, 2.7557319e-6f, -1.9841270e-4f);    // 1/9!, 1/7!
-  s = fmaf_(z, s, 8.3333333e-3f);                       // 1/5!
-  s = fmaf_(z, s, -1.6666667e-1f);                      // 1/3!
-  s = fmaf_(r * z, s, r);
-  float c = fmaf_(z, -2.7557319e-7f, 2.4801587e-5f);    // 1/10!, 1/8!
-  c = fmaf_(z, c, -1.3888889e-3f);                      // 1/6!
-  c = fmaf_(z, c, 4.1666667e-2f);                       // 1/4!
-  c = fmaf_(z, c, -0.5f);
-  c = fmaf_(z, c, 1.0f);
-  const int n = int(quarter) & 3;
-  const float a = n & 1 ? c : s, b = n & 1 ? s : c;
-  *sn = n & 2 ? -a : a;
-  *cs = (n == 1 || n == 2) ? -b : b;
-}
-
 template <int HD, bool F8>
 __global__ __launch_bounds__(kQkThreads) void append_kernel(
     const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
@@ -262,7 +241,6 @@ __global__ __launch_bounds__(kQkThreads) void append_kernel(
 // up to 12001 48 and 5.  Of one row of 60001 keys (16 / 2 heads of 256, 30 us and 6), 2.7
 // us go to the plan, the first keys are there after 6.4, and 2.5 join the waves; 8 rows of
 // up to 4000 (14 and 5) are little else.
-constexpr int kDecodeMaxChunks = 2048 + 1;  // of one row: twice decode_target and the rounding
 template <bool F8>
 struct DecodeTile {
   static constexpr int kKeys = F8 ? 64 : 32;  // a lane's 16 bytes of V: 16 or 8 keys
@@ -272,50 +250,6 @@ struct DecodeTile {
 constexpr int decode_occupancy(int head_dim) { return head_dim == 256 ? 2 : head_dim == 128 ? 3 : 4; }
 // Chunks wanted: as many as run at once.
 int decode_target(const PageDims& d) { return 256 * decode_occupancy(d.head_dim); }
-
-// The length of a row's context, or -1 for a padding row.
-__device__ __forceinline__ int row_len(const int32_t* __restrict__ seqs,
-                                       const int32_t* __restrict__ lens, const PageDims& d, int r,
-                                       int rows) {
-  if (r >= rows) return -1;
-  const int seq = seqs ? seqs[r] : r;
-  const int len = lens[r];
-  if (unsigned(seq) >= unsigned(d.sequences)) return -1;
-  const int most = int(min(int64_t(d.table_width) << d.page_log2, int64_t(0x7fffffff)));
-  return len < 0 ? 0 : min(len, most);
-}
-
-__device__ __forceinline__ int units_of(int len, int unit) {
-  return len > 0 ? (len + unit - 1) / unit : 0;
-}
-
-// The plan, formed by every wave: the most units of a chunk (a row's chunks are even), the
-// fewest that give at most `target` chunks (or two rounds of them, where they are long) where
-// some number up to twice the even share does; `len0`: the lengths of the first 64 rows, a lane each.
-struct Plan {
-  int chunk_units, len0;
-};
-__device__ __forceinline__ Plan make_plan(const int32_t* seqs, const int32_t* lens,
-                                          const PageDims& d, int rows, int unit, int target) {
-  const int lane = threadIdx.x & 63;
-  Plan p;
-  p.len0 = row_len(seqs, lens, d, lane, rows);
-  auto sum = [&](auto&& of) {
-    int64_t total = __builtin_amdgcn_readlane(wave_scan(of(units_of(p.len0, unit))), 63);
-    for (int r = 64; r < rows; r += 64)
-      total += __builtin_amdgcn_readlane(
-          wave_scan(of(units_of(row_len(seqs, lens, d, r + lane, rows), unit))), 63);
-    return total * d.kv_heads;
-  };
-  const int64_t total = sum([](int u) { return u; });
-  if (total >= 16 * int64_t(target)) target *= 2;  // long chunks: a second round evens out the units' speeds
-  const int64_t share = (total + target - 1) / target;
-  const int c0 = share < 1 ? 1 : int(share), step = (c0 + 7) / 8;
-  int c = c0;
-  while (c < 2 * c0 && sum([&](int u) { return (u + c - 1) / c; }) > target) c += step;
-  p.chunk_units = c;
-  return p;
-}
 
 // The sum of the infinite and NaN values among positions k0 .. k1 - 1 of one dim (at: from a page's
 // start to that dim's first position), 0 where there is none.
@@ -360,28 +294,12 @@ __global__ __launch_bounds__(256, decode_occupancy(HD)) void decode_kernel(
   // this workgroup's (row, chunk, kv head)
   const int item = blockIdx.x, kvh = item % d.kv_heads;
   const int want = item / d.kv_heads;
-  const Plan plan = make_plan(seqs, lens, d, rows, kUnit, target);
-  const int cu = plan.chunk_units;
-  int row = -1, chunk = 0, chunks = 0, before = 0, len = 0;
-  for (int r = 0; r < rows; r += 64) {
-    const int l = r == 0 ? plan.len0 : row_len(seqs, lens, d, r + lane, rows);
-    const int n = (units_of(l, kUnit) + cu - 1) / cu;
-    const int sum = wave_scan(n);
-    const uint64_t past = __ballot(before + sum > want);
-    if (past) {
-      const int f = __builtin_ctzll(past);
-      row = r + f;
-      len = __builtin_amdgcn_readlane(l, f);
-      chunks = __builtin_amdgcn_readlane(n, f);
-      before += __builtin_amdgcn_readlane(sum, f) - chunks;
-      chunk = want - before;
-      if (chunk == 0 && kvh == 0 && t == 0)  // for the launch that joins
-        row_chunks[row] = make_int2(before, chunks);
-      break;
-    }
-    before += __builtin_amdgcn_readlane(sum, 63);
-  }
+  const KeyPlan plan = key_plan(seqs, lens, d, rows, kUnit, target);
+  const Chunk ch = find_chunk(plan, seqs, lens, d, rows, kUnit, want);
+  const int row = ch.row, chunk = ch.index, chunks = ch.chunks, before = ch.before, len = ch.len;
   if (row < 0) return;  // uniform: past the last chunk
+  if (chunk == 0 && kvh == 0 && t == 0)  // for the launch that joins
+    row_chunks[row] = make_int2(before, chunks);
   const int seq = seqs ? seqs[row] : row;
   // units / chunks each, the first ones one more
   const int units = units_of(len, kUnit), few = units / chunks, more_units = units % chunks;
@@ -622,94 +540,6 @@ __global__ __launch_bounds__(256, decode_occupancy(HD)) void decode_kernel(
       for (int i = t; i < group * HD; i += 256) output(i, std::true_type{});
 }
 
-// Joins the chunks of DW dims of one (row, head) in a fixed order; rows without
-// keys become 0, rows of one chunk are done already.  Each wave takes every NW-th
-// chunk, eight at a time, whose sums are on their way while the weights form.
-template <int HD, int DW, int NW>
-__global__ __launch_bounds__(64 * NW) void decode_join_kernel(
-    const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
-    const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
-    const float* __restrict__ v_scale, PageDims d, const int2* __restrict__ row_chunks,
-    const float* __restrict__ o_part, const float* __restrict__ ml_part,
-    uint16_t* __restrict__ out) {
-  constexpr int DB = HD / DW, DPL = DW / 64;
-  typedef float vec __attribute__((ext_vector_type(DPL)));
-  __shared__ float ws[kDecodeMaxChunks];
-  __shared__ float red[2][NW];
-  __shared__ vec os[NW][64];
-  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
-  const int dim = DW * (blockIdx.x % DB) + DPL * lane;
-  const int head = blockIdx.x / DB % d.heads, row = blockIdx.x / DB / d.heads;
-  const int group = d.heads / d.kv_heads, kvh = head / group;
-  const int len = row_len(seqs, lens, d, row, rows);
-  const int2 rc = row_chunks[row];  // meaningful where there are keys
-  if (len < 0) return;
-  uint16_t* dst = out + (int64_t(row) * d.heads + head) * HD + dim;
-  if (len == 0) {
-    if (wave == 0)
-      for (int i = 0; i < DPL; ++i) dst[i] = 0;
-    return;
-  }
-  const int n = rc.y;  // 2 .. kDecodeMaxChunks
-  if (n <= 1) return;
-  const int64_t part0 = int64_t(rc.x) * d.heads + head;  // chunk c's partial: c heads further on
-  auto part_of = [&](int c) {
-    return *reinterpret_cast<const vec*>(o_part + (part0 + int64_t(c) * d.heads) * HD + dim);
-  };
-  vec v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = part_of(min(wave + NW * i, n - 1));
-  float M = neg_inf();
-  for (int c = t; c < n; c += 64 * NW) M = fmaxf(M, ml_part[(part0 + int64_t(c) * d.heads) * 2]);
-  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  if (lane == 0) red[0][wave] = M;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < NW; ++w) M = fmaxf(M, red[0][w]);
-  const float ref = M == neg_inf() ? 0.0f : M;
-  float L = 0.0f;
-  for (int c = t; c < n; c += 64 * NW) {
-    const float2 ml = *reinterpret_cast<const float2*>(ml_part + (part0 + int64_t(c) * d.heads) * 2);
-    const float e = __builtin_amdgcn_exp2f(ml.x - ref);
-    ws[c] = e;
-    L = fmaf_(ml.y, e, L);
-  }
-  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
-  if (lane == 0) red[1][wave] = L;
-  __syncthreads();
-  vec O = 0.0f;
-  for (int c0 = wave; c0 < n; c0 += 8 * NW) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c0 + NW * i < n) {  // uniform
-        const float e = ws[c0 + NW * i];
-        // (an infinite sum stays one, however small its chunk's weight)
-        for (int k = 0; k < DPL; ++k) O[k] = fmaf_(v[i][k], __builtin_isinf(v[i][k]) ? 1.0f : e, O[k]);
-      }
-    if (c0 + 8 * NW < n) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = part_of(min(c0 + NW * (8 + i), n - 1));
-    }
-  }
-  os[wave][lane] = O;
-  __syncthreads();
-  if (wave != 0) return;
-  L = red[1][0];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) {
-    L += red[1][w];
-    O += os[w][lane];
-  }
-  const float inv = (L == 0.0f ? 0.0f : 1.0f / L) * (v_scale ? v_scale[kvh] : 1.0f);
-  const uint16_t* gp = qkv + int64_t(row) * qkv_stride + int64_t(head) * 2 * HD + HD + dim;
-#pragma unroll
-  for (int k = 0; k < DPL; ++k) {
-    float y = L == 0.0f ? 0.0f : O[k] * inv;
-    if (d.gated) y *= gate_of(bf16_to_f32(gp[k]));
-    dst[k] = f32_to_bf16(y);
-  }
-}
-
 int decode_unit(const PageDims& d) {
   return d.f8 ? DecodeTile<true>::kUnit : DecodeTile<false>::kUnit;
 }
@@ -773,7 +603,7 @@ int paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int
   int2* row_chunks = reinterpret_cast<int2*>(ml_part + items * group * 2);
   const int target = decode_target(d);
 #define MX_JOIN(HH, DW, NW)                                                                      \
-  hipLaunchKernelGGL((decode_join_kernel<HH, DW, NW>), dim3(unsigned(joins * (HH / DW))),        \
+  hipLaunchKernelGGL((decode_join_kernel<HH, DW, NW, PageDims>), dim3(unsigned(joins * (HH / DW))),        \
                      dim3(64 * NW), 0, s, qkv, qkv_stride, rows, seqs, lens,                     \
                      d.f8 ? v_scale : nullptr, d, row_chunks, o_part, ml_part, out)
 #define MX_DECODE(HH, FF)                                                                        \
