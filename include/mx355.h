@@ -387,6 +387,51 @@ mx_status mx_head_argmax_mfma(const mx_qweight* w, const uint16_t* x, int32_t m,
 mx_status mx_argmax_bf16(const uint16_t* logits, int32_t rows, int32_t n, uint32_t* tokens,
                          void* stream);
 
+/* mx_logits_control_bf16: what is done to bf16 logits [rows, n] (rows `stride`
+ * elements apart, any alignment) before a token is chosen.  Of token j, which
+ * occurs c times in the output of the row's sequence:
+ *   x = logits[r][j]
+ *   x = x < 0 ? x * repetition[r] : x / repetition[r]   where j occurs in its
+ *                                                       prompt or its output
+ *   x -= frequency[r] * c;  x -= presence[r] where c > 0
+ *   x += the row's bias of j;  x = -inf where the row's mask does not allow j
+ * in fp32, rounded once, to out (rows out_stride apart; out = logits with one
+ * stride works in place and touches only what changes; otherwise they must not
+ * overlap).  History: row r's tokens are the first lens[s] of
+ * tokens[s * tokens_stride ..], s = seqs[r] (seqs NULL: r), the first
+ * prompt_lens[s] of them the prompt; lengths are cut to the stride, tokens
+ * outside [0, n) count for nothing, and a row whose s is not in [0, sequences)
+ * is padding and keeps its out.  tokens NULL: no history, no padding.
+ * repetition NULL, <= 0 or not finite = off; frequency, presence NULL or not
+ * finite = off.  Biases: entries bias_starts[r] .. bias_starts[r + 1] - 1 (cut
+ * to bias_count) of bias_tokens and bias_values; of a token named twice the last
+ * entry counts.  Masks: bit j % 32 of word j / 32 of row mask_rows[r] (NULL: r)
+ * of masks, mask_stride words apart; a row outside [0, mask_states) has none.
+ * All arrays are on the device; a NULL one's part is left out.  The result does
+ * not depend on any order of execution.  No reference counterpart. */
+typedef struct mx_logits_controls {
+  const int32_t* tokens;       /* [sequences][tokens_stride] */
+  int64_t tokens_stride;
+  const int32_t* prompt_lens;  /* [sequences], NULL: all output */
+  const int32_t* lens;         /* [sequences] */
+  const int32_t* seqs;         /* [rows] */
+  const float* repetition;     /* [rows] */
+  const float* frequency;      /* [rows] */
+  const float* presence;       /* [rows] */
+  const int32_t* bias_starts;  /* [rows + 1] */
+  const int32_t* bias_tokens;  /* [bias_count] */
+  const float* bias_values;    /* [bias_count] */
+  const uint32_t* masks;       /* [mask_states][mask_stride] */
+  const int32_t* mask_rows;    /* [rows] */
+  int64_t mask_stride;
+  int32_t sequences;
+  int32_t bias_count;
+  int32_t mask_states;
+} mx_logits_controls;
+mx_status mx_logits_control_bf16(const uint16_t* logits, int64_t stride, int32_t rows, int32_t n,
+                                 const mx_logits_controls* controls, uint16_t* out,
+                                 int64_t out_stride, void* stream);
+
 /* mx_sample_bf16: tokens[r] drawn from bf16 logits [rows, n] (rows `stride`
  * elements apart, any alignment) with a given uniform number, beside
  * mx_argmax_bf16's greedy choice.  Tokens are ordered by logit (largest first,
@@ -593,6 +638,116 @@ mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t 
                                 const mx_page_dims* dims, float scale, void* workspace,
                                 uint16_t* out, void* stream);
 
+/* ---- the latent cache ---------------------------------------------------------
+ * A cache of one vector a position for all heads: a latent of latent_dim values,
+ * from which every head's key (nope_dim) and value (v_dim) follow by products,
+ * and a rotary key of rope_dim that the heads share.  What writes it, what reads
+ * it back, attention of single tokens over the latents themselves, and of
+ * prompts over keys and values formed from them.  The products (of q with the
+ * keys' weights, of the result with the values', of latents with both) are the
+ * caller's projections.  No reference counterpart.
+ *
+ * Layout, elements of dtype, page_stride elements from page to page:
+ *   cache   [pages][page_size][latent_dim + rope_dim]
+ *   scales  fp32 [pages][page_size], of MX_DT_F8E4M3 (ignored for MX_DT_BF16):
+ *           the value is the stored number times its position's scale
+ * Pages, tables, sequences, padding rows and workspaces are those of the paged
+ * cache.  What a row does not see may hold anything.  A position with an
+ * infinite or NaN value makes what attention gives the rows that see it NaN, in
+ * the dims of that value at least.
+ *
+ * 1..128 heads; latent_dim 256 or 512; rope_dim 64; nope_dim and v_dim 64 or 128
+ * and the same; page_size 16, 32, 64, 128 or 256; at most 2^30 positions a
+ * sequence (MX_EUNSUPPORTED otherwise).  All rows (strides % 8 == 0), norms,
+ * outputs, workspaces and the cache are 16-byte aligned.  The pointers and the
+ * stream belong to the current device. */
+typedef struct mx_latent_dims {
+  int32_t heads;
+  int32_t nope_dim;     /* of a head's key beside the rotary part */
+  int32_t v_dim;        /* of a head's value */
+  int32_t latent_dim;
+  int32_t rope_dim;
+  int32_t page_size;
+  int32_t pages;
+  int32_t sequences;    /* rows of the page table */
+  int32_t table_width;  /* entries of a row of the page table */
+  int32_t dtype;        /* MX_DT_BF16 or MX_DT_F8E4M3 */
+  int64_t page_stride;  /* >= page_size * (latent_dim + rope_dim), a multiple of 16 */
+} mx_latent_dims;
+/* mx_attn_latent_append: takes projected rows x [rows][latent_dim + rope_dim]
+ * (x_stride elements apart) into the cache and the rotary parts of q
+ * [rows][heads][nope_dim + rope_dim] (q_stride apart) to q_rope bf16 [rows,
+ * heads, rope_dim]: the latent RMS-normalised (x rsqrt(mean x^2 + eps)
+ * (norm + 1); a NULL norm leaves it as it is), the rotary key and the queries
+ * rotated, in fp32 with one rounding.  Row r is position pos[r] of sequence
+ * seqs[r] (seqs NULL: sequence r); rope as mx_attn_paged_append's, with
+ * rotary_dim = rope_dim.  An e4m3 cache takes round(value / scale) with the scale
+ * of the position max(its largest value's size, 2^-100) / 448, which goes to
+ * scales (a position with an infinite value reads as NaN throughout).  A row
+ * whose sequence is not in [0, sequences) is padding: nothing of it is written; a
+ * position outside the table writes q_rope only.  Rows must not name the same
+ * position twice.  The latent form of mx_attn_paged_append. */
+mx_status mx_attn_latent_append(const uint16_t* x, int64_t x_stride, const uint16_t* q,
+                                int64_t q_stride, int32_t rows, const int32_t* seqs,
+                                const int32_t* pos, const int32_t* rope_pos,
+                                const mx_rope_axes* rope, const uint16_t* norm, float eps,
+                                const int32_t* table, const mx_latent_dims* dims, uint16_t* q_rope,
+                                void* cache, float* scales, void* stream);
+/* mx_attn_latent_read: positions back from the cache, as bf16 (of e4m3: times
+ * the scale, in fp32 with one rounding).  Rows starts[s] .. starts[s + 1] - 1 of
+ * latent [rows][latent_dim] and rope [rows][rope_dim] (their strides apart;
+ * starts: int32 [sequences + 1], not decreasing, up to `rows`) are the positions
+ * first[s] (first NULL: 0), first[s] + 1, .. of sequence s; positions without a
+ * page give zeros, rows outside every sequence stay as they are.  What a prompt
+ * on a cached prefix forms that prefix's keys and values from. */
+mx_status mx_attn_latent_read(const void* cache, const float* scales, int32_t rows,
+                              const int32_t* starts, const int32_t* first, const int32_t* table,
+                              const mx_latent_dims* dims, uint16_t* latent, int64_t latent_stride,
+                              uint16_t* rope, int64_t rope_stride, void* stream);
+/* mx_attn_latent_decode: attention of one token a row over positions
+ * 0 .. lens[r] - 1 of its sequence (seqs[r], or r), the latents being both keys
+ * and values (absorbed: q_latent [rows, heads, latent_dim] is q's nope part times
+ * the head's key weights, and the head's value weights are still to be applied to
+ * out [rows, heads, latent_dim]); q_rope [rows, heads, rope_dim] as
+ * mx_attn_latent_append gives it:
+ *   out[r, h] = bf16(softmax((q_latent c^T + q_rope k^T) scale) c)
+ * with scale 0 meaning 1 / sqrt(nope_dim + rope_dim).  P is rounded to bf16 for
+ * the second product.  Rows without positions, padding rows, lengths past the
+ * table, the dependence on the other rows' lengths and the workspace as
+ * mx_attn_paged_decode's; workspace: mx_attn_latent_decode_workspace_bytes(rows,
+ * dims) bytes, which do for fewer rows too.  A sequence's several new tokens (as a
+ * draft's) are rows of that sequence with the lengths of their own positions. */
+size_t mx_attn_latent_decode_workspace_bytes(int32_t rows, const mx_latent_dims* dims);
+mx_status mx_attn_latent_decode(const uint16_t* q_latent, const uint16_t* q_rope, int32_t rows,
+                                const int32_t* seqs, const int32_t* lens, const int32_t* table,
+                                const void* cache, const float* scales, const mx_latent_dims* dims,
+                                float scale, void* workspace, uint16_t* out, void* stream);
+/* mx_attn_latent_prefill: causal attention of packed sequences with every
+ * head's keys and values formed from the latents (expanded).  Rows starts[s] ..
+ * starts[s + 1] - 1 of q [rows][heads][nope_dim + rope_dim] (q_stride apart; its
+ * rotary part is not read, q_rope [rows, heads, rope_dim] is, as
+ * mx_attn_latent_append gives it) are the last positions of sequence s, whose
+ * positions are the rows kv_starts[s] .. kv_starts[s + 1] - 1 of kv
+ * [kv_rows][heads][nope_dim key | v_dim value] (kv_stride apart, below 2^29) and
+ * k_rope [kv_rows][rope_dim] (rope_stride apart; rotated, as mx_attn_latent_read
+ * gives it); starts and kv_starts: int32 [sequences + 1], not decreasing, up to
+ * rows and kv_rows.  Of dims the head's and the number of sequences count.  Row i
+ * of n over a sequence of t positions sits at position t - n + i and sees the
+ * positions up to its own; rows before position 0 see none and give zeros, rows
+ * outside every sequence keep their out [rows, heads, v_dim].  P is rounded to
+ * bf16 for the second product.  workspace:
+ * mx_attn_latent_prefill_workspace_bytes(rows, kv_rows, dims) bytes, which do for
+ * any call of no more rows and kv rows with these dims too (0 bytes: NULL will
+ * do).  The latent form of mx_attn_paged_prefill. */
+size_t mx_attn_latent_prefill_workspace_bytes(int32_t rows, int32_t kv_rows,
+                                              const mx_latent_dims* dims);
+mx_status mx_attn_latent_prefill(const uint16_t* q, int64_t q_stride, const uint16_t* q_rope,
+                                 int32_t rows, const int32_t* starts, const uint16_t* kv,
+                                 int64_t kv_stride, const uint16_t* k_rope, int64_t rope_stride,
+                                 int32_t kv_rows, const int32_t* kv_starts,
+                                 const mx_latent_dims* dims, float scale, void* workspace,
+                                 uint16_t* out, void* stream);
+
 /* mx_gdn_recurrence_fast: mx_gdn_recurrence's contract (groups of t tokens,
  * optional per-token history) with the matrix-core engine's fast-mode
  * arithmetic: the same fp32 delta rule, hardware exp2 / log2 / reciprocal /
@@ -762,7 +917,7 @@ mx_status mx_engine_tensor(mx_engine* e, const char* name, void** device_ptr, si
 #define MX_DT_BF16 1
 #define MX_DT_F16 2
 #define MX_DT_F32 3
-#define MX_DT_F8E4M3 4 /* paged caches only */
+#define MX_DT_F8E4M3 4 /* paged and latent caches only */
 /* Writes one checkpoint tensor, named as in an MLX checkpoint of the hybrid
  * model (the names Weights / HybridModel::load / Mtp::load read:
  * src/weights.rs:22-99, src/hybrid.rs:56-66, 130-142, 335-352, 529-567,

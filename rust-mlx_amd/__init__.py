@@ -74,6 +74,19 @@ class PageDimsC(C.Structure):
         ("page_stride", C.c_int64)]
 
 
+class LatentDimsC(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("heads", "nope_dim", "v_dim", "latent_dim", "rope_dim",
+                                         "page_size", "pages", "sequences", "table_width",
+                                         "dtype")] + [("page_stride", C.c_int64)]
+
+
+class LogitsControlsC(C.Structure):
+    _fields_ = [("tokens", C.c_void_p), ("tokens_stride", C.c_int64)] + [(n, C.c_void_p) for n in (
+        "prompt_lens", "lens", "seqs", "repetition", "frequency", "presence", "bias_starts",
+        "bias_tokens", "bias_values", "masks", "mask_rows")] + [("mask_stride", C.c_int64)] + [
+        (n, C.c_int32) for n in ("sequences", "bias_count", "mask_states")]
+
+
 class RopeAxesC(C.Structure):
     _fields_ = [("rotary_dim", C.c_int32), ("axes", C.c_int32), ("inv_freq", C.c_void_p),
                 ("pair_axis", C.c_uint8 * 128)]
@@ -209,6 +222,18 @@ def _load() -> C.CDLL:
         "mx_attn_paged_prefill_workspace_bytes": ([i32, C.POINTER(PageDimsC)], sz),
         "mx_attn_paged_prefill": ([vp, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp,
                                    C.POINTER(PageDimsC), f32, vp, vp, vp], i32),
+        "mx_attn_latent_append": ([vp, i64, vp, i64, i32, vp, vp, vp, C.POINTER(RopeAxesC), vp, f32,
+                                   vp, C.POINTER(LatentDimsC), vp, vp, vp, vp], i32),
+        "mx_attn_latent_read": ([vp, vp, i32, vp, vp, vp, C.POINTER(LatentDimsC), vp, i64, vp, i64,
+                                 vp], i32),
+        "mx_attn_latent_decode_workspace_bytes": ([i32, C.POINTER(LatentDimsC)], sz),
+        "mx_attn_latent_decode": ([vp, vp, i32, vp, vp, vp, vp, vp, C.POINTER(LatentDimsC), f32, vp,
+                                   vp, vp], i32),
+        "mx_attn_latent_prefill_workspace_bytes": ([i32, i32, C.POINTER(LatentDimsC)], sz),
+        "mx_attn_latent_prefill": ([vp, i64, vp, i32, vp, vp, i64, vp, i64, i32, vp,
+                                    C.POINTER(LatentDimsC), f32, vp, vp, vp], i32),
+        "mx_logits_control_bf16": ([vp, i64, i32, i32, C.POINTER(LogitsControlsC), vp, i64, vp],
+                                   i32),
         "mx_sample_workspace_bytes": ([i32, i32], sz),
         "mx_sample_bf16": ([vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp], i32),
         "mx_engine_create": ([C.POINTER(ModelConfigC), C.POINTER(vp)], i32),

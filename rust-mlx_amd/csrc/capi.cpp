@@ -349,6 +349,33 @@ MX_ABI mx_status mx_argmax_bf16(const uint16_t* logits, int32_t rows, int32_t n,
   return finish(argmax_bf16(logits, rows, n, tokens, hipStream_t(stream)), "mx_argmax_bf16");
 }
 
+MX_ABI mx_status mx_logits_control_bf16(const uint16_t* logits, int64_t stride, int32_t rows,
+                                        int32_t n, const mx_logits_controls* controls,
+                                        uint16_t* out, int64_t out_stride, void* stream) {
+  const char* what = "mx_logits_control_bf16";
+  MX_CHECK(rows >= 0 && n > 0 && stride >= n && out_stride >= n, MX_EINVAL,
+           "mx_logits_control_bf16: bad shape");
+  MX_CHECK(controls != nullptr, MX_EINVAL, "mx_logits_control_bf16: null controls");
+  const mx_logits_controls& c = *controls;
+  MX_CHECK(!c.tokens || (c.lens && c.tokens_stride >= 0 && c.sequences > 0), MX_EINVAL,
+           "mx_logits_control_bf16: tokens need lens, sequences and a stride");
+  MX_CHECK(!c.bias_starts || c.bias_count == 0 || (c.bias_count > 0 && c.bias_tokens && c.bias_values),
+           MX_EINVAL, "mx_logits_control_bf16: biases need tokens and values");
+  MX_CHECK(!c.masks || (c.mask_states > 0 && c.mask_stride >= (int64_t(n) + 31) / 32), MX_EINVAL,
+           "mx_logits_control_bf16: masks need states and a stride of a bit a token");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(logits && out, MX_EINVAL, "mx_logits_control_bf16: null pointer");
+  MX_CHECK(logits != out || stride == out_stride, MX_EINVAL,
+           "mx_logits_control_bf16: in place, both strides are one");
+  const LogitsControls k{c.tokens,      c.tokens_stride, c.prompt_lens, c.lens,
+                         c.seqs,        c.repetition,    c.frequency,   c.presence,
+                         c.bias_starts, c.bias_tokens,   c.bias_values, c.masks,
+                         c.mask_rows,   c.mask_stride,   c.sequences,   c.bias_count,
+                         c.mask_states};
+  return finish(logits_control(logits, stride, rows, n, k, out, out_stride, hipStream_t(stream)),
+                what);
+}
+
 MX_ABI size_t mx_sample_workspace_bytes(int32_t rows, int32_t n) {
   return rows > 0 && n > 0 && n <= kSampleMaxVocab ? sample_workspace(rows, n) : 0;
 }
@@ -699,6 +726,187 @@ MX_ABI mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, i
            "mx_attn_paged_prefill: the workspace and out must be 16-byte aligned");
   return finish(paged_prefill(q, qkv, qkv_stride, rows, starts, lens, table, k_cache, v_cache,
                               k_scale, v_scale, d, sc, workspace, out, hipStream_t(stream)),
+                what);
+}
+
+// ---- the latent cache ---------------------------------------------------------
+namespace {
+
+// As check_pages, of a latent cache.
+const char* check_latent(const mx_latent_dims* dims, LatentDims* d, int* code) {
+  *code = MX_EINVAL;
+  if (!dims) return "null dims";
+  if (dims->heads <= 0) return "heads must be positive";
+  if (dims->pages <= 0 || dims->sequences <= 0 || dims->table_width <= 0)
+    return "pages, sequences and table_width must be positive";
+  *code = MX_EUNSUPPORTED;
+  if (dims->heads > kLatentMaxHeads) return "at most 128 heads";
+  if (dims->latent_dim != 256 && dims->latent_dim != 512) return "latent_dim must be 256 or 512";
+  if (dims->rope_dim != 64) return "rope_dim must be 64";
+  if ((dims->nope_dim != 64 && dims->nope_dim != 128) || dims->v_dim != dims->nope_dim)
+    return "nope_dim must be 64 or 128, and v_dim the same";
+  int log2 = 4;
+  while (log2 < 8 && (1 << log2) != dims->page_size) ++log2;
+  if ((1 << log2) != dims->page_size) return "page_size must be 16, 32, 64, 128 or 256";
+  if (dims->dtype != MX_DT_BF16 && dims->dtype != MX_DT_F8E4M3)
+    return "dtype must be MX_DT_BF16 or MX_DT_F8E4M3";
+  if ((int64_t(dims->table_width) << log2) > (1 << 30))
+    return "table_width * page_size must be at most 2^30";
+  *code = MX_EINVAL;
+  if (dims->page_stride < int64_t(dims->page_size) * (dims->latent_dim + dims->rope_dim) ||
+      dims->page_stride % 16 != 0)
+    return "page_stride must cover a page and be a multiple of 16";
+  if (dims->page_stride > (int64_t(1) << 60) / dims->pages) return "cache too large";
+  *d = LatentDims{dims->heads,      dims->nope_dim, dims->v_dim,     dims->latent_dim,
+                  dims->rope_dim,   log2,           dims->pages,     dims->sequences,
+                  dims->table_width, dims->dtype == MX_DT_F8E4M3, dims->page_stride};
+  return nullptr;
+}
+
+mx_status check_latent(const char* what, const mx_latent_dims* dims, LatentDims* d) {
+  int code = 0;
+  if (const char* err = check_latent(dims, d, &code))
+    return mx_status(set_error(code, std::string(what) + ": " + err));
+  return MX_OK;
+}
+
+// The attentions' factor of the scores: 0 is 1 / sqrt of a key's values.
+mx_status check_latent_scale(const char* what, const LatentDims& d, float scale, float* used) {
+  if (!(scale >= 0.0f && scale < 1e30f))
+    return mx_status(set_error(MX_EINVAL, std::string(what) + ": scale must be finite and not negative"));
+  *used = scale > 0.0f ? scale : 1.0f / __builtin_sqrtf(float(d.nope_dim + d.rope_dim));
+  return MX_OK;
+}
+
+}  // namespace
+
+MX_ABI mx_status mx_attn_latent_append(const uint16_t* x, int64_t x_stride, const uint16_t* q,
+                                       int64_t q_stride, int32_t rows, const int32_t* seqs,
+                                       const int32_t* pos, const int32_t* rope_pos,
+                                       const mx_rope_axes* rope, const uint16_t* norm, float eps,
+                                       const int32_t* table, const mx_latent_dims* dims,
+                                       uint16_t* q_rope, void* cache, float* scales, void* stream) {
+  const char* what = "mx_attn_latent_append";
+  LatentDims d;
+  if (const mx_status rc = check_latent(what, dims, &d); rc != MX_OK) return rc;
+  MX_CHECK(rows >= 0, MX_EINVAL, "mx_attn_latent_append: negative rows");
+  MX_CHECK(rope != nullptr, MX_EINVAL, "mx_attn_latent_append: null rope");
+  MX_CHECK(rope->rotary_dim == d.rope_dim && rope->axes >= 1 && rope->axes <= 4, MX_EINVAL,
+           "mx_attn_latent_append: rotary_dim must be rope_dim, axes 1..4");
+  RopeAxes r{rope->rotary_dim, rope->axes, rope->inv_freq, {}};
+  for (int i = 0; i < rope->rotary_dim / 2; ++i) {
+    MX_CHECK(rope->pair_axis[i] < rope->axes, MX_EINVAL,
+             "mx_attn_latent_append: pair_axis names an axis that is not there");
+    r.pair_axis[i] = rope->pair_axis[i];
+  }
+  MX_CHECK(eps >= 0.0f, MX_EINVAL, "mx_attn_latent_append: eps must not be negative");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(x && q && pos && rope_pos && rope->inv_freq && table && q_rope && cache &&
+               (scales || !d.f8),
+           MX_EINVAL, "mx_attn_latent_append: null pointer");
+  MX_CHECK(x_stride >= d.latent_dim + d.rope_dim &&
+               q_stride >= int64_t(d.heads) * (d.nope_dim + d.rope_dim),
+           MX_EINVAL, "mx_attn_latent_append: x_stride or q_stride shorter than a row");
+  MX_CHECK(aligned16(x) && x_stride % 8 == 0 && aligned16(q) && q_stride % 8 == 0 &&
+               aligned16(norm) && aligned16(q_rope) && aligned16(cache),
+           MX_EUNSUPPORTED,
+           "mx_attn_latent_append: x and q rows, norm, q_rope and the cache must be 16-byte aligned");
+  return finish(latent_append(x, x_stride, q, q_stride, rows, seqs, pos, rope_pos, r, norm, eps,
+                              table, d, q_rope, cache, scales, hipStream_t(stream)),
+                what);
+}
+
+MX_ABI mx_status mx_attn_latent_read(const void* cache, const float* scales, int32_t rows,
+                                     const int32_t* starts, const int32_t* first,
+                                     const int32_t* table, const mx_latent_dims* dims,
+                                     uint16_t* latent, int64_t latent_stride, uint16_t* rope,
+                                     int64_t rope_stride, void* stream) {
+  const char* what = "mx_attn_latent_read";
+  LatentDims d;
+  if (const mx_status rc = check_latent(what, dims, &d); rc != MX_OK) return rc;
+  MX_CHECK(rows >= 0, MX_EINVAL, "mx_attn_latent_read: negative rows");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(cache && starts && table && latent && rope && (scales || !d.f8), MX_EINVAL,
+           "mx_attn_latent_read: null pointer");
+  MX_CHECK(latent_stride >= d.latent_dim && rope_stride >= d.rope_dim, MX_EINVAL,
+           "mx_attn_latent_read: latent_stride or rope_stride shorter than a row");
+  MX_CHECK(aligned16(cache) && aligned16(latent) && latent_stride % 8 == 0 && aligned16(rope) &&
+               rope_stride % 8 == 0,
+           MX_EUNSUPPORTED,
+           "mx_attn_latent_read: the cache and the rows of latent and rope must be 16-byte aligned");
+  return finish(latent_read(cache, scales, rows, starts, first, table, d, latent, latent_stride,
+                            rope, rope_stride, hipStream_t(stream)),
+                what);
+}
+
+MX_ABI size_t mx_attn_latent_decode_workspace_bytes(int32_t rows, const mx_latent_dims* dims) {
+  LatentDims d;
+  int code = 0;
+  if (rows <= 0 || check_latent(dims, &d, &code)) return 0;
+  return latent_decode_workspace(rows, d);
+}
+
+MX_ABI mx_status mx_attn_latent_decode(const uint16_t* q_latent, const uint16_t* q_rope,
+                                       int32_t rows, const int32_t* seqs, const int32_t* lens,
+                                       const int32_t* table, const void* cache,
+                                       const float* scales, const mx_latent_dims* dims, float scale,
+                                       void* workspace, uint16_t* out, void* stream) {
+  const char* what = "mx_attn_latent_decode";
+  LatentDims d;
+  float sc = 0.0f;
+  if (const mx_status rc = check_latent(what, dims, &d); rc != MX_OK) return rc;
+  if (const mx_status rc = check_latent_scale(what, d, scale, &sc); rc != MX_OK) return rc;
+  MX_CHECK(rows >= 0, MX_EINVAL, "mx_attn_latent_decode: negative rows");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(q_latent && q_rope && lens && table && cache && (scales || !d.f8) && workspace && out,
+           MX_EINVAL, "mx_attn_latent_decode: null pointer");
+  MX_CHECK(aligned16(q_latent) && aligned16(q_rope) && aligned16(cache) && aligned16(workspace) &&
+               aligned16(out),
+           MX_EUNSUPPORTED,
+           "mx_attn_latent_decode: q, the cache, the workspace and out must be 16-byte aligned");
+  return finish(latent_decode(q_latent, q_rope, rows, seqs, lens, table, cache, scales, d, sc,
+                              workspace, out, hipStream_t(stream)),
+                what);
+}
+
+MX_ABI size_t mx_attn_latent_prefill_workspace_bytes(int32_t rows, int32_t kv_rows,
+                                                     const mx_latent_dims* dims) {
+  LatentDims d;
+  int code = 0;
+  if (rows <= 0 || kv_rows <= 0 || check_latent(dims, &d, &code)) return 0;
+  return latent_prefill_workspace(rows, kv_rows, d);
+}
+
+MX_ABI mx_status mx_attn_latent_prefill(const uint16_t* q, int64_t q_stride, const uint16_t* q_rope,
+                                        int32_t rows, const int32_t* starts, const uint16_t* kv,
+                                        int64_t kv_stride, const uint16_t* k_rope,
+                                        int64_t rope_stride, int32_t kv_rows,
+                                        const int32_t* kv_starts, const mx_latent_dims* dims,
+                                        float scale, void* workspace, uint16_t* out, void* stream) {
+  const char* what = "mx_attn_latent_prefill";
+  LatentDims d;
+  float sc = 0.0f;
+  if (const mx_status rc = check_latent(what, dims, &d); rc != MX_OK) return rc;
+  if (const mx_status rc = check_latent_scale(what, d, scale, &sc); rc != MX_OK) return rc;
+  MX_CHECK(rows >= 0 && kv_rows >= 0, MX_EINVAL, "mx_attn_latent_prefill: negative rows");
+  MX_CHECK(int64_t(rows) * d.heads <= 0x7fffffff, MX_EUNSUPPORTED,
+           "mx_attn_latent_prefill: rows * heads must stay below 2^31");
+  if (rows == 0) return MX_OK;
+  MX_CHECK(q && q_rope && starts && kv_starts && out && ((kv && k_rope) || kv_rows == 0) &&
+               (workspace || !latent_prefill_splits(rows, kv_rows, d)),
+           MX_EINVAL, "mx_attn_latent_prefill: null pointer");
+  MX_CHECK(q_stride >= int64_t(d.heads) * (d.nope_dim + d.rope_dim) &&
+               kv_stride >= int64_t(d.heads) * (d.nope_dim + d.v_dim) && rope_stride >= d.rope_dim,
+           MX_EINVAL, "mx_attn_latent_prefill: a stride is shorter than its row");
+  MX_CHECK(kv_stride < (int64_t(1) << 29), MX_EUNSUPPORTED,
+           "mx_attn_latent_prefill: kv_stride must stay below 2^29");
+  MX_CHECK(aligned16(q) && q_stride % 8 == 0 && aligned16(q_rope) && aligned16(kv) &&
+               kv_stride % 8 == 0 && aligned16(k_rope) && rope_stride % 8 == 0 &&
+               aligned16(workspace) && aligned16(out),
+           MX_EUNSUPPORTED,
+           "mx_attn_latent_prefill: q, kv and rotary rows, the workspace and out must be 16-byte aligned");
+  return finish(latent_prefill(q, q_stride, q_rope, rows, starts, kv, kv_stride, k_rope, rope_stride,
+                               kv_rows, kv_starts, d, sc, workspace, out, hipStream_t(stream)),
                 what);
 }
 

@@ -244,6 +244,7 @@ int paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, in
                   uint16_t* out, hipStream_t s);
 
 // ---- the latent cache (latent.hip, latent_decode.hip, latent_prefill.hip) ----
+constexpr int kLatentMaxHeads = 128;  // four matrix-core operands
 struct LatentDims {
   int heads;
   int nope_dim, v_dim;        // of a head, as formed from the latents
@@ -252,6 +253,7 @@ struct LatentDims {
   bool f8;
   int64_t page_stride;
   static constexpr int kv_heads = 1;  // all heads read the same positions
+  static constexpr bool gated = false;
 };
 // What attention with keys and values of every head knows of them: each head is a kv head.
 struct LatentPromptDims {
@@ -260,6 +262,24 @@ struct LatentPromptDims {
   int kv_rows;  // packed keys of all sequences
   static constexpr bool gated = false;
 };
+int latent_append(const uint16_t* x, int64_t x_stride, const uint16_t* q, int64_t q_stride, int rows,
+                  const int32_t* seqs, const int32_t* pos, const int32_t* rope_pos,
+                  const RopeAxes& rope, const uint16_t* norm, float eps, const int32_t* table,
+                  const LatentDims& d, uint16_t* q_rope, void* cache, float* scales, hipStream_t s);
+int latent_read(const void* cache, const float* scales, int rows, const int32_t* starts,
+                const int32_t* first, const int32_t* table, const LatentDims& d, uint16_t* latent,
+                int64_t latent_stride, uint16_t* rope, int64_t rope_stride, hipStream_t s);
+size_t latent_decode_workspace(int rows, const LatentDims& d);
+int latent_decode(const uint16_t* q_latent, const uint16_t* q_rope, int rows, const int32_t* seqs,
+                  const int32_t* lens, const int32_t* table, const void* cache, const float* scales,
+                  const LatentDims& d, float scale, void* workspace, uint16_t* out, hipStream_t s);
+size_t latent_prefill_workspace(int rows, int kv_rows, const LatentDims& d);
+bool latent_prefill_splits(int rows, int kv_rows, const LatentDims& d);  // does such a call use its workspace
+int latent_prefill(const uint16_t* q, int64_t q_stride, const uint16_t* q_rope, int rows,
+                   const int32_t* starts, const uint16_t* kv, int64_t kv_stride,
+                   const uint16_t* k_rope, int64_t rope_stride, int kv_rows,
+                   const int32_t* kv_starts, const LatentDims& d, float scale, void* workspace,
+                   uint16_t* out, hipStream_t s);
 
 // ---- MoE ----
 constexpr int kMaxRoutes = 8 * 16 + 1;
@@ -356,6 +376,23 @@ int moe_reduce_norm(const uint16_t* p, const uint16_t* factor, uint16_t* h, cons
 int head_parts(int n, int k);
 int head_partials(const QWeight& w, const uint16_t* x, int m, float* maxima, uint32_t* indices,
                   int* parts, hipStream_t s);
+// ---- controls on logits (logits.hip) ----
+struct LogitsControls {
+  const int32_t* tokens;       // [sequences][tokens_stride], or null
+  int64_t tokens_stride;
+  const int32_t *prompt_lens, *lens;  // [sequences]
+  const int32_t* seqs;         // [rows], or null
+  const float *repetition, *frequency, *presence;  // [rows], or null
+  const int32_t *bias_starts, *bias_tokens;
+  const float* bias_values;
+  const uint32_t* masks;       // [mask_states][mask_stride], or null
+  const int32_t* mask_rows;    // [rows], or null
+  int64_t mask_stride;
+  int sequences, bias_count, mask_states;
+};
+int logits_control(const uint16_t* logits, int64_t stride, int rows, int n, const LogitsControls& c,
+                   uint16_t* out, int64_t out_stride, hipStream_t s);
+
 // ---- sampling (sample.hip) ----
 constexpr int kSampleMaxVocab = 1 << 20;
 size_t sample_workspace(int rows, int n);

@@ -1,0 +1,390 @@
+// Causal attention of the last rows of packed sequences, whose keys and values have been formed from the
+// latents for every head: expanded, so that a (row, key) pair costs 2 (nope + rope + v) operations a head
+// where the latents themselves would cost 2 (2 latent + rope).
+//
+// Sequence s has the rows starts[s] .. starts[s + 1] - 1 and the keys kv_starts[s] .. kv_starts[s + 1] - 1;
+// its rows are its last positions, and each sees the keys up to its own.  A head's key is its nope part
+// beside the rotary key that all heads share; kv rows hold [head][nope | v].
+//
+// The shape is that of the paged cache's prompt attention with one row a pair: four waves take 128 rows
+// of one sequence and head, 32 matrix-core columns a wave, and walk the keys in tiles of 32:
+//   S^T = K Q^T       A: key rows from LDS, 16 bytes a lane, B: q in registers
+//   O^T = V^T P^T     A: value rows read transposed from LDS, B: P as it stands
+// with rows entering in the order that leaves P in the lane that supplies it (bits 2 and 3 exchanged).
+//
+// P is rounded to bf16 for the product, each p by at most 2^-8 of itself, as the output is; the sum that
+// divides takes P before it.
+#include <type_traits>
+
+#include "prompt_plan.hpp"
+
+namespace mx {
+
+namespace {
+
+using namespace pg;
+
+constexpr int NW = 4;   // waves of a workgroup
+static_assert(kPairs == 32 * NW, "32 rows a wave");
+constexpr int KT = 32;  // keys of a tile
+constexpr int D = 3;    // stages of a tile in LDS
+constexpr int DR = 64;  // rope_dim
+typedef short shortx4_t __attribute__((ext_vector_type(4)));
+
+// A stage: the kv rows, 1 KB of them and 128 bytes unused in turn (so that neighbours of a transposed
+// read begin at different halves of the banks), then the rotary keys.
+constexpr int kBlock = 1024 + 128;
+template <int HD>
+constexpr int rows_a_block() {
+  return 1024 / (2 * HD * 2);
+}
+template <int HD>
+constexpr int rope_at() {
+  return KT / rows_a_block<HD>() * kBlock;
+}
+template <int HD>
+constexpr int stage_bytes() {
+  return rope_at<HD>() + KT * DR * 2;
+}
+
+// 16-byte pieces of a row are exchanged by the row's number within their 128 bytes: eight rows'
+// operands meet no bank twice, nor do two pieces of four rows, as the transposed reads take them.
+__device__ __forceinline__ int swizzle(int row) {
+  return (row & 1) << 2 | (row & 2) | ((row >> 2 ^ row >> 3) & 1);
+}
+__device__ __forceinline__ uint4 lds_read16(uint32_t at) {
+  typedef uint32_t vec __attribute__((ext_vector_type(4)));
+  const vec v = *reinterpret_cast<__attribute__((address_space(3))) const vec*>(at);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+// Of sixteen lanes, four rows of sixteen values (lane j: four values of row j / 4 at `at`), lane j gets
+// the four rows' value j.
+__device__ __forceinline__ uint2 lds_read_tr(uint32_t at) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       reinterpret_cast<__attribute__((address_space(3))) shortx4_t*>(at)));
+}
+
+template <int HD>  // nope_dim and v_dim
+__global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
+    const uint16_t* __restrict__ q, int64_t q_stride, const uint16_t* __restrict__ q_rope, int rows,
+    const int32_t* __restrict__ starts, const uint16_t* __restrict__ kv, int64_t kv_stride,
+    const uint16_t* __restrict__ k_rope, int64_t rope_stride, const int32_t* __restrict__ kv_starts,
+    LatentPromptDims d, float scale, float* __restrict__ o_part, float* __restrict__ ml_part,
+    uint16_t* __restrict__ out) {
+  constexpr int KN = HD / 16, KS = KN + DR / 16;  // steps of S^T: of the nope part, all
+  constexpr int ND = HD / 32;                     // 32-dim operands of the output
+  constexpr int RB = 2 * HD * 2;                  // bytes of a kv row in LDS
+  constexpr int BR = rows_a_block<HD>();          // rows of a block
+  constexpr int RW = KT / NW;                     // rows that a wave copies
+  constexpr int CK = RW / BR;                     // copies of a wave: of kv rows, and one of rotary keys
+  constexpr int ROPE = rope_at<HD>(), STAGE = stage_bytes<HD>();
+  constexpr int R = 4;                            // operands read ahead of their products
+  extern __shared__ __align__(128) char lds[];
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+  const int col = lane & 31, h = lane >> 5;
+  const PromptPlan plan = prompt_plan(starts, kv_starts, d, rows, 1);
+  const int splits = plan.splits;
+  const Item it = item_of(blockIdx.x, plan, d.kv_heads);
+  if (it.split >= splits) return;
+  const int head = it.kvh, split = it.split;
+  Block b;
+  if (!find_block(plan, starts, kv_starts, d, rows, 1, it.block, &b)) return;  // uniform
+  const int kv_first = max(kv_starts[b.seq], 0);
+  const int prior = b.len - b.count;  // the first row's position (negative: rows without one)
+  const int last_row = min(b.pair0 + kPairs, b.count) - 1;
+  const int kall = max(prior + last_row + 1, 0);  // keys that the block sees
+  const int tiles = (kall + KT - 1) / KT;
+  const int per = (tiles + splits - 1) / splits;
+  const int tile0 = split * per, tile1 = min(tiles, tile0 + per);
+  const bool whole = tile0 == 0 && tile1 == tiles;  // also a block without keys
+  if (tile0 >= tile1 && !(split == 0 && tiles == 0)) return;
+
+  // this lane's row; lanes past the last one take that, see nothing and write nothing
+  const bool alive = b.pair0 + 32 * wave + col < b.count;
+  const int token = min(b.pair0 + 32 * wave + col, b.count - 1);
+  const int64_t qrow = b.first + token;
+  const int limit = alive ? prior + token : -1;  // the last key that the row sees
+  uint4 qb[KS];
+  {
+    const uint16_t* src = q + qrow * q_stride + int64_t(head) * (HD + DR) + 8 * h;
+    const uint16_t* rot = q_rope + (qrow * d.heads + head) * DR + 8 * h;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      qb[s] = *reinterpret_cast<const uint4*>(s < KN ? src + 16 * s : rot + 16 * (s - KN));
+  }
+  // every live row of the wave sees the keys up to low
+  const int low = prior + b.pair0 + 32 * wave;
+  const bool full = b.pair0 + 32 * wave + 31 < b.count;  // no lane past the last row
+  const int sees_all = prior + b.pair0;  // the last key that every row of the block sees
+  const float sl2 = scale * kLog2e;
+
+  // One tile's copies.  Slot i of a row holds its piece i ^ swizzle(row); a wave takes RW rows, a copy
+  // 1 KB of them.  Keys past the last one are that one: their scores are masked and their values zeroed.
+  const uint32_t lds_at =
+      uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+  const char* kv_at = reinterpret_cast<const char*>(kv + kv_first * kv_stride + int64_t(head) * 2 * HD);
+  const char* rope_src = reinterpret_cast<const char*>(k_rope + kv_first * rope_stride);
+  const int64_t kv_bytes = kv_stride * 2, rope_bytes = rope_stride * 2;
+  constexpr int LR = 64 / BR;  // lanes of a kv row
+  auto copy = [&](int tile, int stage, int i) MX_LAMBDA {  // i: 0 .. CK
+    const uint32_t to = lds_at + stage * STAGE;
+    if (i < CK) {
+      const int r = RW * wave + BR * i + lane / LR;
+      const uint32_t piece = (lane % LR) ^ swizzle(r);
+      const uint32_t dst = to + (RW * wave / BR + i) * kBlock;
+      if (tile + KT <= b.len)  // uniform
+        copy_to_lds(kv_at + (tile + RW * wave + BR * i) * kv_bytes,
+                    uint32_t(lane / LR) * uint32_t(kv_bytes) + 16 * piece, dst);
+      else
+        copy_to_lds(kv_at + min(tile + r, b.len - 1) * kv_bytes + 16 * piece, dst);
+    } else {
+      const int r = RW * wave + lane / 8;
+      const uint32_t piece = (lane % 8) ^ swizzle(r);
+      const uint32_t dst = to + ROPE + wave * 1024;
+      copy_to_lds(rope_src + min(tile + r, b.len - 1) * rope_bytes + 16 * piece, dst);
+    }
+  };
+
+  // operands of the scores' step s, and of output dims 32 n and 16 keys s
+  const int krow = (col & 0x13) | ((col & 4) << 1) | ((col & 8) >> 1);  // bits 2 and 3 exchanged
+  const uint32_t kx = 16 * (h ^ swizzle(krow));
+  const uint32_t k_at = lds_at + krow / BR * kBlock + krow % BR * RB + kx;
+  const uint32_t r_at = lds_at + ROPE + krow * (DR * 2) + kx;
+  const int vrow = 8 * h + ((lane & 15) >> 2);  // and four rows on
+  const uint32_t v_at = lds_at + vrow / BR * kBlock + vrow % BR * RB + HD * 2 + 8 * (lane & 1) +
+                        16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swizzle(vrow));
+  uint32_t kb[4], rb[4], vb[2][2];
+  auto enter = [&](uint32_t stage_at) MX_LAMBDA {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      kb[j] = (k_at ^ (32 * j)) + stage_at;
+      rb[j] = (r_at ^ (32 * j)) + stage_at;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        vb[e][u] = (v_at ^ (64 * e | 16 * u)) + (stage_at + u * (4 / BR * kBlock));
+  };
+  auto k_operand = [&](int s) MX_LAMBDA {
+    return s < KN ? lds_read16(kb[s & 3] + (s >> 2) * 128) : lds_read16(rb[s & 3]);
+  };
+  auto v_operand = [&](int i) MX_LAMBDA {
+    const int n = i % ND, s = i / ND;
+    const uint32_t off = (n >> 1) * 128 + s * (16 / BR * kBlock);
+    const uint2 x = lds_read_tr(vb[n & 1][0] + off), y = lds_read_tr(vb[n & 1][1] + off);
+    return make_uint4(x.x, x.y, y.x, y.y);
+  };
+
+  // (below every score, and finite, so that a masked one's -inf has the weight 0)
+  float m_run = -__FLT_MAX__, l_run = 0.0f;
+  floatx16_t o[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
+
+  // Tiles past the last one are copied like it, into stages that nobody reads: every step has
+  // the same copies, so waiting for all but the latest is waiting for their number.
+  const int last = (tile1 - 1) * KT;
+  if (tile0 < tile1)
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i)
+      each<CK + 1>([&](auto j) MX_LAMBDA { copy(min((tile0 + i) * KT, last), i, j); });
+  int stage = 0;
+  for (int ti = tile0; ti < tile1; ++ti) {
+    const int tile = ti * KT;
+    copies_done<(D - 2) * (CK + 1)>();  // this wave's part of the tile is in LDS ...
+    __syncthreads();  // ... and everyone's; the stage of the tile before is free
+    const uint32_t stage_at = stage * STAGE;
+    // A row's weight of 0 must not meet an infinite or NaN value that it does not see.  Keys past the
+    // last one become 0, in a tile that has any; in one that some rows see and some do not, such values go
+    // to the sums of the rows that see them (they stay infinite or NaN whatever their weight) and
+    // become 0 for the product.
+    auto value_at = [&](int key, int piece) MX_LAMBDA {
+      return lds + stage_at + key / BR * kBlock + key % BR * RB + HD * 2 + 16 * (piece ^ swizzle(key));
+    };
+    const bool some_hidden = tile + KT - 1 > sees_all;
+    if (some_hidden) {  // uniform
+      auto odd = [](uint32_t w) MX_LAMBDA {
+        return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+      };
+      bool some = false;
+      for (int i = t; i < KT * HD / 8; i += 64 * NW) {
+        uint4* p = reinterpret_cast<uint4*>(value_at(i / (HD / 8), i % (HD / 8)));
+        if (tile + i / (HD / 8) >= kall) {
+          *p = make_uint4(0, 0, 0, 0);
+        } else {
+          const uint4 v = *p;
+          some |= odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w);
+        }
+      }
+      if (__syncthreads_or(some)) {
+        for (int key = 0; key < KT; ++key) {
+          const bool in = tile + key <= limit;
+          int half = h;  // addresses formed for each key: kept over the keys they would take
+          asm volatile("" : "+v"(half));  // a register for every sum, in the loop over tiles too
+#pragma unroll
+          for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int dim = 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
+              const uint16_t v = reinterpret_cast<const uint16_t*>(value_at(key, dim >> 3))[dim & 7];
+              if (in && (v & 0x7f80u) == 0x7f80u) o[n][r] += bf16_to_f32(v);
+            }
+        }
+        __syncthreads();
+        for (int i = t; i < KT * HD; i += 64 * NW) {
+          uint16_t* v = reinterpret_cast<uint16_t*>(value_at(i / HD, i % HD / 8)) + i % 8;
+          if ((*v & 0x7f80u) == 0x7f80u) *v = 0;
+        }
+        __syncthreads();
+      }
+    }
+    const int ahead = stage == 0 ? D - 1 : stage - 1;  // of tile ti + D - 1
+    const int at = min((ti + D - 1) * KT, last);
+    enter(stage_at);
+    floatx16_t sc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+    {
+      uint4 a[R];
+      each<R>([&](auto s) MX_LAMBDA { a[s] = k_operand(s); });
+      each<KS>([&](auto s) MX_LAMBDA {
+        __builtin_amdgcn_sched_barrier(0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[s % R]),
+                                                     __builtin_bit_cast(bf16x8_t, qb[s]), sc, 0, 0, 0);
+        if constexpr (s + R < KS) a[s % R] = k_operand(s + R);
+        if constexpr (s <= CK) copy(at, ahead, s);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // sc[r]: key 16 (r / 8) + 8 h + r % 8 of the tile
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] *= sl2;
+    if (tile + KT - 1 > low || !full) {
+      const int end = limit + 1 - tile - 8 * h;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[r] = 16 * (r >> 3) + (r & 7) < end ? sc[r] : neg_inf();
+    }
+    float mt = sc[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mt = fmaxf(mt, sc[r]);
+    mt = max_across_halves(mt);
+    // The reference follows the maximum in steps of at least 8 (a factor of 256, far from any
+    // limit of fp32 or bf16), so that most tiles rescale nothing.
+    if (__any(mt > m_run + 8.0f)) {
+      const float mn = mt > m_run + 8.0f ? mt : m_run;  // each column by its own scores alone
+      const float alpha = __builtin_amdgcn_exp2f(m_run - mn);
+      l_run *= alpha;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
+      m_run = mn;
+    }
+    uint32_t pb[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = __builtin_amdgcn_exp2f(sc[2 * j] - m_run);
+      const float y = __builtin_amdgcn_exp2f(sc[2 * j + 1] - m_run);
+      l_run += x + y;
+      pb[j] = pack2(x, y);
+    }
+    {
+      uint4 a[R];
+      each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(i); });
+      each<2 * ND>([&](auto i) MX_LAMBDA {
+        constexpr int s = i / ND, n = i % ND;
+        __builtin_amdgcn_sched_barrier(0);
+        o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8_t, a[i % R]),
+            __builtin_bit_cast(bf16x8_t,
+                               make_uint4(pb[4 * s], pb[4 * s + 1], pb[4 * s + 2], pb[4 * s + 3])),
+            o[n], 0, 0, 0);
+        if constexpr (i + R < 2 * ND) a[i % R] = v_operand(i + R);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    stage = stage == D - 1 ? 0 : stage + 1;
+  }
+  copies_done<0>();  // none lands in LDS that is no longer this workgroup's
+  if (!alive) return;
+  l_run += __shfl_xor(l_run, 32, 64);
+  const int64_t at = qrow * d.heads + head;
+  if (whole) {
+    const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+    uint16_t* dst = out + at * HD + 4 * h;
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = l_run == 0.0f ? 0.0f : o[n][4 * a + r] * inv;
+        *reinterpret_cast<uint2*>(dst + 32 * n + 8 * a) = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+      }
+    return;
+  }
+  const int64_t part = at * splits + split;
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      *reinterpret_cast<float4*>(o_part + part * HD + 32 * n + 8 * a + 4 * h) = make_float4(
+          o[n][4 * a], o[n][4 * a + 1], o[n][4 * a + 2], o[n][4 * a + 3]);
+  if (h == 0) {
+    ml_part[part * 2] = m_run;
+    ml_part[part * 2 + 1] = l_run;
+  }
+}
+
+LatentPromptDims prompt_dims(int kv_rows, const LatentDims& d) {
+  return LatentPromptDims{d.heads, d.heads, d.sequences, kv_rows};
+}
+
+}  // namespace
+
+size_t latent_prefill_workspace(int rows, int kv_rows, const LatentDims& d) {
+  return prompt_workspace(rows, d.v_dim, prompt_dims(kv_rows, d));
+}
+
+bool latent_prefill_splits(int rows, int kv_rows, const LatentDims& d) {
+  const LatentPromptDims p = prompt_dims(kv_rows, d);
+  return splits_of(least_blocks(rows, p), p) > 1;
+}
+
+int latent_prefill(const uint16_t* q, int64_t q_stride, const uint16_t* q_rope, int rows,
+                   const int32_t* starts, const uint16_t* kv, int64_t kv_stride,
+                   const uint16_t* k_rope, int64_t rope_stride, int kv_rows,
+                   const int32_t* kv_starts, const LatentDims& dims, float scale, void* workspace,
+                   uint16_t* out, hipStream_t s) {
+  const LatentPromptDims d = prompt_dims(kv_rows, dims);
+  const int64_t grid = prompt_grid(rows, d), joins = prompt_joins(rows, d);
+  const int splits = splits_of(least_blocks(rows, d), d);  // at most
+  if (grid > 0x7fffffff || joins > 0x7fffffff) return MX_EUNSUPPORTED;
+  float* o_part = static_cast<float*>(workspace);
+  float* ml_part = o_part + size_t(rows) * d.heads * splits * dims.v_dim;
+#define MX_PREFILL(HD)                                                                             \
+  if (dims.v_dim == HD) {                                                                          \
+    const auto fn = prefill_kernel<HD>;                                                            \
+    constexpr int lb = D * stage_bytes<HD>();                                                      \
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn),                                     \
+                            hipFuncAttributeMaxDynamicSharedMemorySize, lb) != hipSuccess)         \
+      return MX_EHIP;                                                                              \
+    hipLaunchKernelGGL(fn, dim3(unsigned(grid)), dim3(64 * NW), lb, s, q, q_stride, q_rope, rows,  \
+                       starts, kv, kv_stride, k_rope, rope_stride, kv_starts, d, scale, o_part,    \
+                       ml_part, out);                                                              \
+    if (hipGetLastError() != hipSuccess) return MX_EHIP;                                           \
+    if (splits == 1) return MX_OK;                                                                 \
+    hipLaunchKernelGGL((prefill_join_kernel<HD, KT, LatentPromptDims>), dim3(unsigned(joins)),     \
+                       dim3(256), 0, s, nullptr, 0, rows, starts, kv_starts, nullptr, d, o_part,   \
+                       ml_part, out);                                                              \
+    return hipGetLastError() == hipSuccess ? MX_OK : MX_EHIP;                                      \
+  }
+  MX_PREFILL(64) MX_PREFILL(128)
+#undef MX_PREFILL
+  return MX_EUNSUPPORTED;
+}
+
+}  // namespace mx
