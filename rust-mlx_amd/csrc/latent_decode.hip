@@ -522,7 +522,7 @@ __global__ __launch_bounds__(EL * G) void join_kernel(const int32_t* __restrict_
   if (n <= 1) return;
   const floatx4_t* po = reinterpret_cast<const floatx4_t*>(o_part) + int64_t(rp.x) * all + i;
   const float2* pm = reinterpret_cast<const float2*>(ml_part) + int64_t(rp.x) * d.heads + head;
-  constexpr int A = 8;  // pieces on their way
+  constexpr int A = G > 4 ? 4 : 8;  // pieces on their way
   // each set by its own running maximum; the sets' sums are brought together below
   float M = -__FLT_MAX__, L = 0.0f;
   floatx4_t O = 0.0f;
@@ -531,9 +531,13 @@ __global__ __launch_bounds__(EL * G) void join_kernel(const int32_t* __restrict_
     float2 ml[A];
 #pragma unroll
     for (int k = 0; k < A; ++k) {
-      const int64_t p = min(c + G * k, n - 1);
-      v[k] = po[p * all];
-      ml[k] = pm[p * d.heads];
+      const int64_t p = c + G * k;
+      ml[k] = make_float2(-__FLT_MAX__, 0.0f);
+      v[k] = 0.0f;
+      if (p < n) {
+        v[k] = po[p * all];
+        ml[k] = pm[p * d.heads];
+      }
     }
     float m = M;
 #pragma unroll
@@ -543,12 +547,11 @@ __global__ __launch_bounds__(EL * G) void join_kernel(const int32_t* __restrict_
     for (int j = 0; j < 4; ++j) O[j] *= w0;
     M = m;
 #pragma unroll
-    for (int k = 0; k < A; ++k)
-      if (c + G * k < n) {
-        const float w = __builtin_amdgcn_exp2f(ml[k].x - M);
-        L = fmaf_(ml[k].y, w, L);
-        for (int j = 0; j < 4; ++j) O[j] = fmaf_(v[k][j], w, O[j]);
-      }
+    for (int k = 0; k < A; ++k) {
+      const float w = __builtin_amdgcn_exp2f(ml[k].x - M);
+      L = fmaf_(ml[k].y, w, L);
+      for (int j = 0; j < 4; ++j) O[j] = fmaf_(v[k][j], w, O[j]);
+    }
   }
   if constexpr (G > 1) {
     mx[g][e] = M;
@@ -624,7 +627,7 @@ int latent_decode(const uint16_t* q_latent, const uint16_t* q_rope, int rows, co
     if (hipGetLastError() != hipSuccess) return MX_EHIP;                                         \
     /* few rows have many pieces each */                                                         \
     if (rows <= 4)                                                                               \
-      MX_JOIN(DC, 64, 16)                                                                        \
+      MX_JOIN(DC, 16, 64)                                                                        \
     else if (rows <= 16)                                                                         \
       MX_JOIN(DC, 64, 4)                                                                         \
     else                                                                                         \
