@@ -728,8 +728,8 @@ mx_status mx_attn_latent_decode(const uint16_t* q_latent, const uint16_t* q_rope
  * rotary part is not read, q_rope [rows, heads, rope_dim] is, as
  * mx_attn_latent_append gives it) are the last positions of sequence s, whose
  * positions are the rows kv_starts[s] .. kv_starts[s + 1] - 1 of kv
- * [kv_rows][heads][nope_dim key | v_dim value] (kv_stride apart, below 2^29) and
- * k_rope [kv_rows][rope_dim] (rope_stride apart; rotated, as mx_attn_latent_read
+ * [kv_rows][heads][nope_dim key | v_dim value] (kv_stride apart) and k_rope
+ * [kv_rows][rope_dim] (rope_stride apart, both below 2^28; rotated, as mx_attn_latent_read
  * gives it); starts and kv_starts: int32 [sequences + 1], not decreasing, up to
  * rows and kv_rows.  Of dims the head's and the number of sequences count.  Row i
  * of n over a sequence of t positions sits at position t - n + i and sees the

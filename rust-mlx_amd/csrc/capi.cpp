@@ -898,8 +898,8 @@ MX_ABI mx_status mx_attn_latent_prefill(const uint16_t* q, int64_t q_stride, con
   MX_CHECK(q_stride >= int64_t(d.heads) * (d.nope_dim + d.rope_dim) &&
                kv_stride >= int64_t(d.heads) * (d.nope_dim + d.v_dim) && rope_stride >= d.rope_dim,
            MX_EINVAL, "mx_attn_latent_prefill: a stride is shorter than its row");
-  MX_CHECK(kv_stride < (int64_t(1) << 29), MX_EUNSUPPORTED,
-           "mx_attn_latent_prefill: kv_stride must stay below 2^29");
+  MX_CHECK(kv_stride < (int64_t(1) << 28) && rope_stride < (int64_t(1) << 28), MX_EUNSUPPORTED,
+           "mx_attn_latent_prefill: kv_stride and rope_stride must stay below 2^28");
   MX_CHECK(aligned16(q) && q_stride % 8 == 0 && aligned16(q_rope) && aligned16(kv) &&
                kv_stride % 8 == 0 && aligned16(k_rope) && rope_stride % 8 == 0 &&
                aligned16(workspace) && aligned16(out),

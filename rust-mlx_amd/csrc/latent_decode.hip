@@ -61,13 +61,13 @@ constexpr int lds_bytes() {
 }
 
 // A tile lies in LDS as blocks of 64 values of its 32 rows, so that a copy of 1 KB is some rows of a block.
-// 16-byte pieces are exchanged by the row's number within a block's row, so that neither the rows' operands
-// nor the transposed reads, of four rows of bf16 or eight of e4m3 at once, meet a bank twice (e4m3 rows'
-// operands of 8 bytes do, which costs them what 16 bytes cost).
+// 16-byte pieces are exchanged by the row's number within a block's row, so that neither sixteen rows' operands
+// nor the transposed reads, of four rows of bf16 or eight of e4m3 at once, meet one of the 64 banks twice
+// (e4m3 rows' operands of 8 bytes do, which costs them what 16 bytes cost).
 template <bool F8>
 __device__ __forceinline__ int swizzle(int row) {
   return F8 ? ((row >> 1) & 2) ^ ((row >> 3) & 2) ^ ((row >> 1 ^ row >> 3) & 1)
-            : (row & 3) << 1 | ((row >> 2 ^ row >> 3) & 1);
+            : (row & 2) << 1 | (row >> 1 & 2) | (row >> 3 & 1);
 }
 template <class T>
 __device__ __forceinline__ T lds_read(uint32_t at) {
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * HW * shares<HW>(), HW == 1 && !F8 ? 1 : 2) voi
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int u = 0; u < (F8 ? 1 : 2); ++u) {
-        vb[e][u] = (v_at ^ (F8 ? 32 * e : 64 * e | 16 * u)) + (at + u * 4 * RB);
+        vb[e][u] = (v_at ^ (F8 ? 32 * e : 64 * e | 32 * u)) + (at + u * 4 * RB);
         asm volatile("" : "+v"(vb[e][u]));
       }
   };

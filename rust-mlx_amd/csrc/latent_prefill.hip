@@ -31,26 +31,18 @@ constexpr int D = 3;    // stages of a tile in LDS
 constexpr int DR = 64;  // rope_dim
 typedef short shortx4_t __attribute__((ext_vector_type(4)));
 
-// A stage: the kv rows, 1 KB of them and 128 bytes unused in turn (so that neighbours of a transposed
-// read begin at different halves of the banks), then the rotary keys.
-constexpr int kBlock = 1024 + 128;
-template <int HD>
-constexpr int rows_a_block() {
-  return 1024 / (2 * HD * 2);
-}
-template <int HD>
-constexpr int rope_at() {
-  return KT / rows_a_block<HD>() * kBlock;
-}
+// A stage holds blocks of 64 values of its keys' rows: a head's keys and values, then the rotary keys.  Three
+// stages fit twice into a compute unit's LDS (two of 64 keys, 80 KB, do not: 1005 us against 727).
+constexpr int kBlock = KT * 128;
 template <int HD>
 constexpr int stage_bytes() {
-  return rope_at<HD>() + KT * DR * 2;
+  return (2 * HD + DR) / 64 * kBlock;
 }
 
-// 16-byte pieces of a row are exchanged by the row's number within their 128 bytes: eight rows'
-// operands meet no bank twice, nor do two pieces of four rows, as the transposed reads take them.
+// 16-byte pieces of a block's row are exchanged by the row's number: sixteen rows' operands meet none of the
+// 64 banks twice, nor do four pieces of four rows, as the transposed reads take them.
 __device__ __forceinline__ int swizzle(int row) {
-  return (row & 1) << 2 | (row & 2) | ((row >> 2 ^ row >> 3) & 1);
+  return (row & 2) << 1 | (row >> 1 & 2) | (row >> 3 & 1);
 }
 __device__ __forceinline__ uint4 lds_read16(uint32_t at) {
   typedef uint32_t vec __attribute__((ext_vector_type(4)));
@@ -72,12 +64,12 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     LatentPromptDims d, float scale, float* __restrict__ o_part, float* __restrict__ ml_part,
     uint16_t* __restrict__ out) {
   constexpr int KN = HD / 16, KS = KN + DR / 16;  // steps of S^T: of the nope part, all
+  constexpr int KB = KT / 32;                     // 32-key operands of a tile
   constexpr int ND = HD / 32;                     // 32-dim operands of the output
-  constexpr int RB = 2 * HD * 2;                  // bytes of a kv row in LDS
-  constexpr int BR = rows_a_block<HD>();          // rows of a block
-  constexpr int RW = KT / NW;                     // rows that a wave copies
-  constexpr int CK = RW / BR;                     // copies of a wave: of kv rows, and one of rotary keys
-  constexpr int ROPE = rope_at<HD>(), STAGE = stage_bytes<HD>();
+  constexpr int NB = (2 * HD + DR) / 64;          // blocks of a stage, the rotary one last
+  constexpr int G = KT / NW / 8;                  // eights of rows that a wave copies
+  constexpr int NC = NB * G;                      // its copies: eight rows of a block
+  constexpr int STAGE = stage_bytes<HD>();
   constexpr int R = 4;                            // operands read ahead of their products
   extern __shared__ __align__(128) char lds[];
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
@@ -118,60 +110,57 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   const int sees_all = prior + b.pair0;  // the last key that every row of the block sees
   const float sl2 = scale * kLog2e;
 
-  // One tile's copies.  Slot i of a row holds its piece i ^ swizzle(row); a wave takes RW rows, a copy
-  // 1 KB of them.  Keys past the last one are that one: their scores are masked and their values zeroed.
+  // One tile's copies: a wave takes some of its rows, eight a copy of 1 KB of one block.  A lane copies the piece of
+  // its row that its place is for.  Keys past the last one are that one: their scores are masked and their
+  // values zeroed.
   const uint32_t lds_at =
       uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
   const char* kv_at = reinterpret_cast<const char*>(kv + kv_first * kv_stride + int64_t(head) * 2 * HD);
-  const char* rope_src = reinterpret_cast<const char*>(k_rope + kv_first * rope_stride);
+  const char* rope_at = reinterpret_cast<const char*>(k_rope + kv_first * rope_stride);
   const int64_t kv_bytes = kv_stride * 2, rope_bytes = rope_stride * 2;
-  constexpr int LR = 64 / BR;  // lanes of a kv row
-  auto copy = [&](int tile, int stage, int i) MX_LAMBDA {  // i: 0 .. CK
-    const uint32_t to = lds_at + stage * STAGE;
-    if (i < CK) {
-      const int r = RW * wave + BR * i + lane / LR;
-      const uint32_t piece = (lane % LR) ^ swizzle(r);
-      const uint32_t dst = to + (RW * wave / BR + i) * kBlock;
-      if (tile + KT <= b.len)  // uniform
-        copy_to_lds(kv_at + (tile + RW * wave + BR * i) * kv_bytes,
-                    uint32_t(lane / LR) * uint32_t(kv_bytes) + 16 * piece, dst);
+  uint32_t kv_off[G], rope_off[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const uint32_t piece = 16 * ((lane & 7) ^ swizzle(8 * (G * wave + g) + (lane >> 3)));
+    kv_off[g] = uint32_t(lane >> 3) * uint32_t(kv_bytes) + piece;
+    rope_off[g] = uint32_t(lane >> 3) * uint32_t(rope_bytes) + piece;
+  }
+  auto copy = [&](int tile, int stage, int i) MX_LAMBDA {  // i: 0 .. NC - 1
+    const int block = i / G, g = i % G, r = 8 * (G * wave + g);
+    const uint32_t to = lds_at + stage * STAGE + block * kBlock + r * 128;
+    if (tile + KT <= b.len) {  // uniform
+      if (block < NB - 1)
+        copy_to_lds(kv_at + (tile + r) * kv_bytes + block * 128, kv_off[g], to);
       else
-        copy_to_lds(kv_at + min(tile + r, b.len - 1) * kv_bytes + 16 * piece, dst);
+        copy_to_lds(rope_at + (tile + r) * rope_bytes, rope_off[g], to);
     } else {
-      const int r = RW * wave + lane / 8;
-      const uint32_t piece = (lane % 8) ^ swizzle(r);
-      const uint32_t dst = to + ROPE + wave * 1024;
-      copy_to_lds(rope_src + min(tile + r, b.len - 1) * rope_bytes + 16 * piece, dst);
+      const int key = min(tile + r + (lane >> 3), b.len - 1);
+      const uint32_t piece = 16 * ((lane & 7) ^ swizzle(r + (lane >> 3)));
+      copy_to_lds((block < NB - 1 ? kv_at + key * kv_bytes + block * 128 : rope_at + key * rope_bytes) + piece, to);
     }
   };
 
-  // operands of the scores' step s, and of output dims 32 n and 16 keys s
+  // Operands of product i of the scores, and of P V.  Steps differ by the exchanged bits within a block's row.
   const int krow = (col & 0x13) | ((col & 4) << 1) | ((col & 8) >> 1);  // bits 2 and 3 exchanged
-  const uint32_t kx = 16 * (h ^ swizzle(krow));
-  const uint32_t k_at = lds_at + krow / BR * kBlock + krow % BR * RB + kx;
-  const uint32_t r_at = lds_at + ROPE + krow * (DR * 2) + kx;
+  const uint32_t k_at = lds_at + krow * 128 + 16 * (h ^ swizzle(krow));
   const int vrow = 8 * h + ((lane & 15) >> 2);  // and four rows on
-  const uint32_t v_at = lds_at + vrow / BR * kBlock + vrow % BR * RB + HD * 2 + 8 * (lane & 1) +
+  const uint32_t v_at = lds_at + HD / 64 * kBlock + vrow * 128 + 8 * (lane & 1) +
                         16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swizzle(vrow));
-  uint32_t kb[4], rb[4], vb[2][2];
+  uint32_t kb[4], vb[2][2];
   auto enter = [&](uint32_t stage_at) MX_LAMBDA {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       kb[j] = (k_at ^ (32 * j)) + stage_at;
-      rb[j] = (r_at ^ (32 * j)) + stage_at;
+      vb[j >> 1][j & 1] = (v_at ^ (64 * (j >> 1) | 32 * (j & 1))) + (stage_at + (j & 1) * 512);
     }
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        vb[e][u] = (v_at ^ (64 * e | 16 * u)) + (stage_at + u * (4 / BR * kBlock));
   };
-  auto k_operand = [&](int s) MX_LAMBDA {
-    return s < KN ? lds_read16(kb[s & 3] + (s >> 2) * 128) : lds_read16(rb[s & 3]);
+  auto k_operand = [&](int i) MX_LAMBDA {
+    const int s = i / KB;
+    return lds_read16(kb[s & 3] + ((s < KN ? s >> 2 : NB - 1) * kBlock + i % KB * (32 * 128)));
   };
   auto v_operand = [&](int i) MX_LAMBDA {
     const int n = i % ND, s = i / ND;
-    const uint32_t off = (n >> 1) * 128 + s * (16 / BR * kBlock);
+    const uint32_t off = (n >> 1) * kBlock + s * (16 * 128);
     const uint2 x = lds_read_tr(vb[n & 1][0] + off), y = lds_read_tr(vb[n & 1][1] + off);
     return make_uint4(x.x, x.y, y.x, y.y);
   };
@@ -190,11 +179,11 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   if (tile0 < tile1)
 #pragma unroll
     for (int i = 0; i < D - 1; ++i)
-      each<CK + 1>([&](auto j) MX_LAMBDA { copy(min((tile0 + i) * KT, last), i, j); });
+      each<NC>([&](auto j) MX_LAMBDA { copy(min((tile0 + i) * KT, last), i, j); });
   int stage = 0;
   for (int ti = tile0; ti < tile1; ++ti) {
     const int tile = ti * KT;
-    copies_done<(D - 2) * (CK + 1)>();  // this wave's part of the tile is in LDS ...
+    copies_done<(D - 2) * NC>();  // this wave's part of the tile is in LDS ...
     __syncthreads();  // ... and everyone's; the stage of the tile before is free
     const uint32_t stage_at = stage * STAGE;
     // A row's weight of 0 must not meet an infinite or NaN value that it does not see.  Keys past the
@@ -202,7 +191,8 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     // to the sums of the rows that see them (they stay infinite or NaN whatever their weight) and
     // become 0 for the product.
     auto value_at = [&](int key, int piece) MX_LAMBDA {
-      return lds + stage_at + key / BR * kBlock + key % BR * RB + HD * 2 + 16 * (piece ^ swizzle(key));
+      return lds + stage_at + (HD / 64 + (piece >> 3)) * kBlock + key * 128 +
+             16 * ((piece & 7) ^ swizzle(key));
     };
     const bool some_hidden = tile + KT - 1 > sees_all;
     if (some_hidden) {  // uniform
@@ -244,33 +234,38 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     const int ahead = stage == 0 ? D - 1 : stage - 1;  // of tile ti + D - 1
     const int at = min((ti + D - 1) * KT, last);
     enter(stage_at);
-    floatx16_t sc;
+    floatx16_t sc[KB];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
-    {
-      uint4 a[R];
-      each<R>([&](auto s) MX_LAMBDA { a[s] = k_operand(s); });
-      each<KS>([&](auto s) MX_LAMBDA {
-        __builtin_amdgcn_sched_barrier(0);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[s % R]),
-                                                     __builtin_bit_cast(bf16x8_t, qb[s]), sc, 0, 0, 0);
-        if constexpr (s + R < KS) a[s % R] = k_operand(s + R);
-        if constexpr (s <= CK) copy(at, ahead, s);
-      });
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[k][r] = 0.0f;
+    uint4 a[R];
+    each<R>([&](auto i) MX_LAMBDA { a[i] = k_operand(i); });
+    // Issued together the copies hold up every wave of the workgroup at once, so they are spread over the
+    // products.
+    each<KS * KB>([&](auto i) MX_LAMBDA {
       __builtin_amdgcn_sched_barrier(0);
-    }
-    // sc[r]: key 16 (r / 8) + 8 h + r % 8 of the tile
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sc[r] *= sl2;
+      sc[i % KB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[i % R]),
+                                                           __builtin_bit_cast(bf16x8_t, qb[i / KB]),
+                                                           sc[i % KB], 0, 0, 0);
+      if constexpr (i + R < KS * KB) a[i % R] = k_operand(i + R);
+      constexpr int first = i * NC / (KS * KB), end = (i + 1) * NC / (KS * KB);
+      each<end - first>([&](auto j) MX_LAMBDA { copy(at, ahead, first + j); });
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(i); });
+    // sc[k][r]: key 32 k + 16 (r / 8) + 8 h + r % 8 of the tile
     if (tile + KT - 1 > low || !full) {
       const int end = limit + 1 - tile - 8 * h;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] = 16 * (r >> 3) + (r & 7) < end ? sc[r] : neg_inf();
-    }
-    float mt = sc[0];
+      for (int k = 0; k < KB; ++k)
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mt = fmaxf(mt, sc[r]);
-    mt = max_across_halves(mt);
+        for (int r = 0; r < 16; ++r) sc[k][r] = 32 * k + 16 * (r >> 3) + (r & 7) < end ? sc[k][r] : neg_inf();
+    }
+    float mt = sc[0][0];
+#pragma unroll
+    for (int i = 1; i < 16 * KB; ++i) mt = fmaxf(mt, sc[i / 16][i % 16]);
+    mt = max_across_halves(mt) * sl2;
     // The reference follows the maximum in steps of at least 8 (a factor of 256, far from any
     // limit of fp32 or bf16), so that most tiles rescale nothing.
     if (__any(mt > m_run + 8.0f)) {
@@ -283,29 +278,32 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
         for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
       m_run = mn;
     }
-    uint32_t pb[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = __builtin_amdgcn_exp2f(sc[2 * j] - m_run);
-      const float y = __builtin_amdgcn_exp2f(sc[2 * j + 1] - m_run);
+    uint32_t pb[8 * KB];
+    auto pair = [&](auto j) MX_LAMBDA {
+      constexpr int k = j / 8, r = 2 * (j % 8);
+      const float x = __builtin_amdgcn_exp2f(fmaf_(sc[k][r], sl2, -m_run));
+      const float y = __builtin_amdgcn_exp2f(fmaf_(sc[k][r + 1], sl2, -m_run));
       l_run += x + y;
       pb[j] = pack2(x, y);
-    }
-    {
-      uint4 a[R];
-      each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(i); });
-      each<2 * ND>([&](auto i) MX_LAMBDA {
-        constexpr int s = i / ND, n = i % ND;
-        __builtin_amdgcn_sched_barrier(0);
-        o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            __builtin_bit_cast(bf16x8_t, a[i % R]),
-            __builtin_bit_cast(bf16x8_t,
-                               make_uint4(pb[4 * s], pb[4 * s + 1], pb[4 * s + 2], pb[4 * s + 3])),
-            o[n], 0, 0, 0);
-        if constexpr (i + R < 2 * ND) a[i % R] = v_operand(i + R);
-      });
+    };
+    // P V of 16 keys takes four pairs; the next four form between its products
+    each<4>(pair);
+    constexpr int kP = 2 * KB * ND;
+    each<kP>([&](auto i) MX_LAMBDA {
+      constexpr int s = i / ND, n = i % ND;
       __builtin_amdgcn_sched_barrier(0);
-    }
+      o[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          __builtin_bit_cast(bf16x8_t, a[i % R]),
+          __builtin_bit_cast(bf16x8_t,
+                             make_uint4(pb[4 * s], pb[4 * s + 1], pb[4 * s + 2], pb[4 * s + 3])),
+          o[n], 0, 0, 0);
+      if constexpr (i + R < kP) a[i % R] = v_operand(i + R);
+      if constexpr (s + 1 < 2 * KB) {
+        constexpr int first = 4 * n / ND, end = 4 * (n + 1) / ND;
+        each<end - first>([&](auto j) MX_LAMBDA { pair(std::integral_constant<int, 4 * (s + 1) + first + j>{}); });
+      }
+    });
+    __builtin_amdgcn_sched_barrier(0);
     stage = stage == D - 1 ? 0 : stage + 1;
   }
   copies_done<0>();  // none lands in LDS that is no longer this workgroup's
