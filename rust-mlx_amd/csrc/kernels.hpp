@@ -218,6 +218,8 @@ struct PageDims {
   int table_width;    // entries of a row of the page table
   bool f8, gated;     // e4m3 cache; qkv rows hold [q | gate] per head
   int64_t page_stride;  // elements between pages
+  // of prompts: (row, q head) pairs of a workgroup, and workgroups that run at once
+  static constexpr int kPairs = 128, kAtOnce = 512;
 };
 struct RopeAxes {
   int rotary_dim, axes;
@@ -261,6 +263,7 @@ struct LatentPromptDims {
   int sequences;
   int kv_rows;  // packed keys of all sequences
   static constexpr bool gated = false;
+  static constexpr int kPairs = 256, kAtOnce = 256;
 };
 int latent_append(const uint16_t* x, int64_t x_stride, const uint16_t* q, int64_t q_stride, int rows,
                   const int32_t* seqs, const int32_t* pos, const int32_t* rope_pos,

@@ -6,8 +6,8 @@
 // its rows are its last positions, and each sees the keys up to its own.  A head's key is its nope part
 // beside the rotary key that all heads share; kv rows hold [head][nope | v].
 //
-// The shape is that of the paged cache's prompt attention with one row a pair: four waves take 128 rows
-// of one sequence and head, 32 matrix-core columns a wave, and walk the keys in tiles of 32:
+// The shape is that of the paged cache's prompt attention with one row a pair: eight waves take 256 rows
+// of one sequence and head, 32 matrix-core columns a wave, and walk the keys in tiles of 64:
 //   S^T = K Q^T       A: key rows from LDS, 16 bytes a lane, B: q in registers
 //   O^T = V^T P^T     A: value rows read transposed from LDS, B: P as it stands
 // with rows entering in the order that leaves P in the lane that supplies it (bits 2 and 3 exchanged).
@@ -24,15 +24,15 @@ namespace {
 
 using namespace pg;
 
-constexpr int NW = 4;   // waves of a workgroup
-static_assert(kPairs == 32 * NW, "32 rows a wave");
-constexpr int KT = 32;  // keys of a tile
+constexpr int NW = 8;   // waves of a workgroup
+constexpr int kRows = LatentPromptDims::kPairs;
+static_assert(kRows == 32 * NW, "32 rows a wave");
+constexpr int KT = 64;  // keys of a tile
 constexpr int D = 3;    // stages of a tile in LDS
 constexpr int DR = 64;  // rope_dim
 typedef short shortx4_t __attribute__((ext_vector_type(4)));
 
-// A stage holds blocks of 64 values of its keys' rows: a head's keys and values, then the rotary keys.  Three
-// stages fit twice into a compute unit's LDS (two of 64 keys, 80 KB, do not: 1005 us against 727).
+// A stage holds blocks of 64 values of its keys' rows: a head's keys and values, then the rotary keys.
 constexpr int kBlock = KT * 128;
 template <int HD>
 constexpr int stage_bytes() {
@@ -76,14 +76,14 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   const int col = lane & 31, h = lane >> 5;
   const PromptPlan plan = prompt_plan(starts, kv_starts, d, rows, 1);
   const int splits = plan.splits;
-  const Item it = item_of(blockIdx.x, plan, d.kv_heads);
+  const Item it = item_of<LatentPromptDims>(blockIdx.x, plan, d.kv_heads);
   if (it.split >= splits) return;
   const int head = it.kvh, split = it.split;
   Block b;
   if (!find_block(plan, starts, kv_starts, d, rows, 1, it.block, &b)) return;  // uniform
   const int kv_first = max(kv_starts[b.seq], 0);
   const int prior = b.len - b.count;  // the first row's position (negative: rows without one)
-  const int last_row = min(b.pair0 + kPairs, b.count) - 1;
+  const int last_row = min(b.pair0 + kRows, b.count) - 1;
   const int kall = max(prior + last_row + 1, 0);  // keys that the block sees
   const int tiles = (kall + KT - 1) / KT;
   const int per = (tiles + splits - 1) / splits;
@@ -104,8 +104,9 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     for (int s = 0; s < KS; ++s)
       qb[s] = *reinterpret_cast<const uint4*>(s < KN ? src + 16 * s : rot + 16 * (s - KN));
   }
-  // every live row of the wave sees the keys up to low
+  // every live row of the wave sees the keys up to low, none one past high
   const int low = prior + b.pair0 + 32 * wave;
+  const int high = b.pair0 + 32 * wave < b.count ? min(low + 31, prior + b.count - 1) : -1;
   const bool full = b.pair0 + 32 * wave + 31 < b.count;  // no lane past the last row
   const int sees_all = prior + b.pair0;  // the last key that every row of the block sees
   const float sl2 = scale * kLog2e;
@@ -233,6 +234,9 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
     }
     const int ahead = stage == 0 ? D - 1 : stage - 1;  // of tile ti + D - 1
     const int at = min((ti + D - 1) * KT, last);
+    each<NC>([&](auto j) MX_LAMBDA { copy(at, ahead, j); });
+    stage = stage == D - 1 ? 0 : stage + 1;
+    if (tile > high) continue;  // uniform: nothing here that a row of this wave sees
     enter(stage_at);
     floatx16_t sc[KB];
 #pragma unroll
@@ -241,16 +245,12 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
       for (int r = 0; r < 16; ++r) sc[k][r] = 0.0f;
     uint4 a[R];
     each<R>([&](auto i) MX_LAMBDA { a[i] = k_operand(i); });
-    // Issued together the copies hold up every wave of the workgroup at once, so they are spread over the
-    // products.
     each<KS * KB>([&](auto i) MX_LAMBDA {
       __builtin_amdgcn_sched_barrier(0);
       sc[i % KB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[i % R]),
                                                            __builtin_bit_cast(bf16x8_t, qb[i / KB]),
                                                            sc[i % KB], 0, 0, 0);
       if constexpr (i + R < KS * KB) a[i % R] = k_operand(i + R);
-      constexpr int first = i * NC / (KS * KB), end = (i + 1) * NC / (KS * KB);
-      each<end - first>([&](auto j) MX_LAMBDA { copy(at, ahead, first + j); });
     });
     __builtin_amdgcn_sched_barrier(0);
     each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(i); });
@@ -304,7 +304,6 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
       }
     });
     __builtin_amdgcn_sched_barrier(0);
-    stage = stage == D - 1 ? 0 : stage + 1;
   }
   copies_done<0>();  // none lands in LDS that is no longer this workgroup's
   if (!alive) return;

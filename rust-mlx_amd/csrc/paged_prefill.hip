@@ -45,6 +45,7 @@ using namespace pg;
 
 constexpr int NW = 4;            // waves of a workgroup
 constexpr int D = 2;             // stages of a tile in LDS
+constexpr int kPairs = PageDims::kPairs;
 static_assert(kPairs == 32 * NW, "32 pairs a wave");
 
 // Keys of a tile: two stages of K and V fit twice into a compute unit's LDS.
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   const int group = d.heads / d.kv_heads;
   const PromptPlan plan = prompt_plan(starts, lens, d, rows, group);
   const int splits = plan.splits;
-  const Item it = item_of(blockIdx.x, plan, d.kv_heads);
+  const Item it = item_of<PageDims>(blockIdx.x, plan, d.kv_heads);
   if (it.split >= splits) return;
   const int kvh = it.kvh, split = it.split;
   Block b;

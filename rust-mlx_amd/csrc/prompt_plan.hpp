@@ -9,7 +9,7 @@
 namespace mx {
 namespace pg {
 
-constexpr int kPairs = 128;  // of a workgroup
+// Of the description Dims: kPairs, the pairs of a workgroup, and kAtOnce, the workgroups that run at once.
 
 // Lambdas that hold registers by reference: a call would put them into memory.
 #define MX_LAMBDA __attribute__((always_inline))
@@ -58,18 +58,18 @@ __device__ __forceinline__ Rows rows_of(const int32_t* __restrict__ starts,
   }
   return r;
 }
+template <class Dims>
 __device__ __forceinline__ int blocks_of(const Rows& r, int group) {
-  return int((int64_t(r.count) * group + kPairs - 1) / kPairs);
+  return int((int64_t(r.count) * group + Dims::kPairs - 1) / Dims::kPairs);
 }
 
 // How many workgroups share the keys of a query block, with `blocks` of them: as many as bring the
-// launch to two workgroups a compute unit, each with at least four tiles of the longest possible
-// context; in eights with the kv heads where that is possible, for whole XCDs (512 rows on 12001
+// launch to what runs at once, each with at least four tiles of the longest possible context; in eights with the kv heads where that is possible, for whole XCDs (512 rows on 12001
 // keys, two kv heads: 8 splits 126 us, 7 splits 138).  At most 64, never more with more blocks.
 template <class Dims>
 __host__ __device__ __forceinline__ int splits_of(int64_t blocks, const Dims& d) {
   const int64_t all = blocks * d.kv_heads, room = longest_context(d) / 256;
-  int s = all > 256 ? 1 : 512 / int(all < 1 ? 1 : all);
+  int s = all > Dims::kAtOnce / 2 ? 1 : Dims::kAtOnce / int(all < 1 ? 1 : all);
   s = s > room ? int(room) : s;
   s = s > 64 ? 64 : s < 1 ? 1 : s;
   const int low = d.kv_heads & -d.kv_heads, step = low >= 8 ? 1 : 8 / low;  // powers of two
@@ -79,7 +79,7 @@ __host__ __device__ __forceinline__ int splits_of(int64_t blocks, const Dims& d)
 // The fewest blocks that a call of so many rows is laid out for.
 template <class Dims>
 __host__ __device__ __forceinline__ int64_t least_blocks(int rows, const Dims& d) {
-  return (int64_t(rows) * (d.heads / d.kv_heads) + kPairs - 1) / kPairs;
+  return (int64_t(rows) * (d.heads / d.kv_heads) + Dims::kPairs - 1) / Dims::kPairs;
 }
 
 // What follows from all sequences' rows, formed by every wave: the number of query blocks (sequences
@@ -96,7 +96,7 @@ __device__ __forceinline__ PromptPlan prompt_plan(const int32_t* __restrict__ st
   const int lane = threadIdx.x & 63;
   PromptPlan p;
   p.r0 = rows_of(starts, lens, d, rows, lane);
-  int n = blocks_of(p.r0, group);
+  int n = blocks_of<Dims>(p.r0, group);
   constexpr int AHEAD = 8;  // loads on their way; past the last sequence there are no rows
   const int all = min(starts[d.sequences], rows);
   int done = __builtin_amdgcn_readlane(p.r0.first + p.r0.count, 63);  // rows of the sequences so far
@@ -110,7 +110,7 @@ __device__ __forceinline__ PromptPlan prompt_plan(const int32_t* __restrict__ st
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int first = min(max(at[i], 0), rows);
-      n += blocks_of({first, max(min(to[i], rows) - first, 0), 0}, group);
+      n += blocks_of<Dims>({first, max(min(to[i], rows) - first, 0), 0}, group);
     }
     done = __builtin_amdgcn_readlane(to[AHEAD - 1], 63);
   }
@@ -132,7 +132,7 @@ __device__ __forceinline__ bool find_block(const PromptPlan& p, const int32_t* _
   int before = 0;
   for (int s0 = 0; s0 < d.sequences; s0 += 64) {
     const Rows r = s0 == 0 ? p.r0 : rows_of(starts, lens, d, rows, s0 + lane);
-    const int sum = wave_scan(blocks_of(r, group));
+    const int sum = wave_scan(blocks_of<Dims>(r, group));
     const uint64_t past = __ballot(before + sum > want);
     if (past) {
       const int f = __builtin_ctzll(past);
@@ -140,7 +140,7 @@ __device__ __forceinline__ bool find_block(const PromptPlan& p, const int32_t* _
       out->seq = __builtin_amdgcn_readfirstlane(s0 + f);
       out->first = __builtin_amdgcn_readlane(r.first, f);
       out->count = __builtin_amdgcn_readlane(r.count, f);
-      out->pair0 = (before + __builtin_amdgcn_readlane(sum, f) - 1 - want) * kPairs;
+      out->pair0 = (before + __builtin_amdgcn_readlane(sum, f) - 1 - want) * Dims::kPairs;
       out->len = __builtin_amdgcn_readlane(r.len, f);
       return true;
     }
@@ -168,6 +168,7 @@ __host__ __device__ __forceinline__ int items_of(int kv_heads, int splits) {
 // those take the blocks from the last one on: a sequence's blocks have fewer and fewer keys, and
 // so a long one shares its unit with a short one (four prompts of up to 2047 rows on up to 3001,
 // e4m3: 144 us against 152).
+template <class Dims>
 __device__ __forceinline__ Item item_of(int id, const PromptPlan& p, int kv_heads) {
   const int pairs = kv_heads * p.splits, a_block = items_of(kv_heads, p.splits);
   const bool xcd = by_xcd(kv_heads, p.splits);
@@ -176,7 +177,7 @@ __device__ __forceinline__ Item item_of(int id, const PromptPlan& p, int kv_head
   int block = xcd ? j / each : id / pairs;
   if (block >= p.blocks) return Item{block, 0, p.splits};  // past the last block: none
   const int64_t all = int64_t(p.blocks) * a_block;
-  if (all > 256 && all <= 512) {
+  if (all > 256 && all <= Dims::kAtOnce) {
     const int first = 256 / a_block;
     if (block >= first) block = p.blocks - 1 - (block - first);
   }
@@ -198,6 +199,7 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(
   const int kvh = blockIdx.x % d.kv_heads;
   const PromptPlan plan = prompt_plan(starts, lens, d, rows, group);
   const int splits = plan.splits;
+  if (splits == 1) return;  // the rows lie in more blocks than they could have
   const int all = rows * group, first = int(blockIdx.x / d.kv_heads) * kJoinPairs;  // below 2^31
   for (int i = first + wave; i < min(first + kJoinPairs, all); i += 4) {
     const int row = i / group, head = kvh * group + i - row * group;
@@ -214,8 +216,8 @@ __global__ __launch_bounds__(256) void prefill_join_kernel(
       }
     }
     if (pairs == 0) continue;  // a row outside every sequence
-    const int pair0 = (token * group + head - kvh * group) / kPairs * kPairs;  // of its block
-    const int last_pair = min(pair0 + kPairs, pairs) - 1;
+    const int pair0 = (token * group + head - kvh * group) / Dims::kPairs * Dims::kPairs;  // of its block
+    const int last_pair = min(pair0 + Dims::kPairs, pairs) - 1;
     const int kall = max(prior + last_pair / group + 1, 0);
     const int tiles = (kall + KT - 1) / KT, per = (tiles + splits - 1) / splits;
     if (per >= tiles) continue;  // one split (or none) wrote the result
@@ -264,10 +266,10 @@ template <class Dims>
 size_t prompt_workspace(int rows, int head_dim, const Dims& d) {
   const int64_t group = d.heads / d.kv_heads;
   int64_t most = 0;  // rows times splits
-  for (int64_t b = 1; (b - 1) * kPairs < rows * group; ++b) {
+  for (int64_t b = 1; (b - 1) * Dims::kPairs < rows * group; ++b) {
     const int splits = splits_of(b, d);
     if (splits == 1) break;  // and so for more blocks
-    const int64_t r = b * kPairs / group < rows ? b * kPairs / group : rows;  // the last row with b blocks
+    const int64_t r = b * Dims::kPairs / group < rows ? b * Dims::kPairs / group : rows;  // the last row with b blocks
     most = r * splits > most ? r * splits : most;
   }
   return size_t(most) * d.heads * (head_dim + 2) * 4;
@@ -276,11 +278,11 @@ size_t prompt_workspace(int rows, int head_dim, const Dims& d) {
 template <class Dims>
 int64_t prompt_grid(int rows, const Dims& d) {
   // Workgroups for any number of blocks that starts may give: the number itself is the kernel's to
-  // find.  Beyond 256 blocks of a kv head nothing is split, and more blocks have more workgroups.
+  // find.  Beyond kAtOnce / 2 blocks and kv heads nothing is split, and more blocks have more workgroups.
   const int64_t group = d.heads / d.kv_heads, least = least_blocks(rows, d);
-  const int64_t most = int64_t(rows) * group / kPairs + (d.sequences < rows ? d.sequences : rows);
+  const int64_t most = int64_t(rows) * group / Dims::kPairs + (d.sequences < rows ? d.sequences : rows);
   int64_t grid = most * items_of(d.kv_heads, splits_of(most, d));
-  for (int64_t b = least; b < most && b * d.kv_heads <= 256; ++b) {
+  for (int64_t b = least; b < most && b * d.kv_heads <= Dims::kAtOnce / 2; ++b) {
     const int64_t n = b * items_of(d.kv_heads, splits_of(b, d));
     grid = n > grid ? n : grid;
   }
