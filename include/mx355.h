@@ -652,9 +652,11 @@ mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t 
  *   scales  fp32 [pages][page_size], of MX_DT_F8E4M3 (ignored for MX_DT_BF16):
  *           the value is the stored number times its position's scale
  * Pages, tables, sequences, padding rows and workspaces are those of the paged
- * cache.  What a row does not see may hold anything.  A position with an
- * infinite or NaN value makes what attention gives the rows that see it NaN, in
- * the dims of that value at least.
+ * cache.  What a row does not see may hold anything.  Infinite and NaN values
+ * that it sees act as in the formulas: a NaN or +infinite score makes the row's
+ * result NaN throughout; a score of -inf has the weight 0, which leaves the other
+ * positions' result but for NaN in the dims where that position's value is
+ * infinite; an infinite or NaN value makes its dim infinite or NaN.
  *
  * 1..128 heads; latent_dim 256 or 512; rope_dim 64; nope_dim and v_dim 64 or 128
  * and the same; page_size 16, 32, 64, 128 or 256; at most 2^30 positions a
@@ -711,12 +713,15 @@ mx_status mx_attn_latent_read(const void* cache, const float* scales, int32_t ro
  * out [rows, heads, latent_dim]); q_rope [rows, heads, rope_dim] as
  * mx_attn_latent_append gives it:
  *   out[r, h] = bf16(softmax((q_latent c^T + q_rope k^T) scale) c)
- * with scale 0 meaning 1 / sqrt(nope_dim + rope_dim).  P is rounded to bf16 for
- * the second product.  Rows without positions, padding rows, lengths past the
+ * with scale 0 meaning 1 / sqrt(nope_dim + rope_dim).  For the second product P
+ * has 16 bits (two bf16 parts) with up to 64 heads and is rounded to bf16 with
+ * more.  Rows without positions, padding rows, lengths past the
  * table, the dependence on the other rows' lengths and the workspace as
  * mx_attn_paged_decode's; workspace: mx_attn_latent_decode_workspace_bytes(rows,
- * dims) bytes, which do for fewer rows too.  A sequence's several new tokens (as a
- * draft's) are rows of that sequence with the lengths of their own positions. */
+ * dims) bytes, which do for fewer rows too.  rows times (table_width * page_size /
+ * 32 + 8) must be at most 2^30 (MX_EUNSUPPORTED otherwise).  A sequence's several
+ * new tokens (as a draft's) are rows of that sequence with the lengths of their
+ * own positions. */
 size_t mx_attn_latent_decode_workspace_bytes(int32_t rows, const mx_latent_dims* dims);
 mx_status mx_attn_latent_decode(const uint16_t* q_latent, const uint16_t* q_rope, int32_t rows,
                                 const int32_t* seqs, const int32_t* lens, const int32_t* table,

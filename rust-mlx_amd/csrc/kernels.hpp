@@ -254,8 +254,6 @@ struct LatentDims {
   int page_log2, pages, sequences, table_width;  // as in PageDims
   bool f8;
   int64_t page_stride;
-  static constexpr int kv_heads = 1;  // all heads read the same positions
-  static constexpr bool gated = false;
 };
 // What attention with keys and values of every head knows of them: each head is a kv head.
 struct LatentPromptDims {

@@ -37,8 +37,6 @@ using namespace pg;
 
 constexpr int KT = 32;   // positions of a tile
 constexpr int DR = 64;   // rope_dim
-typedef short shortx4_t __attribute__((ext_vector_type(4)));
-typedef int intx2_t __attribute__((ext_vector_type(2)));
 
 // By the number of head waves (of 32 heads each): waves that share their heads; workgroups that share a
 // compute unit; stages of a tile in LDS.
@@ -68,21 +66,6 @@ template <bool F8>
 __device__ __forceinline__ int swizzle(int row) {
   return F8 ? ((row >> 1) & 2) ^ ((row >> 3) & 2) ^ ((row >> 1 ^ row >> 3) & 1)
             : (row & 2) << 1 | (row >> 1 & 2) | (row >> 3 & 1);
-}
-template <class T>
-__device__ __forceinline__ T lds_read(uint32_t at) {
-  return *reinterpret_cast<__attribute__((address_space(3))) const T*>(at);
-}
-// Of sixteen lanes, four rows of sixteen values (lane j: four values of row j / 4 at `at`), lane j gets
-// the four rows' value j.
-__device__ __forceinline__ uint2 lds_read_tr16(uint32_t at) {
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       reinterpret_cast<__attribute__((address_space(3))) shortx4_t*>(at)));
-}
-// The same of bytes: eight rows of sixteen (lane j: eight of row j / 2).
-__device__ __forceinline__ uint2 lds_read_tr8(uint32_t at) {
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                       reinterpret_cast<__attribute__((address_space(3))) intx2_t*>(at)));
 }
 // Four bytes a lane from memory to LDS, lane l's to lds + 4 l (as copy_to_lds).
 __device__ __forceinline__ void copy4_to_lds(const void* src, uint32_t lds) {

@@ -30,7 +30,6 @@ static_assert(kRows == 32 * NW, "32 rows a wave");
 constexpr int KT = 64;  // keys of a tile
 constexpr int D = 3;    // stages of a tile in LDS
 constexpr int DR = 64;  // rope_dim
-typedef short shortx4_t __attribute__((ext_vector_type(4)));
 
 // A stage holds blocks of 64 values of its keys' rows: a head's keys and values, then the rotary keys.
 constexpr int kBlock = KT * 128;
@@ -43,17 +42,6 @@ constexpr int stage_bytes() {
 // 64 banks twice, nor do four pieces of four rows, as the transposed reads take them.
 __device__ __forceinline__ int swizzle(int row) {
   return (row & 2) << 1 | (row >> 1 & 2) | (row >> 3 & 1);
-}
-__device__ __forceinline__ uint4 lds_read16(uint32_t at) {
-  typedef uint32_t vec __attribute__((ext_vector_type(4)));
-  const vec v = *reinterpret_cast<__attribute__((address_space(3))) const vec*>(at);
-  return make_uint4(v.x, v.y, v.z, v.w);
-}
-// Of sixteen lanes, four rows of sixteen values (lane j: four values of row j / 4 at `at`), lane j gets
-// the four rows' value j.
-__device__ __forceinline__ uint2 lds_read_tr(uint32_t at) {
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       reinterpret_cast<__attribute__((address_space(3))) shortx4_t*>(at)));
 }
 
 template <int HD>  // nope_dim and v_dim
@@ -157,12 +145,13 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
   };
   auto k_operand = [&](int i) MX_LAMBDA {
     const int s = i / KB;
-    return lds_read16(kb[s & 3] + ((s < KN ? s >> 2 : NB - 1) * kBlock + i % KB * (32 * 128)));
+    typedef uint32_t vec __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint4, lds_read<vec>(kb[s & 3] + ((s < KN ? s >> 2 : NB - 1) * kBlock + i % KB * (32 * 128))));
   };
   auto v_operand = [&](int i) MX_LAMBDA {
     const int n = i % ND, s = i / ND;
     const uint32_t off = (n >> 1) * kBlock + s * (16 * 128);
-    const uint2 x = lds_read_tr(vb[n & 1][0] + off), y = lds_read_tr(vb[n & 1][1] + off);
+    const uint2 x = lds_read_tr16(vb[n & 1][0] + off), y = lds_read_tr16(vb[n & 1][1] + off);
     return make_uint4(x.x, x.y, y.x, y.y);
   };
 

@@ -603,7 +603,7 @@ int paged_decode(const uint16_t* q, const uint16_t* qkv, int64_t qkv_stride, int
   int2* row_chunks = reinterpret_cast<int2*>(ml_part + items * group * 2);
   const int target = decode_target(d);
 #define MX_JOIN(HH, DW, NW)                                                                      \
-  hipLaunchKernelGGL((decode_join_kernel<HH, DW, NW, PageDims>), dim3(unsigned(joins * (HH / DW))),        \
+  hipLaunchKernelGGL((decode_join_kernel<HH, DW, NW>), dim3(unsigned(joins * (HH / DW))),        \
                      dim3(64 * NW), 0, s, qkv, qkv_stride, rows, seqs, lens,                     \
                      d.f8 ? v_scale : nullptr, d, row_chunks, o_part, ml_part, out)
 #define MX_DECODE(HH, FF)                                                                        \

@@ -82,6 +82,24 @@ __device__ __forceinline__ void copies_done() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
+template <class T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+  return *reinterpret_cast<__attribute__((address_space(3))) const T*>(at);
+}
+// Of sixteen lanes, four rows of sixteen 16-bit values (lane j: four values of row j / 4 at `at`), lane j
+// gets the four rows' value j.
+__device__ __forceinline__ uint2 lds_read_tr16(uint32_t at) {
+  typedef short vec __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       reinterpret_cast<__attribute__((address_space(3))) vec*>(at)));
+}
+// The same of bytes: eight rows of sixteen (lane j: eight of row j / 2).
+__device__ __forceinline__ uint2 lds_read_tr8(uint32_t at) {
+  typedef int vec __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                       reinterpret_cast<__attribute__((address_space(3))) vec*>(at)));
+}
+
 // Sums over groups of N neighbouring lanes (8, 16 or 32), in every lane of the group.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
@@ -168,9 +186,8 @@ __device__ __forceinline__ int units_of(int len, int unit) {
 struct KeyPlan {
   int chunk_units, len0;
 };
-template <class Dims>
 __device__ __forceinline__ KeyPlan key_plan(const int32_t* seqs, const int32_t* lens,
-                                                const Dims& d, int rows, int unit, int target) {
+                                            const PageDims& d, int rows, int unit, int target) {
   const int lane = threadIdx.x & 63;
   KeyPlan p;
   p.len0 = row_len(seqs, lens, d, lane, rows);
@@ -195,9 +212,8 @@ __device__ __forceinline__ KeyPlan key_plan(const int32_t* seqs, const int32_t* 
 struct Chunk {
   int row, index, chunks, before, len;
 };
-template <class Dims>
 __device__ __forceinline__ Chunk find_chunk(const KeyPlan& plan, const int32_t* seqs,
-                                            const int32_t* lens, const Dims& d, int rows, int unit,
+                                            const int32_t* lens, const PageDims& d, int rows, int unit,
                                             int want) {
   const int lane = threadIdx.x & 63, cu = plan.chunk_units;
   Chunk ch = {-1, 0, 0, 0, 0};
@@ -224,11 +240,11 @@ constexpr int kDecodeMaxChunks = 2048 + 1;  // of one row: twice decode_target a
 // Joins the chunks of DW dims of one (row, head) in a fixed order; rows without
 // keys become 0, rows of one chunk are done already.  Each wave takes every NW-th
 // chunk, eight at a time, whose sums are on their way while the weights form.
-template <int HD, int DW, int NW, class Dims>
+template <int HD, int DW, int NW>
 __global__ __launch_bounds__(64 * NW) void decode_join_kernel(
     const uint16_t* __restrict__ qkv, int64_t qkv_stride, int rows,
     const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
-    const float* __restrict__ v_scale, Dims d, const int2* __restrict__ row_chunks,
+    const float* __restrict__ v_scale, PageDims d, const int2* __restrict__ row_chunks,
     const float* __restrict__ o_part, const float* __restrict__ ml_part,
     uint16_t* __restrict__ out) {
   constexpr int DB = HD / DW, DPL = DW / 64;

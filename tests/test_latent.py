@@ -127,3 +127,13 @@ def test_prompt_workspace_never_falls(mx, heads, nope):
     assert f(1 << 20, 1 << 20, C.byref(d)) <= 1024 * 128 * (nope + 2) * 4
     idle = dims(mx, heads=heads, nope_dim=nope, v_dim=nope, sequences=5000)  # sequences without rows
     assert f(40, 3000, C.byref(d)) == f(40, 3000, C.byref(idle))
+
+
+def test_more_tiles_than_are_counted_are_refused(mx):
+    """Rows times the tiles that the table allows each, of 32 positions and 8 more a row, must not pass 2^30."""
+    wide = dims(mx, table_width=1 << 26)                  # 2^30 positions a row: 2^25 tiles
+    for rows in (32, 33, 1 << 20):
+        assert calls(mx, wide, rows=rows)["decode"]() == mx.MX_EUNSUPPORTED, rows
+        assert b"mx_attn_latent_decode: " in mx.lib.mx_last_error()
+    narrow = dims(mx, table_width=2)                      # one tile
+    assert calls(mx, narrow, rows=(1 << 30) // 9 + 1)["decode"]() == mx.MX_EUNSUPPORTED

@@ -13,7 +13,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from latent_ref import ROPE, Latent, attend, attend_formed
+from latent_ref import ROPE, Latent, attend, attend_formed, softmax_rows
 from paged_ref import E4M3, Graph, bf, to_bf
 
 pytestmark = pytest.mark.gpu
@@ -88,6 +88,93 @@ def test_decode_long_rows_split_and_joined(mx, heads, f8):
         lens = np.linspace(1, context, rows).astype(np.int32)[::-1]
         got = run_decode(mx, c, ql, qr, lens, seqs=np.zeros(rows))
         close(got, *expected(c, ql, qr, lens, [0] * rows))
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("heads", [3, 40, 100])
+def test_decode_shares_of_many_tiles(mx, heads, f8):
+    """Workgroups that walk more tiles than they hold page ids of at once, of pages that a tile lies in and of pages
+    of half a tile."""
+    rows, context = 280, 2400
+    for page in (16, 64):
+        say("many tiles", heads, page, f8)
+        c = Latent(mx, heads, 512, page, [context], f8, seed=22 + page)
+        ql, qr = queries(np.random.default_rng(23), rows, heads, 512)
+        lens = context - 3 * (np.arange(rows) % 7)
+        got = run_decode(mx, c, ql, qr, lens, seqs=np.zeros(rows))
+        x, _ = c.values(0, context)
+        for r in range(0, rows, 1 if heads < 10 else 13):
+            k = x[:lens[r]]
+            p = softmax_rows(np.concatenate([F(ql[r]), F(qr[r])], 1) @ k.T * 192 ** -0.5)
+            close(got[r], p @ k[:, :512], p @ np.abs(k[:, :512]))
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("heads,latent", [(20, 512), (50, 256), (128, 512)])
+def test_decode_shares_of_many_rows(mx, heads, latent, f8):
+    """Hundreds of short rows, several to a workgroup, with empty and padding rows between them and behind."""
+    rows, contexts = 700, [70, 1, 33, 5, 64]
+    say("many rows", heads, latent, f8)
+    c = Latent(mx, heads, latent, 16, contexts, f8, seed=24)
+    rng = np.random.default_rng(25)
+    seqs = rng.integers(-1, len(contexts) + 1, rows)
+    pad = (seqs < 0) | (seqs >= len(contexts))
+    most = np.array(contexts + [9, 9])[seqs]
+    lens = rng.integers(0, most + 1)
+    lens[rows // 2:rows // 2 + 130] = 0                   # more than two rounds of 64 without any
+    lens[5], seqs[-3:], pad[-3:] = -7, -1, True
+    ql, qr = queries(rng, rows, heads, latent)
+    before = rng.integers(0, 1 << 15, ql.shape).astype(np.uint16)
+    got = run_decode(mx, c, ql, qr, lens, seqs, out=before)
+    assert (got[pad] == before[pad]).all()
+    x = [c.values(i, n)[0] for i, n in enumerate(contexts)]
+    for r in np.flatnonzero(~pad):
+        if lens[r] <= 0:
+            assert (got[r] == 0).all()
+            continue
+        k = x[seqs[r]][:lens[r]]
+        p = softmax_rows(np.concatenate([F(ql[r]), F(qr[r])], 1) @ k.T * 192 ** -0.5)
+        close(got[r], p @ k[:, :latent], p @ np.abs(k[:, :latent]))
+
+
+def test_decode_replayed_between_other_calls(mx):
+    """Two captured calls that share one workspace, replayed in turn with eager calls of other rows between them: each
+    gives its eager bits."""
+    heads, f8 = 100, False
+    say("replays")
+    c = Latent(mx, heads, 512, 32, [900, 400], f8, seed=26)
+    d, stream = c.dims(), C.c_void_p()
+    mx.check(mx.lib.mx_stream_create(C.byref(stream)))
+    s = stream.value
+    ws = mx.DeviceArray((mx.lib.mx_attn_latent_decode_workspace_bytes(9, C.byref(d)),), np.uint8)
+    calls = []
+    for rows, lens in ((9, [900, 3, 0, 500, 64, 32, 31, 900, 17]), (2, [400, 900]), (5, [1, 33, 900, 900, 400])):
+        ql, qr = queries(np.random.default_rng(27 + rows), rows, heads, 512)
+        seqs = [0 if n > 400 else 1 for n in lens]
+        dev = [up(mx, a) for a in (ql, qr, np.array(seqs, np.int32), np.array(lens, np.int32))]
+        out = mx.DeviceArray(ql.shape, np.uint16)
+
+        def call(dev=dev, out=out, rows=rows):
+            mx.check(mx.lib.mx_attn_latent_decode(dev[0].ptr, dev[1].ptr, rows, dev[2].ptr, dev[3].ptr, c.dtable.ptr,
+                                                  c.dcache.ptr, None, C.byref(d), 0.0, ws.ptr, out.ptr, s))
+        call()
+        mx.check(mx.lib.mx_stream_sync(s))
+        want = out.numpy()
+        close(want, *expected(c, ql, qr, lens, seqs))
+        calls.append((call, out, want))
+    graphs = [Graph(mx, s, call) for call, _, _ in calls[:2]]
+    for _ in range(3):
+        for g, (_, out, want) in zip(graphs, calls):
+            out.upload(np.full(want.shape, 0x1234, np.uint16))
+            g.launch()
+            mx.check(mx.lib.mx_stream_sync(s))
+            assert (out.numpy() == want).all()
+            calls[2][0]()
+            mx.check(mx.lib.mx_stream_sync(s))
+            assert (calls[2][1].numpy() == calls[2][2]).all()
+    for g in graphs:
+        g.close()
+    mx.check(mx.lib.mx_stream_destroy(stream))
 
 
 @pytest.mark.parametrize("f8", [False, True])
