@@ -91,22 +91,22 @@ __global__ __launch_bounds__(kSeg / 8) void control_kernel(const uint16_t* logit
     if (b1 > b0) *reinterpret_cast<uint4*>(entry + i) = make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
-  auto see = [&](int token, int i) {
+  auto see = [&](int token, unsigned i) {  // (unsigned: a step past 2^31 tokens wraps to nothing)
     const unsigned j = unsigned(token) - unsigned(first);
     if (j < unsigned(count)) {
-      if (i < prompt)
+      if (i < unsigned(prompt))
         atomicOr(counts + place_of<kSeg>(j), kInPrompt);
       else
         atomicAdd(counts + place_of<kSeg>(j), 1u);
     }
   };
-  const int whole = len & ~3;
+  const unsigned whole = len & ~3;
   constexpr int A = 4;  // reads of a thread on their way
-  for (int base = 0; base < whole; base += 4 * kThreads * A) {  // uniform, and so is each read's number
+  for (unsigned base = 0; base < whole; base += 4 * kThreads * A) {  // uniform, and so is each read's number
     tokens4 k[A];
 #pragma unroll
     for (int e = 0; e < A; ++e) {
-      const int i = base + 4 * (t + kThreads * e);
+      const unsigned i = base + 4 * (t + kThreads * e);
       k[e] = tokens4{-1, -1, -1, -1};
       if (i < whole) k[e] = *reinterpret_cast<const tokens4*>(tokens + i);
     }
@@ -117,9 +117,9 @@ __global__ __launch_bounds__(kSeg / 8) void control_kernel(const uint16_t* logit
         for (int j = 0; j < 4; ++j) see(k[e][j], base + 4 * (t + kThreads * e) + j);
       }
   }
-  if (t < len - whole) see(tokens[whole + t], whole + t);
+  if (unsigned(t) < len - whole) see(tokens[whole + t], whole + t);
 #pragma unroll 2
-  for (int i = b0 + t; i < b1; i += kThreads) {
+  for (unsigned i = b0 + t; i < unsigned(b1); i += kThreads) {
     const unsigned j = unsigned(c.bias_tokens[i]) - unsigned(first);
     if (j < unsigned(count)) atomicMax(entry + place_of<kSeg>(j), uint32_t(i - b0) + 1u);
   }
@@ -178,7 +178,7 @@ int logits_control(const uint16_t* logits, int64_t stride, int rows, int n, cons
   // often (64 rows of 151936: 19.5 us, 20.8 with 2048 tokens each, 20.2 with 8192).
 #define MX_CONTROL(SEG)                                                                             \
   {                                                                                                 \
-    const int64_t segs = (n + SEG - 1) / SEG, blocks = rows * segs;                                 \
+    const int64_t segs = (int64_t(n) + SEG - 1) / SEG, blocks = rows * segs;                                 \
     if (blocks > 0x7fffffff) return MX_EUNSUPPORTED;                                                \
     hipLaunchKernelGGL((control_kernel<SEG>), dim3(unsigned(blocks)), dim3(SEG / 8),                \
                        SEG * (c.bias_starts ? 8 : 4), s, logits, stride, n, c, out, out_stride,     \

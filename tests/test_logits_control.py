@@ -29,3 +29,9 @@ def test_what_is_absent_is_not_asked_for(mx):
                 bias_tokens=None, bias_values=None, bias_count=0, rows=0)
     assert call(mx, **none) == mx.MX_OK
     assert call(mx, rows=0, bias_count=0, bias_tokens=None, bias_values=None) == mx.MX_OK
+
+
+def test_more_workgroups_than_a_launch_has_are_refused(mx):
+    """The largest vocabulary too: its segments are counted in 64 bits."""
+    n = (1 << 31) - 1
+    assert call(mx, rows=1 << 20, n=n, stride=n, out_stride=n, mask_stride=1 << 26) == mx.MX_EUNSUPPORTED
