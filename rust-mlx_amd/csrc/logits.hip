@@ -11,8 +11,9 @@
 // its tokens in LDS (whole numbers: the order of the counting does not show), the prompt's occurrences as
 // the top bit, so no table of the vocabulary is kept between steps; then it changes its logits in one
 // pass, eight a thread.  64 rows of 151936 with histories of up to 8192, 300 biases and every second row
-// masked take 19.5 us (2.1 TB/s; 15.5 without histories, 16.6 without changes): chains of dependent reads,
-// counts and barriers, two and a half rounds of workgroups of them, rather than bytes.
+// masked take 17.7 us (2.3 TB/s): chains of dependent reads, counts and barriers, two and a half rounds of
+// workgroups of them, rather than bytes; so the first reads of the history and of the biases do not wait for
+// their numbers (0.8 us).  Two eights of logits a thread, with half the threads, take 23.
 // A token that the biases name twice takes the last entry: the largest index wins, whatever the
 // order.
 #include "kernels.hpp"
@@ -66,6 +67,10 @@ __global__ __launch_bounds__(kSeg / 8) void control_kernel(const uint16_t* logit
     }
   };
   if (!in_place) load();
+  for (int i = 4 * t; i < kSeg; i += 4 * kThreads) {
+    *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
+    if (c.bias_starts) *reinterpret_cast<uint4*>(entry + i) = make_uint4(0, 0, 0, 0);
+  }
   const int state = c.masks ? (c.mask_rows ? c.mask_rows[row] : row) : -1;
   const uint8_t* allowed = unsigned(state) < unsigned(c.mask_states)
                                ? reinterpret_cast<const uint8_t*>(c.masks + state * c.mask_stride) + first / 8
@@ -83,46 +88,54 @@ __global__ __launch_bounds__(kSeg / 8) void control_kernel(const uint16_t* logit
   if (!finite(pres)) pres = 0.0f;
   if (c.tokens && unsigned(seq) >= unsigned(c.sequences)) return;  // a padding row (uniform)
   const int64_t room = c.tokens_stride;
-  const int len = c.tokens ? int(min(int64_t(max(c.lens[seq], 0)), room)) : 0;
-  const int prompt = c.tokens && c.prompt_lens ? min(max(c.prompt_lens[seq], 0), len) : 0;
   const int32_t* tokens = c.tokens + int64_t(seq) * room;
-  for (int i = 4 * t; i < kSeg; i += 4 * kThreads) {
-    *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
-    if (b1 > b0) *reinterpret_cast<uint4*>(entry + i) = make_uint4(0, 0, 0, 0);
-  }
+  // The first of the history and of the biases are asked for before their numbers are known.
+  constexpr int A = 2;  // reads of a thread on their way
+  constexpr unsigned kStep = 4 * kThreads;
+  tokens4 ahead[A];
+  auto fetch = [&](unsigned base, int64_t end) {
+#pragma unroll
+    for (int e = 0; e < A; ++e) {
+      const unsigned i = base + 4 * t + kStep * e;
+      ahead[e] = tokens4{-1, -1, -1, -1};
+      if (i + 4 <= end) ahead[e] = *reinterpret_cast<const tokens4*>(tokens + i);
+    }
+  };
+  if (c.tokens) fetch(0, room);
+  const int b_first = t < b1 - b0 ? c.bias_tokens[b0 + t] : -1;
+  const int len = c.tokens ? int(min(int64_t(max(c.lens[seq], 0)), room)) : 0;
+  const unsigned prompt = c.tokens && c.prompt_lens ? min(max(c.prompt_lens[seq], 0), len) : 0;
   __syncthreads();
-  auto see = [&](int token, unsigned i) {  // (unsigned: a step past 2^31 tokens wraps to nothing)
+  auto see = [&](int token, unsigned i) {
     const unsigned j = unsigned(token) - unsigned(first);
     if (j < unsigned(count)) {
-      if (i < unsigned(prompt))
+      if (i < prompt)
         atomicOr(counts + place_of<kSeg>(j), kInPrompt);
       else
         atomicAdd(counts + place_of<kSeg>(j), 1u);
     }
   };
+  // (unsigned: a step past 2^31 tokens does not turn negative)
   const unsigned whole = len & ~3;
-  constexpr int A = 4;  // reads of a thread on their way
-  for (unsigned base = 0; base < whole; base += 4 * kThreads * A) {  // uniform, and so is each read's number
-    tokens4 k[A];
+  for (unsigned base = 0; base < whole;) {  // uniform
 #pragma unroll
     for (int e = 0; e < A; ++e) {
-      const unsigned i = base + 4 * (t + kThreads * e);
-      k[e] = tokens4{-1, -1, -1, -1};
-      if (i < whole) k[e] = *reinterpret_cast<const tokens4*>(tokens + i);
-    }
+      const unsigned i = base + 4 * t + kStep * e;
+      if (i < whole) {
 #pragma unroll
-    for (int e = 0; e < A; ++e)
-      if (base + 4 * kThreads * e < whole) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) see(k[e][j], base + 4 * (t + kThreads * e) + j);
+        for (int j = 0; j < 4; ++j) see(ahead[e][j], i + j);
       }
+    }
+    base += kStep * A;
+    if (base < whole) fetch(base, whole);
   }
   if (unsigned(t) < len - whole) see(tokens[whole + t], whole + t);
-#pragma unroll 2
-  for (unsigned i = b0 + t; i < unsigned(b1); i += kThreads) {
-    const unsigned j = unsigned(c.bias_tokens[i]) - unsigned(first);
-    if (j < unsigned(count)) atomicMax(entry + place_of<kSeg>(j), uint32_t(i - b0) + 1u);
-  }
+  auto see_bias = [&](int token, unsigned i) {
+    const unsigned j = unsigned(token) - unsigned(first);
+    if (j < unsigned(count)) atomicMax(entry + place_of<kSeg>(j), i + 1);
+  };
+  if (t < b1 - b0) see_bias(b_first, t);
+  for (unsigned i = b0 + t + kThreads; i < unsigned(b1); i += kThreads) see_bias(c.bias_tokens[i], i - b0);
   __syncthreads();
   if (at >= count) return;
   uint32_t cs[8], es[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -175,10 +188,10 @@ __global__ __launch_bounds__(kSeg / 8) void control_kernel(const uint16_t* logit
 int logits_control(const uint16_t* logits, int64_t stride, int rows, int n, const LogitsControls& c,
                    uint16_t* out, int64_t out_stride, hipStream_t s) {
   // Few rows take short segments, for more workgroups; many take long ones, whose histories are read less
-  // often (64 rows of 151936: 19.5 us, 20.8 with 2048 tokens each, 20.2 with 8192).
+  // often (64 rows of 151936 one after another: 18.2 us, 20.0 with 2048 tokens each, 18.7 with 8192).
 #define MX_CONTROL(SEG)                                                                             \
   {                                                                                                 \
-    const int64_t segs = (int64_t(n) + SEG - 1) / SEG, blocks = rows * segs;                                 \
+    const int64_t segs = (int64_t(n) + SEG - 1) / SEG, blocks = rows * segs;                        \
     if (blocks > 0x7fffffff) return MX_EUNSUPPORTED;                                                \
     hipLaunchKernelGGL((control_kernel<SEG>), dim3(unsigned(blocks)), dim3(SEG / 8),                \
                        SEG * (c.bias_starts ? 8 : 4), s, logits, stride, n, c, out, out_stride,     \
