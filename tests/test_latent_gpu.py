@@ -493,6 +493,38 @@ def test_what_later_rows_hold_stays_unseen(mx, heads, nope, count, total):
     assert np.isnan(F(got[row + 30:])).all()
 
 
+@pytest.mark.parametrize("heads,nope", [(3, 128), (2, 64)])
+def test_infinite_values_in_one_sequence_of_many(mx, heads, nope):
+    """An infinite value, NaN and one of each sign, early, late and in one head of a sequence among others, over
+    several blocks of rows and with the keys split: what does not see them keeps its bits, what does has the formula's
+    infinity or NaN in that dim and its other dims within the usual bounds."""
+    new, total = [40, 600, 1, 300, 20], [300, 1900, 700, 300, 20]
+    for count in (5, 2):  # the second: few rows, keys split
+        say("infinite prompts", heads, nope, count)
+        n, t = (new, total) if count == 5 else ([30, 100], [1500, 1300])
+        starts, kv_starts = np.cumsum([0] + n), np.cumsum([0] + t)
+        q, qr, kv, kr = formed(np.random.default_rng(31), starts[-1], kv_starts[-1], heads, nope)
+        base = run_prefill(mx, q, qr, kv, kr, starts, kv_starts, heads, nope)
+        check_prefill(base, q, qr, kv, kr, starts, kv_starts, heads, nope)
+        kv2 = kv.copy()
+        v = kv2.reshape(len(kv), heads, 2 * nope)
+        at = [10, t[1] - 25, t[1] - 5]           # in sequence 1: what every row sees, and what its last rows see
+        v[kv_starts[1] + at[0], 0, nope + 7] = 0xFF80
+        v[kv_starts[1] + at[1], 1, nope + 9] = 0x7F80
+        v[kv_starts[1] + at[2], 1, nope + 9] = 0xFF80
+        got = run_prefill(mx, q, qr, kv2, kr, starts, kv_starts, heads, nope)
+        a, b = starts[1], starts[2]
+        seen = np.arange(t[1] - n[1], t[1])      # a row's own position
+        same = np.ones(got.shape, bool)
+        same[a:b, 0, 7] = False
+        same[a:b, 1, 9] = seen < at[1]
+        assert (F(got[a:b, 0, 7]) == -np.inf).all()
+        late = F(got[a:b, 1, 9])
+        assert (late[(seen >= at[1]) & (seen < at[2])] == np.inf).all() and np.isnan(late[seen >= at[2]]).all()
+        assert (got[same] == base[same]).all()
+        assert (run_prefill(mx, q, qr, kv2, kr, starts, kv_starts, heads, nope) == got).all()
+
+
 @pytest.mark.parametrize("f8", [False, True])
 def test_a_request_from_prompt_to_tokens(mx, f8):
     """The set as it is used, with a model's projections: two prompts enter the cache, the first in two parts (its
