@@ -16,7 +16,7 @@
 // divides takes P before it.
 //
 // The matrix units bound it: 8192 rows of 32 heads take 627 to 669 us from card to card (1.03 to 1.10
-// PFLOP/s), 512 rows of 20 heads on 12001 positions 97 to 101 (six splits, 9 of it the join).  256 rows a
+// PFLOP/s), 512 rows of 20 heads on 12001 positions 97 to 105 (six splits, 9 of it the join).  256 rows a
 // workgroup read each key half as often as 128; with 128 and tiles of 32 keys these took 746 and 113 us.  A
 // tile's copies are all issued at its top: spread over its products they take a quarter longer.
 #include <type_traits>

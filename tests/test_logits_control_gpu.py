@@ -191,3 +191,17 @@ def test_the_same_bits_whatever_the_history_order(mx):
     k["tokens"] = k["tokens"][:, rng.permutation(6000)]
     assert (run(mx, logits, n, np.zeros_like(logits), **k) == first).all()
     check(first, logits, n, np.zeros_like(logits), k)
+
+
+@pytest.mark.parametrize("rows,n", [(5, 3001), (40, 40000)])
+def test_whole_histories_of_every_stride(mx, rows, n):
+    """Histories that fill their row, reach past it (cut), end a token before it or are empty, of lengths around the
+    reads of a workgroup, with more biases a row than it has threads."""
+    rng = np.random.default_rng(33)
+    for stride in (1, 2, 3, 4, 5, 1023, 1025, 2048, 2051, 4096, 4099, 8195, 20000):
+        say("histories", rows, n, stride)
+        logits, k = make(rng, rows, n, n, stride, rows, 900, 2)
+        k["lens"] = np.array([stride, stride + 9, stride - 1, 0, -4], np.int32)[np.arange(rows) % 5]
+        k["seqs"] = rng.permutation(rows).astype(np.int32)
+        before = np.full((rows, n), 0x1234, np.uint16)
+        check(run(mx, logits, n, before, **k), logits, n, before, k)
