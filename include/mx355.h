@@ -656,7 +656,8 @@ mx_status mx_attn_paged_prefill(const uint16_t* q, const uint16_t* qkv, int64_t 
  * that it sees act as in the formulas: a NaN or +infinite score makes the row's
  * result NaN throughout; a score of -inf has the weight 0, which leaves the other
  * positions' result but for NaN in the dims where that position's value is
- * infinite; an infinite or NaN value makes its dim infinite or NaN.
+ * infinite, and zeros where all scores are; an infinite or NaN value makes its dim
+ * infinite or NaN.
  *
  * 1..128 heads; latent_dim 256 or 512; rope_dim 64; nope_dim and v_dim 64 or 128
  * and the same; page_size 16, 32, 64, 128 or 256; at most 2^30 positions a

@@ -162,11 +162,11 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
 
   // A row's weight of 0 must not meet an infinite or NaN value that it does not see.  It would leave NaN in
   // the row's sums, so tiles are taken as they are, and where a sum is not finite all of them are taken once
-  // more, with care.  (With care at once one prompt of 256 rows takes 19.6 us instead of 17.9, nine of up to
-  // 399 rows 26.2 instead of 25.6.)
+  // more, with care, in code of its own, so that the first turn's has the registers.  (With care at once one
+  // prompt of 256 rows takes 19.6 us instead of 17.9, nine of up to 399 rows 26.2 instead of 25.6.)
   float m_run, l_run;
   floatx16_t o[ND];
-  for (bool careful = false;; careful = true) {  // uniform
+  auto walk = [&](auto careful) MX_LAMBDA {
     // (below every score, and finite, so that a masked one's -inf has the weight 0)
     m_run = -__FLT_MAX__, l_run = 0.0f;
 #pragma unroll
@@ -187,54 +187,12 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
       copies_done<(D - 2) * NC>();  // this wave's part of the tile is in LDS ...
       __syncthreads();  // ... and everyone's; the stage of the tile before is free
       const uint32_t stage_at = stage * STAGE;
-      // The careful turn: keys past the last one become 0, in a tile that has any; in one that some rows see
-      // and some do not, infinite and NaN values go to the sums of the rows that see them (they stay infinite or
-      // NaN whatever their weight) and become 0 for the product.
-      auto value_at = [&](int key, int piece) MX_LAMBDA {
-        return lds + stage_at + (HD / 64 + (piece >> 3)) * kBlock + key * 128 +
-               16 * ((piece & 7) ^ swizzle(key));
-      };
-      if (careful && tile + KT - 1 > sees_all) {  // uniform
-        auto odd = [](uint32_t w) MX_LAMBDA {
-          return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-        };
-        bool some = false;
-        for (int i = t; i < KT * HD / 8; i += 64 * NW) {
-          uint4* p = reinterpret_cast<uint4*>(value_at(i / (HD / 8), i % (HD / 8)));
-          if (tile + i / (HD / 8) >= kall) {
-            *p = make_uint4(0, 0, 0, 0);
-          } else {
-            const uint4 v = *p;
-            some |= odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w);
-          }
-        }
-        if (__syncthreads_or(some)) {
-          for (int key = 0; key < KT; ++key) {
-            const bool in = tile + key <= limit;
-            int half = h;  // addresses formed for each key: kept over the keys they would take
-            asm volatile("" : "+v"(half));  // a register for every sum, in the loop over tiles too
-#pragma unroll
-            for (int n = 0; n < ND; ++n)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const int dim = 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
-                const uint16_t v = reinterpret_cast<const uint16_t*>(value_at(key, dim >> 3))[dim & 7];
-                if (in && (v & 0x7f80u) == 0x7f80u) o[n][r] += bf16_to_f32(v);
-              }
-          }
-          __syncthreads();
-          for (int i = t; i < KT * HD; i += 64 * NW) {
-            uint16_t* v = reinterpret_cast<uint16_t*>(value_at(i / HD, i % HD / 8)) + i % 8;
-            if ((*v & 0x7f80u) == 0x7f80u) *v = 0;
-          }
-          __syncthreads();
-        }
-      }
       const int ahead = stage == 0 ? D - 1 : stage - 1;  // of tile ti + D - 1
       const int at = min((ti + D - 1) * KT, last);
       each<NC>([&](auto j) MX_LAMBDA { copy(at, ahead, j); });
       stage = stage == D - 1 ? 0 : stage + 1;
-      if (tile > high) continue;  // uniform: nothing here that a row of this wave sees
+      // uniform: nothing here that a row of this wave sees (the careful turn's barriers are for all waves)
+      if (!careful && tile > high) continue;
       enter(stage_at);
       floatx16_t sc[KB];
 #pragma unroll
@@ -251,7 +209,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
         if constexpr (i + R < KS * KB) a[i % R] = k_operand(i + R);
       });
       __builtin_amdgcn_sched_barrier(0);
-      each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(i); });
+      if (!careful) each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(i); });
       // sc[k][r]: key 32 k + 16 (r / 8) + 8 h + r % 8 of the tile
       if (tile + KT - 1 > low || !full) {
         const int end = limit + 1 - tile - 8 * h;
@@ -276,6 +234,64 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
           for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
         m_run = mn;
       }
+      // The careful turn: keys past the last one become 0, in a tile that has any; in one that some rows see
+      // and some do not, infinite and NaN values go to the sums of the rows that see them (they stay infinite or
+      // NaN whatever their weight, but for that of a score of -inf, which makes NaN of them) and become 0 for the
+      // product.
+      if (careful && tile + KT - 1 > sees_all) {  // uniform
+        auto value_at = [&](int key, int piece) MX_LAMBDA {
+          return lds + stage_at + (HD / 64 + (piece >> 3)) * kBlock + key * 128 +
+                 16 * ((piece & 7) ^ swizzle(key));
+        };
+        auto odd = [](uint32_t w) MX_LAMBDA {
+          return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+        };
+        bool some = false;
+        for (int i = t; i < KT * HD / 8; i += 64 * NW) {
+          uint4* p = reinterpret_cast<uint4*>(value_at(i / (HD / 8), i % (HD / 8)));
+          if (tile + i / (HD / 8) >= kall) {
+            *p = make_uint4(0, 0, 0, 0);
+          } else {
+            const uint4 v = *p;
+            some |= odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w);
+          }
+        }
+        if (__syncthreads_or(some)) {
+          uint32_t counts[KB];  // the row's scores above -inf, a key a bit
+#pragma unroll
+          for (int k = 0; k < KB; ++k) {
+            counts[k] = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              counts[k] |= uint32_t(sc[k][r] != neg_inf()) << (16 * (r >> 3) + 8 * h + (r & 7));
+            counts[k] |= __shfl_xor(counts[k], 32, 64);
+          }
+          for (int key = 0; key < KT; ++key) {
+            const bool in = tile + key <= limit;
+            uint32_t mine = counts[0];
+#pragma unroll
+            for (int k = 1; k < KB; ++k) mine = key >> 5 == k ? counts[k] : mine;
+            const float by = mine >> (key & 31) & 1 ? 1.0f : 0.0f;
+            int half = h;  // addresses formed for each key: kept over the keys they would take
+            asm volatile("" : "+v"(half));  // a register for every sum, in the loop over tiles too
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const int dim = 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
+                const uint16_t v = reinterpret_cast<const uint16_t*>(value_at(key, dim >> 3))[dim & 7];
+                if (in && (v & 0x7f80u) == 0x7f80u) o[n][r] += bf16_to_f32(v) * by;
+              }
+          }
+          __syncthreads();
+          for (int i = t; i < KT * HD; i += 64 * NW) {
+            uint16_t* v = reinterpret_cast<uint16_t*>(value_at(i / HD, i % HD / 8)) + i % 8;
+            if ((*v & 0x7f80u) == 0x7f80u) *v = 0;
+          }
+          __syncthreads();
+        }
+      }
+      if (careful) each<R>([&](auto i) MX_LAMBDA { a[i] = v_operand(i); });  // as they are now
       uint32_t pb[8 * KB];
       auto pair = [&](auto j) MX_LAMBDA {
         constexpr int k = j / 8, r = 2 * (j % 8);
@@ -304,14 +320,14 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
       __builtin_amdgcn_sched_barrier(0);
     }
     copies_done<0>();  // none lands in LDS that is no longer this workgroup's, or the next turn's
-    if (careful) break;
-    float most = 0.0f;
+  };
+  walk(std::false_type{});
+  float most = 0.0f;
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
+  for (int n = 0; n < ND; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) most += o[n][r] * 0.0f;  // NaN of what is not finite
-    if (!__syncthreads_or(alive && !(most == 0.0f))) break;
-  }
+    for (int r = 0; r < 16; ++r) most += o[n][r] * 0.0f;  // NaN of what is not finite
+  if (__syncthreads_or(alive && !(most == 0.0f))) walk(std::true_type{});
   if (!alive) return;
   l_run += __shfl_xor(l_run, 32, 64);
   const int64_t at = qrow * d.heads + head;
