@@ -689,7 +689,13 @@ typedef struct mx_latent_dims {
  * scales (a position with an infinite value reads as NaN throughout).  A row
  * whose sequence is not in [0, sequences) is padding: nothing of it is written; a
  * position outside the table writes q_rope only.  Rows must not name the same
- * position twice.  The latent form of mx_attn_paged_append. */
+ * position twice.  The latent form of mx_attn_paged_append.
+ * Norm weights are the zero-centred ones of the q and k norms.  Of a model whose
+ * weights w are plain, take a norm of zeros (the latent normalised alone, NULL is
+ * not that) and multiply w into the products that take the latents, the keys' and
+ * the values': w - 1 in bf16 would lose the bits of a small w.  Rotary pairs are
+ * (i, i + rope_dim / 2); of a model whose pairs are (2 i, 2 i + 1), project the
+ * rotary values of x and q in the order 0, 2, .., 1, 3, .. */
 mx_status mx_attn_latent_append(const uint16_t* x, int64_t x_stride, const uint16_t* q,
                                 int64_t q_stride, int32_t rows, const int32_t* seqs,
                                 const int32_t* pos, const int32_t* rope_pos,
