@@ -26,10 +26,16 @@
 // A row whose tiles meet several workgroups' shares leaves partials in fp32, which a second launch joins in
 // order.
 //
-// Memory bounds it.  64 rows of 128 heads on up to 8192 positions: 121 us, of which the tiles (298 MB) take
-// about 63, q (147 KB) and sums (256 KB) of each workgroup's pieces 37, and the join 20.  40 rows of 20 heads
-// on up to 12001 of e4m3: 59 us (145 MB; without either product three quarters of that).  One row of 16 heads
-// on 60001: 26 us, 6 of them the join.
+// 64 rows of 128 heads on up to 8192 positions: 118 to 123 us, of which the tiles (298 MB, memory's bound) take
+// about 63, the rows' beginnings and ends in each workgroup 37, and the join 20.  A piece's beginning and end
+// move 147 KB of q and 256 KB of sums, but they are a chain too: with a latent of 512 and more than 64 heads a
+// wave's q and sums leave too few registers, so 16 are kept in scratch memory (of e4m3 11), whose reloads between
+// the first tiles' copies wait for these, and the last six of q's 18 loads follow one after another.  Forms with
+// fewer heads or a latent of 256 keep everything in registers.  40 rows of 20 heads on up to 12001 of e4m3: 58 us
+// (145 MB; without either product three quarters of that).  One row of 16 heads on 60001: 26 us, 6 of them the
+// join.
+//
+// Heads are taken in whole 32s, and past 64 in whole 128s: 65 heads compute as 128 do.
 #include <type_traits>
 
 #include "prompt_plan.hpp"
@@ -571,7 +577,8 @@ __global__ __launch_bounds__(EL * G) void join_kernel(const int32_t* __restrict_
 }
 
 int head_waves(const LatentDims& d) { return d.heads <= 32 ? 1 : d.heads <= 64 ? 2 : 4; }
-// The fewest tiles of a share: below, joining partials (heads times latent_dim of fp32) costs more.
+// The fewest tiles of a share: below, joining partials (heads times latent_dim of fp32) costs more.  Set where all
+// compute units have work; one row of 128 heads on 1000 positions takes 4 of them, on 8192 32.
 int least_tiles(const LatentDims& d) { return d.heads > 64 ? 8 : 4; }
 // The most pieces of rows: a workgroup's and a row's end each begin one.
 int64_t decode_pieces(int rows, const LatentDims& d) {

@@ -15,8 +15,8 @@
 // P is rounded to bf16 for the product, each p by at most 2^-8 of itself, as the output is; the sum that
 // divides takes P before it.
 //
-// The matrix units bound it: 8192 rows of 32 heads take 627 to 669 us from card to card (1.03 to 1.10
-// PFLOP/s), 512 rows of 20 heads on 12001 positions 97 to 105 (six splits, 9 of it the join).  256 rows a
+// The matrix units bound it: 8192 rows of 32 heads take 622 to 675 us from card to card (1.02 to 1.11
+// PFLOP/s), 512 rows of 20 heads on 12001 positions 96 to 105 (six splits, 9 of it the join).  256 rows a
 // workgroup read each key half as often as 128; with 128 and tiles of 32 keys these took 746 and 113 us.  A
 // tile's copies are all issued at its top: spread over its products they take a quarter longer.
 #include <type_traits>
@@ -162,8 +162,8 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_kernel(
 
   // A row's weight of 0 must not meet an infinite or NaN value that it does not see.  It would leave NaN in
   // the row's sums, so tiles are taken as they are, and where a sum is not finite all of them are taken once
-  // more, with care, in code of its own, so that the first turn's has the registers.  (With care at once one
-  // prompt of 256 rows takes 19.6 us instead of 17.9, nine of up to 399 rows 26.2 instead of 25.6.)
+  // more, with care, in code of its own, so that the first turn's has the registers.  (One prompt of 256 rows
+  // takes 17.5 us; 17.9 with one loop for both turns, 19.6 with care at once.)
   float m_run, l_run;
   floatx16_t o[ND];
   auto walk = [&](auto careful) MX_LAMBDA {

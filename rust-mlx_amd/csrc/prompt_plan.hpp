@@ -64,8 +64,9 @@ __device__ __forceinline__ int blocks_of(const Rows& r, int group) {
 }
 
 // How many workgroups share the keys of a query block, with `blocks` of them: as many as bring the
-// launch to what runs at once, each with at least four tiles of the longest possible context; in eights with the kv heads where that is possible, for whole XCDs (512 rows on 12001
-// keys, two kv heads: 8 splits 126 us, 7 splits 138).  At most 64, never more with more blocks.
+// launch to what runs at once, each with at least 256 keys of the longest possible context; in eights with the
+// kv heads where that is possible, for whole XCDs (512 rows on 12001 keys, two kv heads: 8 splits 126 us, 7 splits
+// 138).  At most 64, never more with more blocks.
 template <class Dims>
 __host__ __device__ __forceinline__ int splits_of(int64_t blocks, const Dims& d) {
   const int64_t all = blocks * d.kv_heads, room = longest_context(d) / 256;
@@ -167,7 +168,7 @@ __host__ __device__ __forceinline__ int items_of(int kv_heads, int splits) {
 // Where all workgroups run at once, the second 256 beside the first on the same compute units,
 // those take the blocks from the last one on: a sequence's blocks have fewer and fewer keys, and
 // so a long one shares its unit with a short one (four prompts of up to 2047 rows on up to 3001,
-// e4m3: 144 us against 152).
+// e4m3: 144 us against 152).  Only where two workgroups share a unit, so never of latent prompts.
 template <class Dims>
 __device__ __forceinline__ Item item_of(int id, const PromptPlan& p, int kv_heads) {
   const int pairs = kv_heads * p.splits, a_block = items_of(kv_heads, p.splits);
